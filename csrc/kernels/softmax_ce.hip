@@ -1,0 +1,839 @@
+// Softmax cross entropy of logits z = x W^T + b over V classes, for N rows of D features:
+//   m_n = max_v z_nv,  s_n = sum_v exp(z_nv - m_n),  loss_n = log s_n + (m_n - z_{n, t_n})
+//   dz_nv = g_n (exp(z_nv - m_n) / s_n - [v = t_n]),  dx = dz W,  dW = dz^T x,  db_v = sum_n dz_nv
+// N V logits are never stored.  The forward pass keeps (max, sum of exp) of each row and 256
+// classes; the backward pass goes over the classes in pieces, forms a piece's logits again,
+// stores its dz in the operand type and multiplies it into dx and dW while it is in cache.
+#include "kernels/softmax_ce.h"
+
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+#include <set>
+#include <utility>
+
+#include "kernels/gemm_tile.h"
+#include "runtime/common.h"
+
+namespace oap {
+namespace kern {
+
+namespace {
+
+constexpr int kBM = 256;  // rows of a tile's first operand (classes, or rows in dx)
+
+// exp(d) for d <= 0 (or a little above): v_exp_f32 of d log2(e).  The difference is formed
+// first, in fp32: scaling both terms before it would lose |z| 2^-24 of the exponent.
+__device__ inline float exp_of(float d) {
+  return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+}
+
+// ------------------------------------------------------------------------------ operand images
+// fp32 as three bf16 planes whose sum is the value to 2^-24 (each remainder is exact)
+template <int PLANES, typename T>
+__device__ inline void planes_of(float v, T (&out)[PLANES]) {
+  out[0] = static_cast<T>(v);
+  if constexpr (PLANES == 3) {
+    const float r = v - static_cast<float>(out[0]);
+    out[1] = static_cast<T>(r);
+    out[2] = static_cast<T>(r - static_cast<float>(out[1]));
+  }
+}
+
+// dst[row][plane][dp] = planes of src[row][0..dim), zero beyond dim and in rows that are left
+// out (target == ignore, or bias == -inf): an infinity or NaN there must not meet a coefficient
+// of zero in the gradients' products
+template <typename S, typename T, int PLANES>
+__global__ __launch_bounds__(256) void oap_ce_pack(const S* __restrict__ src, int64_t ld,
+                                                   int64_t rows, int dim, int dp,
+                                                   const int64_t* __restrict__ target,
+                                                   int64_t ignore,
+                                                   const float* __restrict__ bias,
+                                                   T* __restrict__ dst) {
+  const int per = dp / 8;
+  const int64_t total = rows * per;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += int64_t(gridDim.x) * 256) {
+    const int64_t row = i / per;
+    const int c = int(i - row * per) * 8;
+    const bool out = target ? target[row] == ignore : bias && bias[row] == -INFINITY;
+    Vec16<T> o[PLANES];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      T p[PLANES];
+      const bool in = !out && c + j < dim;
+      planes_of<PLANES, T>(in ? static_cast<float>(src[row * ld + c + j]) : 0.f, p);
+#pragma unroll
+      for (int q = 0; q < PLANES; ++q) o[q].v[j] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q)
+      *reinterpret_cast<Vec16<T>*>(dst + (row * PLANES + q) * dp + c) = o[q];
+  }
+}
+
+// ------------------------------------------------------------------------------------ logits
+struct LogitArgs {
+  GtOperand w, x;      // rows: the piece's classes, all rows
+  int64_t dp;          // k extent
+  const float* bias;   // of the piece, or null
+  const int64_t* target;
+  int64_t class0;      // first class of the piece
+  int64_t n;
+  int vtiles, ntiles;
+  // statistics
+  float2* part;        // [class tile][npad]: max, sum of exp(z - max)
+  int64_t npad;
+  float* zt;           // [n] target's logit
+  // gradient
+  const float2* stat;  // [n] the row's (max, sum)
+  const float* coef;   // [n] upstream gradient over its largest magnitude, 0: no loss
+  float pscale;
+  void* dz;            // [npad][PLANES][vp]
+  int64_t vp;
+  float* dbpart;       // [row tile][vp] sums of dz over the tile's rows, or null
+};
+
+// Tile of a workgroup: workgroups go to the 8 XCDs in turn, so each XCD takes a run of
+// consecutive tiles and its L2 sees the same class rows again for every row tile.
+__device__ inline int xcd_tile(int total) {
+  const int b = blockIdx.x, per = total >> 3, rest = total & 7;
+  const int x = b & 7, i = b >> 3;
+  return x * per + (x < rest ? x : rest) + i;
+}
+
+// One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
+// over the tile's classes is mostly within the lane.
+template <typename T, int BN, int WAVES_M, int PLANES, bool GRAD>
+__global__ __launch_bounds__(kGtThreads) void oap_ce_logits(LogitArgs a) {
+  typedef GtTile<T, kBM, kAlongK, BN, kAlongK, WAVES_M, PLANES> Tile;
+  static_assert(BN * kBM * 2 <= Tile::kLds, "the dz tile fits the staging buffers");
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float sbias[kBM];
+  __shared__ float2 smerge[WAVES_M][BN];
+  __shared__ int left_out;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int t = xcd_tile(a.vtiles * a.ntiles);
+  const int vt = t / a.ntiles, nt = t - vt * a.ntiles;
+  const int v0 = vt * kBM, n0 = nt * BN;
+  if (tid == 0) left_out = 0;
+  __syncthreads();
+  if (tid < kBM) {
+    const float b = v0 + tid >= a.w.rows ? -INFINITY : a.bias ? a.bias[v0 + tid] : 0.f;
+    sbias[tid] = b;
+    if (b == -INFINITY) left_out = 1;
+  }
+  gt_f32x16 acc[Tile::MI][Tile::NI];
+  Tile::clear(acc);
+  Tile::run(a.w, a.x, v0, n0, 0, a.dp, lds, acc);
+  const int i0 = Tile::row0(), j0 = Tile::col0();
+  const bool masked = left_out != 0;  // (written before run()'s barriers)
+#pragma unroll
+  for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float b = sbias[i0 + Tile::row_of(mi, e)];
+#pragma unroll
+      for (int ni = 0; ni < Tile::NI; ++ni) {
+        const float z = acc[mi][ni][e] + b;
+        // (a class that is left out has no logit, whatever its weights hold)
+        acc[mi][ni][e] = masked && b == -INFINITY ? -INFINITY : z;
+      }
+    }
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni) {
+    const int j = j0 + 32 * ni;
+    const int64_t n = n0 + j;
+    const int64_t tg = n < a.n ? a.target[n] - a.class0 - v0 - i0 : -1;
+    // the target's offset where it may be one of this lane's classes, else -1
+    const int tgt = tg >= 0 && tg < Tile::WM ? int(tg) : -1;
+    if constexpr (!GRAD) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[mi][ni][e]);
+      float sum = 0.f;
+      const float ref = m > -INFINITY ? m : 0.f;
+#pragma unroll
+      for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += exp_of(acc[mi][ni][e] - ref);
+      if (__ballot(tgt >= 0)) {
+        float zt = 0.f;
+        bool mine = false;
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const bool hit = tgt == Tile::row_of(mi, e);
+            zt = hit ? acc[mi][ni][e] : zt;
+            mine |= hit;
+          }
+        if (mine) a.zt[n] = zt;
+      }
+      const float mo = __shfl_xor(m, 32, 64), so = __shfl_xor(sum, 32, 64);
+      const float mm = fmaxf(m, mo), mr = mm > -INFINITY ? mm : 0.f;
+      // (a part that is -inf throughout has the sum 0; NaN stays in the sums)
+      const float st = sum * exp_of(m - mr) + so * exp_of(mo - mr);
+      if (lane < 32) smerge[Tile::wave_m()][j] = make_float2(mm, st);
+    } else {
+      const float2 st = n < a.n ? a.stat[n] : make_float2(0.f, 0.f);
+      const float c = n < a.n ? a.coef[n] : 0.f;
+      const float cs = st.y == 0.f ? 0.f : c / st.y;
+#pragma unroll
+      for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float z = acc[mi][ni][e];
+          // (a row without a loss has no gradient, whatever its logits are)
+          acc[mi][ni][e] = z == -INFINITY || c == 0.f ? 0.f : exp_of(z - st.x) * cs;
+        }
+      if (__ballot(tgt >= 0)) {
+        const int hit = tgt >= 0 && sbias[i0 + tgt] == -INFINITY ? -1 : tgt;
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            acc[mi][ni][e] -= hit == Tile::row_of(mi, e) ? c : 0.f;
+      }
+    }
+  }
+  if constexpr (!GRAD) {
+    __syncthreads();
+    if (tid < BN) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < WAVES_M; ++k) m = fmaxf(m, smerge[k][tid].x);
+      const float ref = m > -INFINITY ? m : 0.f;
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < WAVES_M; ++k) s += smerge[k][tid].y * exp_of(smerge[k][tid].x - ref);
+      a.part[int64_t(vt) * a.npad + n0 + tid] = make_float2(m, s);
+    }
+  } else {
+    if (a.dbpart) {
+      float* sdb = reinterpret_cast<float*>(lds);  // [wave column][kBM]
+#pragma unroll
+      for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float v = 0.f;
+#pragma unroll
+          for (int ni = 0; ni < Tile::NI; ++ni) v += acc[mi][ni][e];
+#pragma unroll
+          for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+          if ((lane & 31) == 0) sdb[Tile::wave_n() * kBM + i0 + Tile::row_of(mi, e)] = v;
+        }
+      __syncthreads();
+      if (tid < kBM) {
+        float v = 0.f;
+        for (int k = 0; k < Tile::WAVES_N; ++k) v += sdb[k * kBM + tid];
+        a.dbpart[int64_t(nt) * a.vp + v0 + tid] = v;
+      }
+    }
+    // dz through LDS, plane by plane: [row][256 classes], the 16-byte chunk c of row j at slot
+    // c ^ (j & 31), then out in whole rows
+    T* out = static_cast<T*>(a.dz);
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q) {
+      __syncthreads();
+#pragma unroll
+      for (int ni = 0; ni < Tile::NI; ++ni)
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            struct alignas(8) Four {
+              T v[4];
+            } f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // the plane, and in its place what it leaves for the next
+              const float v = acc[mi][ni][4 * g + e] * (q == 0 ? a.pscale : 1.f);
+              f.v[e] = static_cast<T>(v);
+              if (PLANES > 1) acc[mi][ni][4 * g + e] = v - static_cast<float>(f.v[e]);
+            }
+            const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
+            *reinterpret_cast<Four*>(lds + j * (kBM * 2) + (((i >> 3) ^ (j & 31)) << 4) +
+                                     ((i & 4) << 1)) = f;
+          }
+      __syncthreads();
+      for (int c = tid; c < BN * (kBM / 8); c += kGtThreads) {
+        const int j = c >> 5, k = c & 31;
+        *reinterpret_cast<float4*>(out + ((int64_t(n0) + j) * PLANES + q) * a.vp + v0 + k * 8) =
+            *reinterpret_cast<const float4*>(lds + j * (kBM * 2) + ((k ^ (j & 31)) << 4));
+      }
+    }
+  }
+}
+
+// Rows: (max, sum) of every class tile into the row's and the loss, log(sum) + (max - z_t): the
+// difference is formed first, so logits of any size keep the loss's own precision.  A workgroup
+// takes `cols` rows (a power of two) and shares the class tiles of each among its other threads.
+__global__ __launch_bounds__(1024) void oap_ce_rows(const float2* __restrict__ part, int vtiles,
+                                                    int64_t npad, int64_t n, int cols,
+                                                    const int64_t* __restrict__ target,
+                                                    int64_t ignore, int64_t classes,
+                                                    const float* __restrict__ zt,
+                                                    float* __restrict__ loss,
+                                                    float2* __restrict__ stat) {
+  __shared__ float2 red[1024];
+  const int c = threadIdx.x & (cols - 1), r0 = threadIdx.x / cols, nr = 1024 / cols;
+  const int64_t row = int64_t(blockIdx.x) * cols + c;
+  float m = -INFINITY, s = 0.f;
+  if (row < n) {
+    for (int t = r0; t < vtiles; t += nr) {
+      const float2 p = part[int64_t(t) * npad + row];
+      const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
+      s = s * exp_of(m - ref) + p.y * exp_of(p.x - ref);
+      m = mm;
+    }
+  }
+  red[threadIdx.x] = make_float2(m, s);
+  for (int h = nr / 2; h >= 1; h >>= 1) {
+    __syncthreads();
+    if (r0 < h) {
+      const float2 p = red[threadIdx.x + h * cols];
+      const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
+      s = s * exp_of(m - ref) + p.y * exp_of(p.x - ref);
+      m = mm;
+      red[threadIdx.x] = make_float2(m, s);
+    }
+  }
+  if (r0 == 0 && row < n) {
+    stat[row] = make_float2(m, s);
+    const int64_t t = target[row];
+    if (t == ignore)
+      loss[row] = 0.f;
+    else if (t < 0 || t >= classes)
+      loss[row] = NAN;
+    else
+      loss[row] = zt[row] == -INFINITY ? INFINITY : logf(s) + (m - zt[row]);
+  }
+}
+
+// Sum (or mean over the rows that have a loss) in a fixed order, in fp64.
+__global__ __launch_bounds__(1024) void oap_ce_total(const float* __restrict__ loss,
+                                                     const int64_t* __restrict__ target,
+                                                     int64_t ignore, int64_t n, int mean,
+                                                     float* __restrict__ total) {
+  __shared__ double red[1024];
+  __shared__ unsigned long long cnt[1024];
+  double s = 0.0;
+  unsigned long long k = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024)
+    if (target[i] != ignore) {
+      s += double(loss[i]);
+      ++k;
+    }
+  red[threadIdx.x] = s;
+  cnt[threadIdx.x] = k;
+  for (int h = 512; h >= 1; h >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < unsigned(h)) {
+      red[threadIdx.x] += red[threadIdx.x + h];
+      cnt[threadIdx.x] += cnt[threadIdx.x + h];
+    }
+  }
+  if (threadIdx.x == 0) *total = float(mean ? red[0] / double(cnt[0] ? cnt[0] : 1) : red[0]);
+}
+
+// Upstream gradient of every row as g_n = gscale * coef_n with |coef_n| <= 1: products of the
+// coefficient with a probability then fit 16 bits.  Rows without a loss (or with a target that
+// is no class) get the coefficient 0.
+__global__ __launch_bounds__(1024) void oap_ce_coef(const float* __restrict__ grad, int per_row,
+                                                    int mean, const int64_t* __restrict__ target,
+                                                    int64_t ignore, int64_t classes, int64_t n,
+                                                    float* __restrict__ coef,
+                                                    float* __restrict__ gscale) {
+  __shared__ float red[1024];
+  __shared__ unsigned long long cnt[1024];
+  float m = 0.f;
+  unsigned long long k = 0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const int64_t t = target[i];
+    k += t != ignore;
+    if (per_row && t >= 0 && t < classes && t != ignore) {
+      const float g = fabsf(grad[i]);
+      m = g <= m ? m : g;  // (a NaN is kept)
+    }
+  }
+  red[threadIdx.x] = m;
+  cnt[threadIdx.x] = k;
+  for (int h = 512; h >= 1; h >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < unsigned(h)) {
+      const float o = red[threadIdx.x + h];
+      red[threadIdx.x] = o <= red[threadIdx.x] ? red[threadIdx.x] : o;
+      cnt[threadIdx.x] += cnt[threadIdx.x + h];
+    }
+  }
+  __syncthreads();
+  const float top = red[0];
+  if (threadIdx.x == 0)
+    *gscale = per_row ? top : mean ? grad[0] / float(cnt[0] ? cnt[0] : 1) : grad[0];
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const int64_t t = target[i];
+    const bool has = t >= 0 && t < classes && t != ignore;
+    coef[i] = !has ? 0.f : per_row ? (top == 0.f ? 0.f : grad[i] / top) : 1.f;
+  }
+}
+
+// ------------------------------------------------------------------------------------- products
+struct ProdArgs {
+  GtOperand a, b;
+  int64_t k;           // extent, a multiple of 64
+  int64_t m, n;        // valid rows / columns of the result
+  int mtiles, ntiles, splits;
+  void* out;           // dW: [m][n] elements; dx: fp32 slabs [split][m][n]
+  int add;             // dx: add to the slab
+  const float* gscale; // dW
+  float unscale;
+  const float* bias;   // dW: rows of classes that are left out are zero
+};
+
+// dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
+// part to the same elements, so the order of the sums is fixed.
+template <typename T, int BN, int WAVES_M, int PLANES>
+__global__ __launch_bounds__(kGtThreads) void oap_ce_dx(ProdArgs a) {
+  typedef GtTile<T, kBM, kAlongK, BN, kAcrossK, WAVES_M, PLANES> Tile;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int t = xcd_tile(a.mtiles * a.ntiles * a.splits);
+  const int sp = t / (a.mtiles * a.ntiles), u = t - sp * a.mtiles * a.ntiles;
+  const int mt = u / a.ntiles, nt = u - mt * a.ntiles;
+  const int64_t blocks = a.k / kGtK;
+  const int64_t k0 = blocks * sp / a.splits * kGtK, k1 = blocks * (sp + 1) / a.splits * kGtK;
+  gt_f32x16 acc[Tile::MI][Tile::NI];
+  Tile::clear(acc);
+  Tile::run(a.a, a.b, mt * kBM, nt * BN, k0, k1, lds, acc);
+  float* out = static_cast<float*>(a.out) + int64_t(sp) * a.m * a.n;
+  const int64_t i0 = int64_t(mt) * kBM + Tile::row0(), j0 = nt * BN + Tile::col0();
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni)
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t i = i0 + Tile::row_of(mi, e), j = j0 + 32 * ni;
+        if (i < a.m && j < a.n) {
+          float* o = out + i * a.n + j;
+          *o = a.add ? *o + acc[mi][ni][e] : acc[mi][ni][e];
+        }
+      }
+}
+
+template <typename S>
+__global__ __launch_bounds__(256) void oap_ce_dx_out(const float* __restrict__ slab, int splits,
+                                                     int64_t count,
+                                                     const float* __restrict__ gscale,
+                                                     float unscale, S* __restrict__ dx) {
+  const float g = *gscale * unscale;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count;
+       i += int64_t(gridDim.x) * 256) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += slab[int64_t(s) * count + i];
+    dx[i] = static_cast<S>(v * g);
+  }
+}
+
+template <typename S, typename T, int BN, int WAVES_M, int PLANES>
+__global__ __launch_bounds__(kGtThreads) void oap_ce_dw(ProdArgs a) {
+  typedef GtTile<T, kBM, kAcrossK, BN, kAcrossK, WAVES_M, PLANES> Tile;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int t = xcd_tile(a.mtiles * a.ntiles);
+  const int mt = t / a.ntiles, nt = t - mt * a.ntiles;
+  gt_f32x16 acc[Tile::MI][Tile::NI];
+  Tile::clear(acc);
+  Tile::run(a.a, a.b, mt * kBM, nt * BN, 0, a.k, lds, acc);
+  const float g = *a.gscale * a.unscale;
+  S* out = static_cast<S*>(a.out);
+  const int64_t i0 = int64_t(mt) * kBM + Tile::row0(), j0 = nt * BN + Tile::col0();
+#pragma unroll
+  for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t i = i0 + Tile::row_of(mi, e);
+      if (i >= a.m) continue;
+      const bool out_of = a.bias && a.bias[i] == -INFINITY;
+#pragma unroll
+      for (int ni = 0; ni < Tile::NI; ++ni) {
+        const int64_t j = j0 + 32 * ni;
+        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : acc[mi][ni][e] * g);
+      }
+    }
+}
+
+__global__ __launch_bounds__(256) void oap_ce_db(const float* __restrict__ part, int ntiles,
+                                                 int64_t vp, int64_t classes,
+                                                 const float* __restrict__ gscale,
+                                                 float* __restrict__ db) {
+  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (v >= classes) return;
+  float s = 0.f;
+  for (int t = 0; t < ntiles; ++t) s += part[int64_t(t) * vp + v];
+  db[v] = s * *gscale;
+}
+
+template <typename S>
+__global__ __launch_bounds__(256) void oap_ce_fill0(S* __restrict__ p, int64_t count) {
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count;
+       i += int64_t(gridDim.x) * 256)
+    p[i] = S(0.f);
+}
+
+// ------------------------------------------------------------------------------------- planning
+// Operand type and planes of an element type
+template <typename S>
+struct Operand {
+  typedef S T;
+  static constexpr int planes = 1;
+};
+template <>
+struct Operand<float> {
+  typedef __bf16 T;
+  static constexpr int planes = 3;
+};
+
+struct Plan {
+  int planes;
+  int64_t dp;             // dim to a multiple of 64
+  bool x_direct, w_direct;  // the operand is read where it lies
+  int bn;                 // row tile of the logits
+  int64_t npad;
+  int64_t piece;          // classes per piece, a multiple of 256
+  int dbn;                // feature tile of dx and dW
+  int splits;
+};
+
+bool direct(const CeArgs& a, const void* p, int64_t ld) {
+  return a.elem != Elem::F32 && a.dim % kGtK == 0 && ld % 8 == 0 &&
+         reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+
+constexpr int64_t kPieceBytes = int64_t(1) << 29;  // of one dz image or one class image
+
+Plan make_plan(const CeArgs& a, bool grad) {
+  Plan p;
+  p.planes = a.elem == Elem::F32 ? 3 : 1;
+  p.dp = int64_t(round_up(size_t(a.dim), kGtK));
+  // (the gradients read images in which the rows that are left out are zero)
+  p.x_direct = !grad && direct(a, a.x, a.ldx);
+  p.w_direct = direct(a, a.w, a.ldw) && !(grad && a.bias);
+  p.bn = a.n <= 64 ? 64 : 256;
+  p.npad = int64_t(round_up(size_t(a.n), size_t(p.bn)));
+  const int64_t vpad = int64_t(round_up(size_t(a.classes), kBM));
+  int64_t per = p.dp;  // elements per class of the largest image
+  if (grad) per = std::max(per, p.npad);
+  p.piece = kPieceBytes / (per * 2 * p.planes) / kBM * kBM;
+  p.piece = std::max<int64_t>(kBM, std::min(p.piece, vpad));
+  if (!grad && p.w_direct) p.piece = std::min<int64_t>(vpad, int64_t(1) << 22);
+  p.dbn = a.dim <= 128 ? 128 : 256;
+  const int64_t tiles = ceil_div(a.n, kBM) * ceil_div(a.dim, p.dbn);
+  const int64_t by_k = std::max<int64_t>(1, p.piece / 1024);
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>(by_k, 512 / tiles)));
+  return p;
+}
+
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += round_up(count * sizeof(T), 256);
+    return p;
+  }
+};
+
+// More than 64 KiB of LDS is asked for once per kernel and device.
+template <typename F>
+void set_lds(F kernel, int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int device = 0;
+  OAP_HIP_CHECK(hipGetDevice(&device));
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done.emplace(reinterpret_cast<const void*>(kernel), device).second) return;
+  OAP_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+unsigned stride_grid(int64_t threads) {
+  return unsigned(std::max<int64_t>(1, std::min<int64_t>(ceil_div(threads, 256), 8192)));
+}
+
+template <typename S>
+struct Ce {
+  typedef typename Operand<S>::T T;
+  static constexpr int P = Operand<S>::planes;
+
+  static void pack(const S* src, int64_t ld, int64_t rows, int dim, int64_t dp,
+                   const int64_t* target, int64_t ignore, const float* bias, T* dst,
+                   hipStream_t s) {
+    oap_ce_pack<S, T, P><<<stride_grid(rows * dp / 8), 256, 0, s>>>(
+        src, ld, rows, dim, int(dp), target, ignore, bias, dst);
+    OAP_HIP_CHECK(hipGetLastError());
+  }
+
+  static GtOperand image(const T* p, int64_t dp, int64_t rows) {
+    return {p, dp * P, rows, dp, dp};
+  }
+
+  template <bool GRAD>
+  static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
+    const unsigned grid = unsigned(l.vtiles * l.ntiles);
+    if (p.bn == 64) {
+      auto k = oap_ce_logits<T, 64, 4, P, GRAD>;
+      constexpr int lds = GtTile<T, kBM, kAlongK, 64, kAlongK, 4, P>::kLds;
+      set_lds(k, lds);
+      k<<<dim3(grid), kGtThreads, lds, s>>>(l);
+    } else {
+      auto k = oap_ce_logits<T, 256, 2, P, GRAD>;
+      constexpr int lds = GtTile<T, kBM, kAlongK, 256, kAlongK, 2, P>::kLds;
+      set_lds(k, lds);
+      k<<<dim3(grid), kGtThreads, lds, s>>>(l);
+    }
+    OAP_HIP_CHECK(hipGetLastError());
+  }
+
+  struct Work {
+    T *ximg, *wimg, *dz;
+    float2* part;
+    float *zt, *coef, *gscale, *slab, *dbpart;
+  };
+
+  static size_t carve_forward(const CeArgs& a, const Plan& p, void* base, Work& w) {
+    Carver c{static_cast<char*>(base)};
+    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp * P);
+    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp * P);
+    w.part = c.take<float2>(size_t(ceil_div(a.classes, kBM)) * p.npad);
+    w.zt = c.take<float>(a.n);
+    return c.used;
+  }
+
+  static size_t carve_backward(const CeArgs& a, const Plan& p, void* base, bool dx, bool dw,
+                               bool db, Work& w) {
+    Carver c{static_cast<char*>(base)};
+    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp * P);
+    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp * P);
+    w.coef = c.take<float>(a.n);
+    w.gscale = c.take<float>(1);
+    w.dz = c.take<T>(size_t(p.npad) * P * p.piece);
+    w.slab = dx ? c.take<float>(size_t(p.splits) * a.n * a.dim) : nullptr;
+    w.dbpart = db ? c.take<float>(size_t(p.npad / p.bn) * p.piece) : nullptr;
+    return c.used;
+  }
+
+  static void forward(const CeArgs& a, float* loss, float2* stat, float* total, bool mean,
+                      void* work, hipStream_t s) {
+    const Plan p = make_plan(a, false);
+    Work w;
+    carve_forward(a, p, work, w);
+    const S* x = static_cast<const S*>(a.x);
+    const S* wt = static_cast<const S*>(a.w);
+    LogitArgs l = {};
+    l.x = {a.x, a.ldx, a.n, p.dp, 0};
+    if (!p.x_direct) {
+      pack(x, a.ldx, a.n, a.dim, p.dp, nullptr, 0, nullptr, w.ximg, s);
+      l.x = image(w.ximg, p.dp, a.n);
+    }
+    l.dp = p.dp;
+    l.target = a.target;
+    l.n = a.n;
+    l.ntiles = int(p.npad / p.bn);
+    l.npad = p.npad;
+    l.zt = w.zt;
+    for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
+      const int64_t nc = std::min(p.piece, a.classes - c0);
+      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp, 0};
+      if (!p.w_direct) {
+        pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, nullptr, w.wimg, s);
+        l.w = image(w.wimg, p.dp, nc);
+      }
+      l.bias = a.bias ? a.bias + c0 : nullptr;
+      l.class0 = c0;
+      l.vtiles = int(ceil_div(nc, kBM));
+      l.part = w.part + c0 / kBM * p.npad;
+      logits<false>(p, l, s);
+    }
+    const int vtiles = int(ceil_div(a.classes, kBM));
+    int cols = 1;
+    while (cols < 64 && cols < a.n) cols *= 2;
+    oap_ce_rows<<<dim3(unsigned(ceil_div(a.n, cols))), 1024, 0, s>>>(
+        w.part, vtiles, p.npad, a.n, cols, a.target, a.ignore, a.classes, w.zt, loss, stat);
+    OAP_HIP_CHECK(hipGetLastError());
+    if (total) {
+      oap_ce_total<<<1, 1024, 0, s>>>(loss, a.target, a.ignore, a.n, mean, total);
+      OAP_HIP_CHECK(hipGetLastError());
+    }
+  }
+
+  template <int BN, int WAVES_M>
+  static void products(const CeArgs& a, const Plan& p, const Work& w, const LogitArgs& l,
+                       int64_t nc, int64_t c0, float unscale, void* dx, void* dw,
+                       hipStream_t s) {
+    constexpr int lds = GtTile<T, kBM, kAcrossK, BN, kAcrossK, WAVES_M, P>::kLds;
+    ProdArgs g = {};
+    g.ntiles = int(ceil_div(a.dim, BN));
+    g.n = a.dim;
+    g.gscale = w.gscale;
+    g.unscale = unscale;
+    const int64_t ncp = int64_t(round_up(size_t(nc), kGtK));
+    if (dx) {
+      auto k = oap_ce_dx<T, BN, WAVES_M, P>;
+      set_lds(k, lds);
+      g.a = image(w.dz, p.piece, p.npad);
+      g.b = l.w;
+      g.k = ncp;
+      g.m = a.n;
+      g.mtiles = int(ceil_div(a.n, kBM));
+      g.splits = p.splits;
+      g.out = w.slab;
+      g.add = c0 > 0;
+      k<<<dim3(unsigned(g.mtiles * g.ntiles * g.splits)), kGtThreads, lds, s>>>(g);
+      OAP_HIP_CHECK(hipGetLastError());
+    }
+    if (dw) {
+      auto k = oap_ce_dw<S, T, BN, WAVES_M, P>;
+      set_lds(k, lds);
+      g.a = image(w.dz, p.piece, p.npad);
+      g.b = l.x;
+      g.k = int64_t(round_up(size_t(a.n), kGtK));
+      g.m = nc;
+      g.mtiles = int(ceil_div(nc, kBM));
+      g.out = static_cast<S*>(dw) + c0 * a.dim;
+      g.bias = a.bias ? a.bias + c0 : nullptr;
+      k<<<dim3(unsigned(g.mtiles * g.ntiles)), kGtThreads, lds, s>>>(g);
+      OAP_HIP_CHECK(hipGetLastError());
+    }
+  }
+
+  static void backward(const CeArgs& a, const float2* stat, const float* grad, bool per_row,
+                       bool mean, void* dx, void* dw, float* db, void* work, hipStream_t s) {
+    const Plan p = make_plan(a, true);
+    Work w;
+    carve_backward(a, p, work, dx, dw, db, w);
+    const S* x = static_cast<const S*>(a.x);
+    const S* wt = static_cast<const S*>(a.w);
+    // fp16 images hold dz times 2^14: |dz| <= 1 stays finite and 2^-28 is still a normal number
+    const float pscale = a.elem == Elem::F16 ? 0x1p14f : 1.f;
+    oap_ce_coef<<<1, 1024, 0, s>>>(grad, per_row, mean, a.target, a.ignore, a.classes, a.n,
+                                   w.coef, w.gscale);
+    OAP_HIP_CHECK(hipGetLastError());
+    LogitArgs l = {};
+    l.x = {a.x, a.ldx, a.n, p.dp, 0};
+    if (!p.x_direct) {
+      pack(x, a.ldx, a.n, a.dim, p.dp, a.target, a.ignore, nullptr, w.ximg, s);
+      l.x = image(w.ximg, p.dp, a.n);
+    }
+    l.dp = p.dp;
+    l.target = a.target;
+    l.n = a.n;
+    l.ntiles = int(p.npad / p.bn);
+    l.npad = p.npad;
+    l.stat = stat;
+    l.coef = w.coef;
+    l.pscale = pscale;
+    l.dz = w.dz;
+    l.vp = p.piece;
+    l.dbpart = w.dbpart;
+    for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
+      const int64_t nc = std::min(p.piece, a.classes - c0);
+      const float* bias = a.bias ? a.bias + c0 : nullptr;
+      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp, 0};
+      if (!p.w_direct) {
+        pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, bias, w.wimg, s);
+        l.w = image(w.wimg, p.dp, nc);
+      }
+      l.bias = bias;
+      l.class0 = c0;
+      l.vtiles = int(ceil_div(nc, kBM));
+      logits<true>(p, l, s);
+      if (p.dbn == 128)
+        products<128, 4>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      else
+        products<256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      if (db) {
+        oap_ce_db<<<dim3(unsigned(ceil_div(nc, 256))), 256, 0, s>>>(w.dbpart, l.ntiles, p.piece,
+                                                                     nc, w.gscale, db + c0);
+        OAP_HIP_CHECK(hipGetLastError());
+      }
+    }
+    if (dx) {
+      oap_ce_dx_out<S><<<stride_grid(a.n * a.dim), 256, 0, s>>>(
+          w.slab, p.splits, a.n * a.dim, w.gscale, 1.f / pscale, static_cast<S*>(dx));
+      OAP_HIP_CHECK(hipGetLastError());
+    }
+  }
+
+  static void zeros(const CeArgs& a, void* dx, void* dw, float* db, hipStream_t s) {
+    const int64_t nx = a.n * a.dim, nw = a.classes * a.dim;
+    if (dx && nx) oap_ce_fill0<S><<<stride_grid(nx), 256, 0, s>>>(static_cast<S*>(dx), nx);
+    if (dw && nw) oap_ce_fill0<S><<<stride_grid(nw), 256, 0, s>>>(static_cast<S*>(dw), nw);
+    if (db && a.classes)
+      oap_ce_fill0<float><<<stride_grid(a.classes), 256, 0, s>>>(db, a.classes);
+    OAP_HIP_CHECK(hipGetLastError());
+  }
+};
+
+void check(const CeArgs& a) {
+  OAP_CHECK(a.n >= 0 && a.n < (int64_t(1) << 31) - kBM && a.classes >= 1 &&
+                a.classes < (int64_t(1) << 31) - kBM && a.dim >= 1 && a.dim <= (1 << 20) &&
+                a.ldx >= a.dim && a.ldw >= a.dim,
+            "softmax_cross_entropy: bad shape");
+  OAP_CHECK(ceil_div(a.n, 64) * ceil_div(a.classes, kBM) < (int64_t(1) << 31),
+            "softmax_cross_entropy: " << a.n << " x " << a.classes << " tiles are too many");
+}
+
+}  // namespace
+
+size_t ce_forward_bytes(const CeArgs& a) {
+  check(a);
+  if (a.n == 0) return 0;
+  size_t r = 0;
+  elem_dispatch(a.elem, [&](auto t) {
+    typename Ce<decltype(t)>::Work w;
+    r = Ce<decltype(t)>::carve_forward(a, make_plan(a, false), nullptr, w);
+  });
+  return r;
+}
+
+void ce_forward(const CeArgs& a, float* loss, float2* stat, float* total, bool mean, void* work,
+                hipStream_t s) {
+  check(a);
+  if (a.n == 0) {  // no row: the sum and the mean are 0
+    if (total) oap_ce_fill0<float><<<1, 256, 0, s>>>(total, 1);
+    OAP_HIP_CHECK(hipGetLastError());
+    return;
+  }
+  elem_dispatch(a.elem, [&](auto t) {
+    Ce<decltype(t)>::forward(a, loss, stat, total, mean, work, s);
+  });
+}
+
+size_t ce_backward_bytes(const CeArgs& a, bool want_dx, bool want_dw, bool want_db) {
+  check(a);
+  if (a.n == 0) return 0;
+  size_t r = 0;
+  elem_dispatch(a.elem, [&](auto t) {
+    typename Ce<decltype(t)>::Work w;
+    r = Ce<decltype(t)>::carve_backward(a, make_plan(a, true), nullptr, want_dx, want_dw, want_db,
+                                        w);
+  });
+  return r;
+}
+
+void ce_backward(const CeArgs& a, const float2* stat, const float* grad, bool per_row, bool mean,
+                 void* dx, void* dw, float* db, void* work, hipStream_t s) {
+  check(a);
+  elem_dispatch(a.elem, [&](auto t) {
+    if (a.n == 0)
+      Ce<decltype(t)>::zeros(a, dx, dw, db, s);
+    else
+      Ce<decltype(t)>::backward(a, stat, grad, per_row, mean, dx, dw, db, work, s);
+  });
+}
+
+}  // namespace kern
+}  // namespace oap

@@ -1,25 +1,34 @@
 """Array-level ops on torch tensors: the MI355X kernels without the Spark-style estimator layer.
 
 GPU tensors are used in place (zero-copy table views over ``tensor.data_ptr()``; a padded copy is
-made only when the row stride does not match the kernel layout), outputs are device tensors, and
-every op orders itself after torch's current stream and finishes its own stream before returning.
-CPU tensors (or a process without a GPU world) go through the native CPU engine.  All ops run on
-the process world (``oap_mllib_amd.init_world``): with several ranks, every rank passes its own
-row shard and collective ops (``kmeans_fit``, ``pca``) return the global result on every rank.
+made only when the row stride does not match the kernel layout), outputs are device tensors.
+``kmeans_assign``, ``kmeans_fit`` and ``pca`` order themselves after torch's current stream and
+finish their own stream before returning; CPU tensors (or a process without a GPU world) go
+through the native CPU engine. They run on the process world (``oap_mllib_amd.init_world``): with
+several ranks, every rank passes its own row shard and collective ops (``kmeans_fit``, ``pca``)
+return the global result on every rank.
 
     import torch, oap_mllib_amd.ops as ops
     x = torch.randn(10_000_000, 50, device="cuda")
     centers, cost, iters = ops.kmeans_fit(x, k=200)
     labels, dist2 = ops.kmeans_assign(x, centers)     # int32 / float32 tensors on x.device
     pc, explained = ops.pca(x, k=10)
+
+The training ops (:mod:`oap_mllib_amd.ops.training`) are differentiable, need no world and run on
+torch's current stream without a synchronisation:
+
+    h = ops.dropout(x, 0.1, seed=step)                          # mask from a counter, not stored
+    weights, experts, counts = ops.route(h @ gate, k=2)         # top-k gate of a mixture
+    loss = ops.softmax_cross_entropy(h, item_factors, target)   # logits are never stored
 """
 from __future__ import annotations
 
 import numpy as np
 
 from .. import _loader
+from .training import dropout, route, softmax_cross_entropy
 
-__all__ = ["kmeans_assign", "kmeans_fit", "pca"]
+__all__ = ["dropout", "kmeans_assign", "kmeans_fit", "pca", "route", "softmax_cross_entropy"]
 
 
 def _torch():

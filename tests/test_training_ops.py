@@ -1,0 +1,638 @@
+"""oap_mllib_amd.ops training ops (softmax_cross_entropy, dropout, route) against plain 64-bit
+implementations: every case runs on the host engine and, marked gpu, on the kernels.
+
+Tolerances follow the arithmetic: u is half a step of the element type (relative), fp32 sums of n
+terms are off by at most n 2^-23 of the sum of the terms' magnitudes (the matrix units may
+truncate), and a result is rounded once to its type."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oap_mllib_amd import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+E32 = 2.0 ** -23
+INF = math.inf
+
+
+def half_step(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def rand(shape, seed, dtype=torch.float32, device="cpu", scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(device)
+
+
+def cpu64(t):
+    return t.detach().cpu().double()
+
+
+def check(got, ref, tol, what):
+    got = cpu64(got)
+    assert got.shape == ref.shape, (what, got.shape, ref.shape)
+    same = (got == ref) | (got.isnan() & ref.isnan())
+    bad = ~same & ~((got - ref).abs() <= tol)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:4], ref[bad][:4],
+                           torch.as_tensor(tol).expand_as(ref)[bad][:4])
+
+
+# --------------------------------------------------------------------- softmax cross entropy
+def ce_oracle(x, w, t, b, up, ignore=-100):
+    """64-bit losses, gradients (for the upstream row gradients `up`) and the bounds of their
+    errors per unit of relative error of dz."""
+    x, w, t = cpu64(x), cpu64(w), t.cpu().long()
+    n, v = len(x), len(w)
+    out = torch.zeros(v, dtype=torch.bool) if b is None else cpu64(b) == -INF
+    x = torch.where((t == ignore)[:, None], torch.zeros_like(x), x)
+    w = torch.where(out[:, None], torch.zeros_like(w), w)
+    bias = torch.zeros(v).double() if b is None else cpu64(b)
+    z = x @ w.t() + bias
+    lse = torch.logsumexp(z, dim=1)
+    p = torch.where(out, torch.zeros_like(z), (z - lse[:, None]).exp())
+    valid = (t >= 0) & (t < v) & (t != ignore)
+    tt = torch.where(valid, t, torch.zeros_like(t))
+    zt = z.gather(1, tt[:, None])[:, 0]
+    loss = torch.where(zt == -INF, torch.full_like(zt, INF), lse - zt)
+    loss = torch.where(t == ignore, torch.zeros_like(loss),
+                       torch.where(valid, loss, torch.full_like(loss, math.nan)))
+    hot = torch.zeros_like(p)
+    hot[torch.arange(n), tt] = (valid & ~out[tt]).double()
+    u = torch.where(valid, cpu64(up).expand(n), torch.zeros(n).double())
+    dz = u[:, None] * (p - hot)
+    mag = u.abs()[:, None] * (p + hot)
+    # largest error of a logit, and of the sums
+    absz = (x.abs() @ w.abs().t()).max().item() if n and v else 0.0
+    fin = bias[bias > -INF]
+    bmax = fin.abs().max().item() if len(fin) else 0.0
+    zerr = (x.shape[1] + 8) * E32 * absz + 2 * E32 * (absz + bmax)
+    return {"loss": loss, "dx": dz @ w, "dw": dz.t() @ x, "db": dz.sum(0), "zerr": zerr,
+            "mdx": mag @ w.abs(), "mdw": mag.t() @ x.abs(), "mdb": mag.sum(0), "lse": lse}
+
+
+def ce_check(x, w, t, b, reduction="mean", up=None, ignore=-100, want=(True, True, True)):
+    leaves = [None if o is None else o.detach().requires_grad_(q)  # (the strides of a view)
+              for o, q in zip((x, w, b), want)]
+    n = len(x)
+    count = max(1, int((t != ignore).sum()))
+    loss = ops.softmax_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2],
+                                     ignore_index=ignore, reduction=reduction)
+    if reduction == "none":
+        rows = up if up is not None else torch.ones(n, device=x.device)
+    else:
+        rows = torch.full((n,), 1.0 / count if reduction == "mean" else 1.0)
+    ref = ce_oracle(x, w, t, b, rows, ignore)
+    u = half_step(x.dtype)
+    # (inf - inf of an excluded or infinite row compares equal in check)
+    ltol = 2 * ref["zerr"] + 4 * E32 * (ref["lse"].nan_to_num(0, 0, 0).abs() + 1)
+    if reduction == "none":
+        check(loss, ref["loss"], ltol, "loss")
+    else:
+        kept = ref["loss"][t.cpu() != ignore]
+        total = kept.sum() / (count if reduction == "mean" else 1)
+        scale = kept.nan_to_num(0, 0, 0).abs().sum() / (count if reduction == "mean" else 1)
+        tol = ltol.max() * (1 if reduction == "mean" else n) + 2 * E32 * scale
+        check(loss, total, tol, "total")
+    assert loss.dtype == torch.float32
+    use = [(k, v) for k, v in zip(("dx", "dw", "db"), leaves) if v is not None and v.requires_grad]
+    if not use:
+        return
+    grads = torch.autograd.grad(loss, [v for _, v in use],
+                                rows.to(loss.device) if reduction == "none" else None)
+    top = rows.abs().max().item() if n else 0.0
+    for (name, leaf), g in zip(use, grads):
+        assert g.dtype == leaf.dtype and g.shape == leaf.shape
+        terms = {"dx": len(w), "dw": n, "db": n}[name]
+        # dz: logits, lse and exp in fp32; rounded to the operand type unless summed for db
+        rel = 2 * ref["zerr"] + 16 * E32 + (0 if name == "db" else u) + (terms + 8) * E32
+        uo = half_step(leaf.dtype)
+        # fp16: dz below 2^-28 of the largest upstream gradient and results below the normal
+        # range lose bits
+        small = 2.0 ** -38 * top * (terms * float(cpu64(w if name == "dx" else x)
+                                                  .nan_to_num(0, 0, 0).abs().amax())
+                                    if terms and x.numel() and w.numel() else 1.0)
+        tiny = (small + 2.0 ** -24 if leaf.dtype == torch.float16 else 1e-37)
+        check(g, ref[name], ref["m" + name] * (rel + uo) + uo * ref[name].abs() + tiny, name)
+
+
+CE_SIZES = [(1, 1, 1), (1, 2, 3), (3, 5, 8), (5, 7, 13), (2, 300, 64), (64, 255, 64),
+            (65, 257, 100), (130, 1000, 128), (257, 513, 200), (70, 2050, 65), (33, 40, 513)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", CE_SIZES)
+def test_ce_sizes(device, dtype, n, v, d):
+    x = rand((n, d), 1, dtype, device)
+    w = rand((v, d), 2, dtype, device, 2 / math.sqrt(d))
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).to(device)
+    t[::4] = -100
+    b = rand((v,), 4, torch.float32, device)
+    ce_check(x, w, t, b)
+    ce_check(x, w, t, None, "sum")
+    up = rand((n,), 5, torch.float32, device)
+    ce_check(x, w, t, b, "none", up)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ce_left_out_rows_and_classes(device, dtype):
+    """Ignored rows and classes with bias -inf may hold anything; an excluded or invalid target
+    gives inf or NaN and touches no other row."""
+    n, v, d = 70, 300, 64
+    x, w = rand((n, d), 1, dtype, device), rand((v, d), 2, dtype, device, 0.3)
+    t = torch.arange(n, device=device) % v
+    t[5:20] = -100
+    x[6], x[7, 3], x[8, 0] = math.nan, INF, -INF
+    b = rand((v,), 3, torch.float32, device)
+    b[100:200:3] = -INF
+    w[100], w[103, 1], w[106, 2] = math.nan, INF, -INF
+    ce_check(x, w, t, b)
+    t[30], t[31], t[32] = 100, v, -7  # excluded target; two that are no class
+    ones = torch.ones(n, device=device)
+    ce_check(x, w, t, b, "none", ones)
+    loss = ops.softmax_cross_entropy(x, w, t, b, reduction="none").cpu()
+    assert loss[30] == INF and loss[31].isnan() and loss[32].isnan()
+    assert loss.isfinite().sum() == n - 3
+    assert ops.softmax_cross_entropy(x, w, t, b).isnan()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ce_nothing_left(device):
+    n, v, d = 10, 20, 16
+    for dtype in DTYPES:
+        x = rand((n, d), 1, dtype, device).requires_grad_()
+        w = rand((v, d), 2, dtype, device).requires_grad_()
+        t = torch.full((n,), -100, device=device)
+        loss = ops.softmax_cross_entropy(x, w, t)
+        gx, gw = torch.autograd.grad(loss, [x, w])
+        assert loss.item() == 0 and not gx.any() and not gw.any()
+        # every class left out
+        b = torch.full((v,), -INF, device=device)
+        t = torch.arange(n, device=device)
+        loss = ops.softmax_cross_entropy(x, w, t, b, reduction="none")
+        gx, gw = torch.autograd.grad(loss, [x, w], torch.ones_like(loss))
+        assert (loss == INF).all() and not gx.any() and not gw.any()
+        # the type's lowest value is a bias like any other: the softmax is flat
+        b = torch.full((v,), torch.finfo(torch.float32).min, device=device)
+        loss = ops.softmax_cross_entropy(x, w, t, b, reduction="none")
+        check(loss, torch.full((n,), math.log(v)).double(), 64 * E32 * math.log(v) + 1e-5,
+              "lowest")
+        # no row
+        loss = ops.softmax_cross_entropy(x[:0], w, t[:0])
+        gw, = torch.autograd.grad(loss, [w])
+        assert loss.item() == 0 and not gw.any() and gw.shape == w.shape
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ce_strides_and_types(device, dtype):
+    n, v, d = 40, 130, 64
+    wide = rand((n, d + 9), 1, dtype, device)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).to(device)
+    w = rand((v, d), 2, dtype, device, 0.3)
+    for x in (wide[:, 1:d + 1], wide[:, 8:d + 8], rand((d, n), 4, dtype, device).t(),
+              rand((1, d), 5, dtype, device).expand(n, d), rand((2 * n, d), 6, dtype, device)[::2]):
+        ce_check(x, w, t, None)
+    ce_check(wide[:, :d], rand((d, v), 7, dtype, device).t(), t.int(),
+             rand((v,), 8, torch.bfloat16, device))
+    tt = torch.stack([t, t], 1)[:, 0]  # a strided target
+    ce_check(wide[:, :d], w, tt, None, "sum", want=(True, False, False))
+    ce_check(wide[:, :d], w, tt, None, "sum", want=(False, True, False))
+    ce_check(wide[:, :d], w, tt, rand((v,), 9, torch.float32, device), want=(False, False, True))
+    t0 = torch.where(t % 3 == 0, torch.zeros_like(t), t)
+    ce_check(wide[:, :d], w, t0, None, ignore=0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ce_gradient_against_differences(device):
+    n, v, d = 6, 50, 20
+    x, w, b = rand((n, d), 1), rand((v, d), 2), rand((v,), 3)
+    t = torch.tensor([3, 3, -100, 49, 0, 7])
+    up = torch.rand(n, generator=torch.Generator().manual_seed(4)) + 0.5
+    leaves = [q.to(device).requires_grad_() for q in (x, w, b)]
+    loss = ops.softmax_cross_entropy(*leaves[:2], t.to(device), leaves[2], reduction="none")
+    grads = torch.autograd.grad(loss, leaves, up.to(device))
+
+    def f(h, dirs):
+        xs = [q.double() + h * r for q, r in zip((x, w, b), dirs)]
+        z = xs[0] @ xs[1].t() + xs[2]
+        rows = torch.logsumexp(z, 1) - z.gather(1, t.clamp(min=0)[:, None])[:, 0]
+        return (rows * up.double() * (t != -100)).sum()
+
+    for seed in range(5):
+        dirs = [rand(q.shape, 10 + seed).double() for q in (x, w, b)]
+        h = 1e-4
+        diff = (f(h, dirs) - f(-h, dirs)) / (2 * h)
+        got = sum((cpu64(g) * r).sum() for g, r in zip(grads, dirs))
+        size = sum((cpu64(g).abs() * r.abs()).sum() for g, r in zip(grads, dirs))
+        # h^2 / 6 of a third derivative of at most a few |z'|^3 (|z'| below 60 here): below
+        # 1e-8 / 6 * 2 * 60^3 * n; the gradients' own error: (d + v + 30) 2^-23
+        assert abs(diff - got) <= 1e-8 / 6 * 2 * 60 ** 3 * n + (d + v + 30) * E32 * size
+
+
+def test_ce_refusals():
+    x, w, t = rand((4, 8), 1), rand((9, 8), 2), torch.zeros(4, dtype=torch.int64)
+    f = ops.softmax_cross_entropy
+    for bad in [lambda: f(x[0], w, t), lambda: f(x, w[0], t), lambda: f(x, w[:, :5], t),
+                lambda: f(x, w.half(), t), lambda: f(x.double(), w.double(), t),
+                lambda: f(x, w, t[:3]), lambda: f(x, w, t.float()), lambda: f(x, w, t, x[:, 0]),
+                lambda: f(x, w, t, torch.zeros(9, dtype=torch.int64)),
+                lambda: f(x, w, t, reduction="avg"), lambda: f(x[:, :0], w[:, :0], t),
+                lambda: f(x, w[:0], t), lambda: f([1], w, t), lambda: f(x, w, [0] * 4),
+                lambda: f(x, w.to("meta"), t), lambda: f(x.to("meta"), w, t)]:
+        with pytest.raises(ValueError):
+            bad()
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(f(leaf, w, t), [leaf], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), [leaf])
+
+
+@pytest.mark.gpu
+def test_ce_pieces_gpu():
+    """Classes in more than one piece, and a row count whose tiles span several workgroups."""
+    for dtype, n, v, d, bias in [(torch.bfloat16, 8190, 40_001, 64, False),
+                                 (torch.float32, 2000, 50_003, 5, True)]:
+        g = torch.Generator(device="cuda").manual_seed(1)
+        x = torch.randn(n, d, generator=g, device="cuda").to(dtype).requires_grad_()
+        w = (torch.randn(v, d, generator=g, device="cuda") * 0.3).to(dtype).requires_grad_()
+        b = torch.randn(v, generator=g, device="cuda").requires_grad_() if bias else None
+        t = torch.randint(0, v, (n,), generator=g, device="cuda")
+        leaves = [x, w] + ([b] if bias else [])
+        loss = ops.softmax_cross_entropy(x, w, t, b)
+        grads = torch.autograd.grad(loss, leaves)
+        xd, wd = x.detach().double(), w.detach().double()
+        z = xd @ wd.t() + (b.detach().double() if bias else 0)
+        p = torch.softmax(z, 1)
+        ref = -p.gather(1, t[:, None]).log().mean()
+        p.scatter_add_(1, t[:, None], -torch.ones_like(p[:, :1]))
+        p /= n
+        u = half_step(dtype)
+        assert abs(loss.item() - ref.item()) <= 1e-5 * abs(ref.item())
+        for got, want, mag in [(grads[0], p @ wd, p.abs() @ wd.abs()),
+                               (grads[1], p.t() @ xd, p.abs().t() @ xd.abs())] + \
+                ([(grads[2], p.sum(0), p.abs().sum(0))] if bias else []):
+            # sums over blocks: at most 2^16 terms in one fp32 run
+            tol = mag * (u + 2e-5 + 256 * E32) + u * want.abs() + 1e-30
+            err = (got.double() - want).abs()
+            assert (err <= tol).all(), (dtype, (err / tol).max())
+
+
+# ----------------------------------------------------------------------------------- dropout
+def philox_words(count, offset, seed):
+    """Words of elements offset .. offset + count - 1, in plain integers."""
+    out = []
+    for i in range(offset, offset + count):
+        c = [(i >> 2) & 0xFFFFFFFF, i >> 34, 0, 0]
+        k = [seed & 0xFFFFFFFF, seed >> 32]
+        for _ in range(10):
+            a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+            c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+            k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+        out.append(c[i & 3])
+    return out
+
+
+def test_philox_known_answer():
+    # the generator's published answers for a counter and key of zeros
+    assert philox_words(4, 0, 0) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    ones = torch.ones(4)
+    for i, w in enumerate(philox_words(4, 0, 0)):
+        p = w / 2 ** 32  # kept at the threshold itself, dropped just above
+        assert ops.dropout(ones, p, 0)[i] != 0
+        assert ops.dropout(ones, (w + 1) / 2 ** 32, 0)[i] == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,offset", [(1, 0), (3, 5), (8, 4), (9, 8), (1001, 3), (1001, 1 << 35),
+                                      (4111, (1 << 40) + 2), (70, (1 << 64) - 70)])
+def test_dropout(device, dtype, n, offset):
+    seed = 0xFEDCBA9876543210 + n
+    x, res, g = (rand((n,), i, dtype, device) for i in range(3))
+    words = torch.tensor(philox_words(n, offset, seed))
+    u = half_step(dtype)
+    for p in (0.0, 0.3, 0.875, 1.0):
+        keep = (words >= round(p * 2 ** 32)).double()
+        f = keep / (1 - p) if p < 1 else keep * 0
+        for r in (None, res):
+            xl, rl = x.clone().requires_grad_(), res.clone().requires_grad_()
+            y = ops.dropout(xl, p, seed, offset=offset, residual=rl if r is not None else None)
+            ref = cpu64(x) * f + (cpu64(res) if r is not None else 0)
+            tol = 2 * E32 * (cpu64(x) * f).abs() + (u + E32) * ref.abs() + 2.0 ** -25
+            check(y, ref, tol if dtype == torch.float16 else tol - 2.0 ** -25 + 1e-38, "y")
+            assert ((y.cpu() == 0) | (keep > 0)).all() or r is not None
+            grads = torch.autograd.grad(y, [xl] + ([rl] if r is not None else []), g)
+            check(grads[0], cpu64(g) * f, (2 * E32 + u) * (cpu64(g) * f).abs() + 2.0 ** -25, "dx")
+            if r is not None:
+                assert torch.equal(grads[1], g)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_dropout_places_and_shapes(device):
+    x = rand((6, 50, 7), 1, torch.float32, device)
+    x[0, :10] = math.nan
+    x[1, :10] = INF
+    y = ops.dropout(x, 0.5, 7)
+    keep = (torch.tensor(philox_words(x.numel(), 0, 7)) >= 1 << 31).view(x.shape)
+    assert not y.cpu()[~keep].any() and y.cpu()[0, :10][keep[0, :10]].isnan().all()
+    assert not ops.dropout(x, 1.0, 7).any()
+    # a shard draws what the whole table draws; so do views, an unaligned one among them
+    assert torch.equal(ops.dropout(x[2:], 0.5, 7, offset=2 * 350), y[2:])
+    flat = rand((2001,), 2, torch.bfloat16, device)
+    assert torch.equal(ops.dropout(flat[1:], 0.5, 9), ops.dropout(flat[1:].clone(), 0.5, 9))
+    z = rand((30, 40), 3, torch.float32, device)
+    assert torch.equal(ops.dropout(z.t(), 0.5, 9), ops.dropout(z.t().contiguous(), 0.5, 9))
+    zl = z.clone().requires_grad_()
+    g, = torch.autograd.grad(ops.dropout(zl, 0.25, 9).sum(), [zl])  # (an expanded gradient)
+    assert torch.equal(g, ops.dropout(torch.ones_like(z), 0.25, 9))
+    seed = torch.tensor([9], device=device)
+    assert torch.equal(ops.dropout(z, 0.25, seed), ops.dropout(z, 0.25, 9))
+    assert torch.equal(ops.dropout(z, 0.25, -1), ops.dropout(z, 0.25, (1 << 64) - 1))
+    y = ops.dropout(zl, 0.25, seed)
+    seed += 1
+    with pytest.raises(RuntimeError):  # (the mask of the gradient would be another)
+        torch.autograd.grad(y.sum(), [zl])
+    assert ops.dropout(z[:0], 0.25, 9).shape == (0, 40)
+    many = ops.dropout(torch.ones(1 << 20, device=device), 0.1, 5)
+    # binomial: six standard deviations of 2^20 draws
+    assert abs((many == 0).double().mean().item() - 0.1) < 6 * math.sqrt(0.09 / 2 ** 20)
+
+
+def test_dropout_refusals():
+    x = torch.ones(8)
+    for bad in [lambda: ops.dropout(x, -0.1, 1), lambda: ops.dropout(x, 1.1, 1),
+                lambda: ops.dropout(x, math.nan, 1), lambda: ops.dropout(x.double(), 0.1, 1),
+                lambda: ops.dropout(x.long(), 0.1, 1), lambda: ops.dropout(x, 0.1, 1 << 64),
+                lambda: ops.dropout(x, 0.1, 1, offset=-4),
+                lambda: ops.dropout(x, 0.1, 1, offset=(1 << 64) - 7),
+                lambda: ops.dropout(x, 0.1, 1, residual=x[:4]),
+                lambda: ops.dropout(x, 0.1, 1, residual=x.half()),
+                lambda: ops.dropout(x, 0.1, torch.tensor([1, 2])),
+                lambda: ops.dropout(x, 0.1, torch.tensor([1.0])),
+                lambda: ops.dropout(x, 0.1, torch.ones(1, dtype=torch.int64, device="meta")),
+                lambda: ops.dropout([1.0], 0.1, 1)]:
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ------------------------------------------------------------------------------------- route
+def route_oracle(z, k, score, bias, groups, top, renorm, scale, g):
+    """Plain 64-bit gate: weights, indices, counts and the logits' gradient."""
+    z = cpu64(z).numpy()
+    t, e = z.shape
+    w, idx = np.zeros((t, k)), np.full((t, k), -1)
+    dz = np.zeros((t, e))
+    per = e // groups
+    b = np.zeros(e) if bias is None else cpu64(bias).numpy()
+    for i in range(t):
+        zi = np.where(np.isnan(z[i]), -INF, z[i])
+        m = zi.max()
+        if score == "softmax":
+            s = np.where(zi > -INF, np.exp(zi - (m if m > -INF else 0)), 0.0)
+            s = s / s.sum() if s.sum() > 0 else s
+        else:
+            s = np.where(zi > -INF, 1 / (1 + np.exp(-np.maximum(zi, -700))), 0.0)
+        c = s + b
+        ok = (zi > -INF) & (c > -INF)
+        if top < groups:
+            gv = []
+            for j in range(groups):
+                best = np.sort(c[j * per:(j + 1) * per][ok[j * per:(j + 1) * per]])[::-1][:2]
+                gv.append(best.sum() if len(best) else -INF)
+            order = sorted(range(groups), key=lambda j: (-gv[j], j))
+            for j in order[top:]:
+                ok[j * per:(j + 1) * per] = False
+        by = zi if bias is None else c
+        order = sorted((j for j in range(e) if ok[j]), key=lambda j: (-by[j], j))[:k]
+        r = len(order)
+        idx[i, :r] = order
+        so = s[order]
+        if renorm and r:  # ratios of scores, from their logarithms
+            ls = zi[order] if score == "softmax" else -np.logaddexp(0, -zi[order])
+            so = np.exp(ls - ls.max())
+            so = so / so.sum()
+        w[i, :r] = so * scale
+        gi = g[i, :r]
+        if renorm:
+            d = w[i, :r] * (gi - (gi * w[i, :r]).sum() / scale)
+        else:
+            d = w[i, :r] * gi
+        if score == "sigmoid":
+            d = d * (1 - s[order])
+        dz[i, order] = d
+        if score == "softmax" and not renorm:
+            dz[i] -= s * (gi * w[i, :r]).sum()
+    counts = np.bincount(idx[idx >= 0], minlength=e)
+    return (torch.from_numpy(w), torch.from_numpy(idx), torch.from_numpy(counts),
+            torch.from_numpy(dz))
+
+
+def route_check(z, k, score="softmax", bias=None, groups=1, top=None, renorm=True, scale=1.0):
+    zl = z.detach().requires_grad_()
+    w, idx, counts = ops.route(zl, k, score=score, bias=bias, groups=groups, top_groups=top,
+                               renormalize=renorm, scale=scale)
+    g = rand(w.shape, 77)
+    dz, = torch.autograd.grad(w, [zl], g.to(w.device))
+    rw, ri, rc, rd = route_oracle(z, k, score, bias, groups, groups if top is None else top,
+                                  renorm, scale, g.double().numpy())
+    assert idx.dtype == torch.int32 and counts.dtype == torch.int32 and w.dtype == torch.float32
+    assert torch.equal(idx.cpu().long(), ri) and torch.equal(counts.cpu().long(), rc)
+    # exponentials of differences of logits |z| <= zm (relative 2 E32 (zm + 1) each) and sums of
+    # up to E terms
+    e = z.shape[1]
+    fin = z[z.isfinite()].abs()
+    zm = fin.max().item() if fin.numel() else 0.0
+    rel = (e + 16 + 8 * zm) * E32
+    check(w, rw, rel * rw + 1e-37, "weights")
+    gm = g.abs().amax(dim=1, keepdim=True).double() if g.numel() else 0
+    u = half_step(z.dtype)
+    wsum = rw.abs().sum(dim=1, keepdim=True)
+    small = 2.0 ** -24 if z.dtype == torch.float16 else 1e-37
+    check(dz, rd, 4 * rel * gm * torch.maximum(wsum, rd.abs()) + u * rd.abs() + small, "dz")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (1, 64, 2), (5, 3, 3), (17, 16, 4), (33, 17, 5),
+                                   (9, 60, 32), (40, 64, 8), (50, 128, 8), (130, 200, 6),
+                                   (20, 256, 16), (7, 500, 10), (5, 1024, 32), (600, 8, 2)])
+def test_route(device, dtype, t, e, k):
+    z = rand((t, e), t + e, dtype, device, 1.5)
+    bias = rand((e,), 5, torch.float32, device, 0.1)
+    for score in ("softmax", "sigmoid"):
+        for renorm in (True, False):
+            route_check(z, k, score, renorm=renorm, scale=2.5)
+            route_check(z, k, score, bias, renorm=renorm)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("e,groups,top,k", [(8, 8, 3, 3), (16, 4, 2, 5), (64, 8, 3, 6),
+                                            (128, 2, 1, 8), (256, 8, 4, 8), (192, 64, 5, 15),
+                                            (1000, 10, 7, 20), (12, 3, 3, 4)])
+def test_route_groups(device, e, groups, top, k):
+    for dtype in DTYPES:
+        z = rand((37, e), e, dtype, device)
+        bias = rand((e,), 6, torch.float32, device, 0.05)
+        for score in ("softmax", "sigmoid"):
+            route_check(z, k, score, bias, groups, top, scale=2.5)
+            route_check(z, k, score, None, groups, top, renorm=False)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_route_ties_and_left_out(device):
+    z = torch.zeros((9, 70), device=device)
+    z[1, 5:] = 1.0
+    z[2, ::7] = -1.0
+    z[3, 3:] = -INF      # three are left
+    z[4] = -INF          # none
+    z[5, 1::2] = math.nan
+    z[6] = 200.0         # scores that round to 1, and to 0
+    z[7] = -200.0
+    z[7, 9] = -199.0
+    z[8, 60:] = 3e38
+    route_check(z, 5)
+    route_check(z[:6], 5, renorm=False)
+    for groups, top in ((1, 1), (7, 3), (10, 2)):
+        route_check(z, 5, "sigmoid", None, groups, top)
+        route_check(z[:6], 5, "sigmoid", None, groups, top, renorm=False)
+        bias = torch.zeros(70, device=device)
+        bias[10:13] = -INF
+        bias[20], bias[33] = math.nan, torch.finfo(torch.float32).min
+        route_check(z[:6], 5, "sigmoid", bias, groups, top)
+        route_check(z[:6], 5, "softmax", bias, groups, top, renorm=False)
+    # near ties: choice values that differ by less than a step of fp32
+    z = torch.zeros((4, 40), device=device)
+    bias = torch.full((40,), 0.25, device=device)
+    z[:, 30] = 2.0 ** -24
+    w, idx, _ = ops.route(z, 3, score="sigmoid", bias=bias)
+    assert idx.cpu().tolist() == [[30, 0, 1]] * 4
+    w, idx, counts = ops.route(z[:0], 3)
+    assert w.shape == (0, 3) and not counts.any() and counts.shape == (40,)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_route_strides(device):
+    wide = rand((50, 77), 1, torch.float32, device)
+    for z in (wide[:, 1:65], wide[:, :64], wide[::2, 4:68], rand((64, 30), 2, device=device).t(),
+              rand((1, 64), 3, device=device).expand(20, 64)):
+        route_check(z, 4)
+
+
+def test_route_refusals():
+    z = torch.zeros((3, 16))
+    b = torch.zeros(16)
+    for bad in [lambda: ops.route(z[0], 2), lambda: ops.route(z, 0), lambda: ops.route(z, 17),
+                lambda: ops.route(z, 2, groups=3), lambda: ops.route(z, 2, groups=0),
+                lambda: ops.route(z, 2, groups=4, top_groups=5),
+                lambda: ops.route(z, 2, groups=4, top_groups=0),
+                lambda: ops.route(z, 9, groups=4, top_groups=2),
+                lambda: ops.route(torch.zeros((3, 1025)), 2),
+                lambda: ops.route(torch.zeros((3, 64)), 33), lambda: ops.route(z[:, :0], 1),
+                lambda: ops.route(torch.zeros((3, 130)), 2, groups=65),
+                lambda: ops.route(z, 2, score="relu"), lambda: ops.route(z, 2, scale=0.0),
+                lambda: ops.route(z, 2, scale=math.nan), lambda: ops.route(z, 2, bias=b[:3]),
+                lambda: ops.route(z, 2, bias=b.half()), lambda: ops.route(z.double(), 2),
+                lambda: ops.route(z.long(), 2), lambda: ops.route([[1.0]], 1)]:
+        with pytest.raises(ValueError):
+            bad()
+
+
+# ------------------------------------------------------------------------ together, as in use
+def step(x, gate, experts, items, bias, target, seed, p=0.2, k=2):
+    """Denoising features -> gate -> mixture of projections -> softmax over the catalogue."""
+    h = ops.dropout(x, p, seed)
+    w, idx, counts = ops.route(h.float() @ gate, k)
+    dense = (w[:, :, None] * (idx[:, :, None] == torch.arange(len(experts), device=x.device))) \
+        .sum(1)
+    user = sum(dense[:, e:e + 1] * (h.float() @ experts[e]) for e in range(len(experts)))
+    user = user.to(x.dtype)
+    return ops.softmax_cross_entropy(user, items, target, bias), counts
+
+
+def step_inputs(device, dtype, n=37, d=24, e=6, v=211):
+    x = rand((n, d), 1, dtype, device)
+    leaves = [rand((d, e), 2, torch.float32, device, 0.5),
+              rand((e, d, d), 3, torch.float32, device, 0.3), rand((v, d), 4, dtype, device, 0.4),
+              rand((v,), 5, torch.float32, device)]
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(6)).to(device)
+    t[3::5] = -100
+    return x, [q.requires_grad_() for q in leaves], t
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_training_step_together(device):
+    x, leaves, t = step_inputs(device, torch.float32)
+    x.requires_grad_()
+    loss, counts = step(x, *leaves, t, 11)
+    grads = torch.autograd.grad(loss, [x] + leaves)
+    # the same in 64 bits from elementary operations
+    p64 = [cpu64(q).requires_grad_() for q in [x] + leaves]
+    words = torch.tensor(philox_words(x.numel(), 0, 11)).view(x.shape)
+    h = p64[0] * (words >= round(0.2 * 2 ** 32)).double() / 0.8
+    z = h @ p64[1]
+    top, idx = z.topk(2, dim=1)
+    w = torch.softmax(top, 1)
+    mixed = torch.stack([(h[:, :, None] * p64[2][idx[:, j]]).sum(1) for j in range(2)], 1)
+    user = (w[:, :, None] * mixed).sum(1)
+    ref = torch.nn.functional.cross_entropy(user @ p64[3].t() + p64[4], t.cpu())
+    want = torch.autograd.grad(ref, p64)
+    assert torch.equal(counts.cpu().long(), torch.bincount(idx.reshape(-1), minlength=6))
+    # five fp32 stages of at most a few hundred terms: 2^-23 times 2000 of the largest entry
+    check(loss, ref.detach(), 2000 * E32 * ref.item(), "loss")
+    for i, (g, r) in enumerate(zip(grads, want)):
+        check(g, r, 2000 * E32 * r.abs().max().item(), f"grad {i}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_training_step_captured(dtype):
+    """One captured training step, replayed with new inputs and seeds, against the eager step."""
+    x, leaves, t = step_inputs("cuda", dtype, n=70, v=600)
+    seed = torch.tensor([1], device="cuda")
+
+    def run():
+        loss, counts = step(x, *leaves, t, seed)
+        return [loss.detach(), counts, *torch.autograd.grad(loss, leaves)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs, replayed in turn: neither may use the other's workspace
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = run()
+        graphs.append((g, out))
+    for i in range(4):
+        x.copy_(rand(x.shape, 50 + i, dtype))
+        seed.fill_(100 + i)
+        eager = run()
+        g, out = graphs[i % 2]
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(eager, out):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_other_stream_gives_the_same():
+    x, leaves, t = step_inputs("cuda", torch.bfloat16, n=300, v=3000)
+    want = step(x, *leaves, t, 5)[0]
+    want = [want.detach(), *torch.autograd.grad(want, leaves)]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        got = step(x, *leaves, t, 5)[0]
+        got = [got.detach(), *torch.autograd.grad(got, leaves)]
+    s.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)  # (fixed order of every sum)

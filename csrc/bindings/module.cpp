@@ -390,9 +390,8 @@ PYBIND11_MODULE(_native, m) {
                py::gil_scoped_release r;
                if (t.rows > 0 && ctx->is_gpu()) {
                  ctx->activate();
-                 OAP_HIP_CHECK(hipMemcpy2D(dst, size_t(t.cols) * 4, t.data.data(), size_t(t.ld) * 4,
-                                           size_t(t.cols) * 4, size_t(t.rows),
-                                           hipMemcpyDeviceToHost));
+                 ctx->download_rows(dst, size_t(t.cols) * 4, t.data.data(), size_t(t.ld) * 4,
+                                    size_t(t.cols) * 4, t.rows);
                } else {
                  for (int64_t i = 0; i < t.rows; ++i)
                    std::memcpy(dst + size_t(i) * t.cols, t.data.as<float>() + size_t(i) * t.ld,

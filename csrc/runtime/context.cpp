@@ -166,9 +166,13 @@ void Context::download_rows(void* dst, size_t dst_pitch, const void* src, size_t
   Event done[2];
   auto issue = [&](int64_t c) {
     const int64_t r0 = c * per, nr = std::min(per, rows - r0);
-    OAP_HIP_CHECK(hipMemcpy2DAsync(stage_[c & 1].data(), width,
-                                   static_cast<const char*>(src) + size_t(r0) * src_pitch,
-                                   src_pitch, width, size_t(nr), hipMemcpyDeviceToHost, st));
+    const char* from = static_cast<const char*>(src) + size_t(r0) * src_pitch;
+    if (src_pitch == width)  // (rows without padding are one run)
+      OAP_HIP_CHECK(hipMemcpyAsync(stage_[c & 1].data(), from, size_t(nr) * width,
+                                   hipMemcpyDeviceToHost, st));
+    else
+      OAP_HIP_CHECK(hipMemcpy2DAsync(stage_[c & 1].data(), width, from, src_pitch, width,
+                                     size_t(nr), hipMemcpyDeviceToHost, st));
     done[c & 1].record(st);
   };
   issue(0);

@@ -430,7 +430,7 @@ __global__ __launch_bounds__(WAVES * 64, 1) void oap_kmeans_lloyd_t1(LeanArgs a)
     for (int s = 0; s < KS; ++s) {
       f16x8 v;
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {  // v_pk_mul_f32 + v_cvt_pk_f16_f32 (RNE): 1 op / value
+      for (int j = 0; j < 8; j += 2) {  // v_mul_f32 x2 + v_cvt_pk_f16_f32 (RNE)
         const f32x2 p = f32x2{x.at(s, j), x.at(s, j + 1)} * s_;
         const f16x2 q = __builtin_convertvector(p, f16x2);
         v[j] = q[0];

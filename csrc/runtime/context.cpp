@@ -6,9 +6,9 @@
 namespace oap {
 
 // -------------------------------------------------------------------------------- Stream/Event
-Stream::Stream(int device, int priority) : device_(device) {
+Stream::Stream(int device) : device_(device) {
   OAP_HIP_CHECK(hipSetDevice(device));
-  OAP_HIP_CHECK(hipStreamCreateWithPriority(&s_, hipStreamNonBlocking, priority));
+  OAP_HIP_CHECK(hipStreamCreateWithFlags(&s_, hipStreamNonBlocking));
 }
 Stream::~Stream() {
   if (s_) (void)hipStreamDestroy(s_);
@@ -78,11 +78,9 @@ Context::Context(int device, double hbm_fraction, int cpu_threads)
     size_t budget = static_cast<size_t>(static_cast<double>(info_.free_mem) * hbm_fraction);
     // 1 GiB segments: few hipMallocs for 288 GB-class devices, little waste for small fits.
     arena_ = std::make_shared<DeviceArena>(device, budget, size_t(1) << 30);
-    int lo = 0, hi = 0;
-    OAP_HIP_CHECK(hipDeviceGetStreamPriorityRange(&lo, &hi));
-    compute_ = std::make_unique<Stream>(device, 0);
-    comm_ = std::make_unique<Stream>(device, hi);  // collectives get the higher priority
-    h2d_ = std::make_unique<Stream>(device, 0);
+    compute_ = std::make_unique<Stream>(device);
+    comm_ = std::make_unique<Stream>(device);
+    h2d_ = std::make_unique<Stream>(device);
   } else {
     info_.id = -1;
     info_.name = "cpu";

@@ -19,11 +19,12 @@
 
 namespace oap {
 
-// RAII HIP stream.
+// RAII HIP stream, always at the default priority (work on streams of different priorities has
+// hung).
 class Stream {
  public:
   Stream() = default;
-  explicit Stream(int device, int priority = 0);
+  explicit Stream(int device);
   ~Stream();
   Stream(const Stream&) = delete;
   Stream& operator=(const Stream&) = delete;

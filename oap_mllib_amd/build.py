@@ -25,11 +25,10 @@ BUILD = ROOT / "build" / "native"
 PKG = ROOT / "oap_mllib_amd"
 ARCH = os.environ.get("PYTORCH_ROCM_ARCH", "gfx950").split(";")[0] or "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-# Device code without the packed fp32 instructions (v_pk_add / mul / fma_f32), for the units that
-# were written for it: some of their forms have given wrong results.  The roundings are the same.
-# The host pass does not know the feature and says so; that line is filtered from the warnings.
+# Device code without the packed fp32 instructions (v_pk_add / mul / fma_f32): some of their
+# forms have given wrong results.  The roundings are the same.  The host pass does not know the
+# feature and says so; that line is filtered from the warnings.
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-NO_PACKED_UNITS = {"dropout.hip", "route.hip", "softmax_ce.hip"}
 
 
 def ext_path() -> Path:
@@ -94,9 +93,7 @@ def _compile(src: Path, debug: bool) -> tuple[Path, str]:
     obj = _obj(src)
     cmd = [HIPCC] + _common_flags(debug) + _includes()
     if src.suffix == ".hip":
-        cmd += ["-x", "hip", f"--offload-arch={ARCH}", "-munsafe-fp-atomics"]
-        if src.name in NO_PACKED_UNITS:
-            cmd += NO_PACKED_FP32
+        cmd += ["-x", "hip", f"--offload-arch={ARCH}", "-munsafe-fp-atomics"] + NO_PACKED_FP32
     else:
         cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]
         if "linalg" in src.parts:  # host fp64 dense kernels: x86-64-v3 (both hosts have it)

@@ -1,23 +1,22 @@
-// Tile core of the products of the softmax cross entropy: C[m, n] = sum_k A(m, k) B(n, k) in
-// bf16 or fp16 on v_mfma_f32_32x32x16 with fp32 sums.  Each operand lies in memory either with k
-// along its rows (kAlongK: element (r, k) at r * ld + k) or with k across them (kAcrossK: at
-// k * ld + r), so no operand is ever transposed in memory.
+// Tile core of the products of the softmax cross entropy: C[m, n] = sum_k A(m, k) B(n, k) on the
+// matrix units, in bf16 or fp16 (v_mfma_f32_32x32x16) or fp32 (v_mfma_f32_32x32x2), with fp32
+// sums.  Each operand lies in memory either with k along its rows (kAlongK: element (r, k) at
+// r * ld + k) or with k across them (kAcrossK: at k * ld + r), so no operand is ever transposed
+// in memory.
 //
-// A workgroup of 8 waves owns a BM x BN tile.  k advances in blocks of 64, staged by
-// global_load_lds (16 bytes a lane) into one of two LDS buffers while the other feeds the MFMAs:
-// one barrier a block.
+// A workgroup of 4 waves, one per SIMD, owns a BM x BN tile; a wave's part of up to 128 x 128
+// keeps 256 accumulators, so a byte read from LDS feeds the most MFMAs.  k advances in blocks of
+// 128 bytes of a row (64 or 32 elements) in two LDS buffers: the next block is loaded into
+// registers while this one is multiplied, and written to the other buffer before the last of
+// its four steps; one barrier a block, and behind it the last step's MFMAs cover the first reads
+// of the next block.
 //  * kAlongK: 128 bytes of each row; the 16-byte chunk c of row r lies at slot c ^ (r & 7), so
 //    the eight rows that a fragment read (ds_read_b128) touches at once use different banks.
-//  * kAcrossK: 64 rows of k with R elements each, read by ds_read_b64_tr_b16: the 16 lanes of
-//    a group pass the addresses of 4 x 16 elements (4 of k, 16 of r) and get them transposed,
-//    lane i the four k of r = i.  Two reads make a fragment.  The 64-byte granule of a row is
-//    xor-ed with bits of k, so the four k rows of a read use different banks.
-// global_load_lds writes its 64 lanes' data in lane order, so both permutations are applied to
-// the global addresses.
-//
-// fp32 operands come as three bf16 planes per row (x = h + m + l, 8 bits each: all 24 bits of
-// the significand); the six plane products above 2^-24 are summed as if k were six times as
-// long, smallest first.
+//  * kAcrossK, 16 bits: 64 rows of k, read by ds_read_b64_tr_b16: the 16 lanes of a group pass
+//    the addresses of 4 x 16 elements (4 of k, 16 of r) and get them transposed, lane i the four
+//    k of r = i.  Two reads make a fragment.  The 64-byte granule of a row is xor-ed with bits
+//    of k, so the four k rows of a read use different banks.
+//  * kAcrossK, fp32: 32 rows of k, read by ds_read_b32 (32 lanes along a row).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,20 +30,25 @@ typedef __bf16 gt_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 gt_f16x8 __attribute__((ext_vector_type(8)));
 typedef short gt_s16x4 __attribute__((ext_vector_type(4)));
 typedef short gt_s16x8 __attribute__((ext_vector_type(8)));
+typedef float gt_f32x4 __attribute__((ext_vector_type(4)));
 typedef float gt_f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void* gt_lds_ptr;
+typedef unsigned gt_u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) gt_s16x4* gt_lds_s16x4;
-typedef const __attribute__((address_space(1))) void* gt_glb_ptr;
 
+// A fragment: the 16 bytes of a lane that one step of k multiplies
 template <typename T>
-struct GtVec;
+struct GtFrag;
 template <>
-struct GtVec<__bf16> {
+struct GtFrag<__bf16> {
   typedef gt_bf16x8 type;
 };
 template <>
-struct GtVec<_Float16> {
+struct GtFrag<_Float16> {
   typedef gt_f16x8 type;
+};
+template <>
+struct GtFrag<float> {
+  typedef gt_f32x4 type;
 };
 
 __device__ inline gt_f32x16 gt_mfma(gt_bf16x8 a, gt_bf16x8 b, gt_f32x16 c) {
@@ -53,101 +57,154 @@ __device__ inline gt_f32x16 gt_mfma(gt_bf16x8 a, gt_bf16x8 b, gt_f32x16 c) {
 __device__ inline gt_f32x16 gt_mfma(gt_f16x8 a, gt_f16x8 b, gt_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
+__device__ inline gt_f32x16 gt_mfma(gt_f32x4 a, gt_f32x4 b, gt_f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
 
-constexpr int kGtK = 64;         // elements of k per block
-constexpr int kGtThreads = 512;  // 8 waves
+constexpr int kGtThreads = 256;  // 4 waves
 
-// `rows` x `cols` elements in memory, row stride `ld`; plane q of a row starts at q * plane.
-// Reads beyond the last row or the last whole 16 bytes of a row are moved back onto them, so
-// what lies there is the caller's to leave out.  cols is a multiple of 8, p 16-byte aligned.
+// elements of k per block, and per 16-byte chunk
+template <typename T>
+constexpr int gt_block() {
+  return 128 / int(sizeof(T));
+}
+template <typename T>
+constexpr int gt_chunk() {
+  return 16 / int(sizeof(T));
+}
+
+// `rows` x `cols` elements in memory, row stride `ld`; cols and ld are multiples of a chunk and
+// p is 16-byte aligned.  256 rows span less than 2^31 bytes.  k beyond the extent of the operand
+// reads as 0; rows beyond `rows` (kAlongK) or columns beyond `cols` (kAcrossK) read as some
+// others, and the results they belong to are the caller's to leave out.
 struct GtOperand {
   const void* p;
   int64_t ld;
   int64_t rows, cols;
-  int64_t plane;
 };
 
 enum GtOrder { kAlongK, kAcrossK };
 
-// One operand of R rows in a tile; W waves' worth of pieces.
+// One operand of R rows of a tile
 template <typename T, int R, GtOrder ORDER>
 struct GtSide {
-  static constexpr int kBytes = R * kGtK * 2;  // of a staged block
-  static constexpr int kPieces = kBytes / 1024;
-  static constexpr int kChunks = R / 8;  // 16-byte chunks of a k row (kAcrossK)
-  typedef typename GtVec<T>::type V8;
+  static constexpr int BK = gt_block<T>(), CH = gt_chunk<T>();
+  static constexpr int kBytes = R * 128;                // of a staged block
+  static constexpr int kLoads = kBytes / 16 / kGtThreads;  // 16-byte loads of a thread
+  static constexpr int kChunks = R / CH;                // chunks of a k row (kAcrossK)
+  static constexpr int kRowBytes = R * int(sizeof(T));  // of a k row (kAcrossK)
+  static constexpr int kStep = ORDER == kAlongK ? kGtThreads / 8 : kGtThreads / kChunks;
+  typedef typename GtFrag<T>::type Frag;
+  static_assert(kLoads >= 1, "a thread stages at least 16 bytes of each operand");
 
   // xor on the chunk index of k row r
   __device__ static int swizzle(int r) {
+    if (sizeof(T) == 4) return 0;
     return R >= 256 ? (r & 7) << 2 : R == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
   }
 
-  // Global address of this lane's 16 bytes of piece `piece` for k block 0 of the range
-  struct Source {
-    const char* p;
-    int64_t row, limit;  // kAcrossK: k row and the last valid one
-    int64_t step;        // bytes per k block
-    int64_t ld;          // bytes
-    __device__ const char* at(int64_t kb, int64_t plane_bytes) const {
-      if (ORDER == kAlongK) return p + kb * step + plane_bytes;
-      const int64_t r = row + kb * kGtK;
-      return p + (r < limit ? r : limit) * ld + plane_bytes;
+  // The thread's loads: rows r, r + kStep, ... of a block (rows of the tile, or rows of k)
+  struct Loader {
+    const char* base;  // uniform: the tile's first element at the range's first k
+    uint32_t off[kLoads];
+    uint32_t ldb;      // bytes of a row in memory
+    int left;          // k from the block's first to the end of the operand or the range
+    int sub;           // the thread's place in k within a block: its chunk's first k, or row
+    uint32_t lds;      // byte in the staged block
+
+    __device__ void init(const GtOperand& o, int64_t r0, int64_t k0, int64_t k1) {
+      const int t = threadIdx.x;
+      ldb = uint32_t(o.ld * sizeof(T));
+      if (ORDER == kAlongK) {
+        const int r = t >> 3, chunk = t & 7;
+        base = static_cast<const char*>(o.p) + r0 * o.ld * sizeof(T) + k0 * sizeof(T);
+        const int64_t last = o.rows - 1 - r0;  // >= 0: a tile starts within the operand
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int q = r + i * kStep;
+          off[i] = uint32_t(q < last ? q : last) * ldb + chunk * 16;
+        }
+        left = int((k1 < o.cols ? k1 : o.cols) - k0);
+        sub = chunk * CH;
+        lds = r * 128 + ((chunk ^ (r & 7)) << 4);
+      } else {
+        const int k = t / kChunks, chunk = t % kChunks;
+        base = static_cast<const char*>(o.p) + k0 * o.ld * sizeof(T) + r0 * sizeof(T);
+        const int64_t last = o.cols - CH - r0;  // >= 0
+        const int64_t c = int64_t(chunk) * CH;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          off[i] = uint32_t(k + i * kStep) * ldb + uint32_t((c < last ? c : last) * sizeof(T));
+        left = int((k1 < o.rows ? k1 : o.rows) - k0);
+        sub = k;
+        lds = k * kRowBytes + ((chunk ^ swizzle(k)) << 4);
+      }
+    }
+    // loads the block and steps to the next.  Buffer loads: an offset beyond the resource reads
+    // as 0, so what lies beyond the extent of k needs no branch (a branch would make the compiler
+    // wait for the loads where its paths join).
+    __device__ void load(gt_u32x4 (&v)[kLoads]) {
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), short(0),
+                                                          0x7fffffff, 0x00020000);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int k = sub + (ORDER == kAlongK ? 0 : i * kStep);
+        const uint32_t o = k < left ? off[i] : 0x80000000u;
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, o, 0, 0);
+      }
+      base += ORDER == kAlongK ? 128u : BK * ldb;
+      left -= BK;
+    }
+    __device__ void store(char* block, const gt_u32x4 (&v)[kLoads]) const {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+        *reinterpret_cast<gt_u32x4*>(block + lds +
+                                     i * kStep * (ORDER == kAlongK ? 128 : kRowBytes)) = v[i];
     }
   };
-  __device__ static Source source(const GtOperand& o, int piece, int lane, int64_t r0,
-                                  int64_t k0) {
-    Source s;
-    s.ld = o.ld * 2;
-    s.limit = o.rows - 1;
-    if (ORDER == kAlongK) {
-      const int64_t r = r0 + piece * 8 + (lane >> 3);
-      const int chunk = (lane & 7) ^ (lane >> 3);
-      s.p = static_cast<const char*>(o.p) + (r < o.rows ? r : o.rows - 1) * s.ld + k0 * 2 +
-            chunk * 16;
-      s.step = kGtK * 2;
-      s.row = 0;
-    } else {
-      const int kr = piece * (64 / kChunks) + lane / kChunks;
-      const int chunk = (lane % kChunks) ^ swizzle(kr);
-      const int64_t c = r0 + chunk * 8;
-      s.p = static_cast<const char*>(o.p) + (c < o.cols ? c : o.cols - 8) * 2;
-      s.step = 0;
-      s.row = k0 + kr;
-    }
-    return s;
-  }
 
-  // Per-lane LDS offsets of the fragments of rows base + 32 i
+  // Fragments of the rows base + 32 i
   template <int N>
   struct Reader {
-    int off[ORDER == kAlongK ? 1 : N][2];
+    static constexpr int kOffs = ORDER == kAcrossK && sizeof(T) == 2 ? N : 1;
+    int off[kOffs][2];
     int r7;
     __device__ void init(int lane, int base) {
       if (ORDER == kAlongK) {
         off[0][0] = (base + (lane & 31)) * 128;
         r7 = lane & 7;
+      } else if (sizeof(T) == 4) {
+        off[0][0] = 4 * (lane >> 5) * kRowBytes + (base + (lane & 31)) * 4;
       } else {
         const int g = lane >> 4, s = lane & 15;
 #pragma unroll
-        for (int i = 0; i < (ORDER == kAlongK ? 1 : N); ++i)
+        for (int i = 0; i < kOffs; ++i)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int k = 8 * (g >> 1) + (s >> 2) + 4 * q;
             const int chunk = (base + 32 * i + 16 * (g & 1)) / 8 + ((s & 3) >> 1);
-            off[i][q] = k * R * 2 + (chunk ^ swizzle(k)) * 16 + (s & 1) * 8;
+            off[i][q] = k * kRowBytes + ((chunk ^ swizzle(k)) << 4) + (s & 1) * 8;
           }
       }
     }
-    __device__ V8 read(const char* block, int i, int ks, int lane) const {
+    __device__ Frag read(const char* block, int i, int ks, int lane) const {
       if constexpr (ORDER == kAlongK) {
-        const int slot = ((2 * ks + (lane >> 5)) ^ r7) * 16;
-        return *reinterpret_cast<const V8*>(block + off[0][0] + i * 32 * 128 + slot);
+        const int slot = ((2 * ks + (lane >> 5)) ^ r7) << 4;
+        return *reinterpret_cast<const Frag*>(block + off[0][0] + slot + i * 32 * 128);
+      } else if constexpr (sizeof(T) == 4) {
+        const char* p = block + off[0][0] + ks * 8 * kRowBytes + i * 32 * 4;
+        Frag f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(p + j * kRowBytes);
+        return f;
       } else {
-        const char* p = block + ks * 16 * R * 2;
+        const char* p = block + ks * 16 * kRowBytes;
         const gt_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)(p + off[i][0]));
         const gt_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)(p + off[i][1]));
         const gt_s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(V8, v);
+        return __builtin_bit_cast(Frag, v);
       }
     }
   };
@@ -155,106 +212,79 @@ struct GtSide {
 
 // Element (row i, column j) of acc[mi][ni][e] in lane l of wave (wm, wn):
 //   i = wm * WM + 32 mi + 8 (e >> 2) + 4 (l >> 5) + (e & 3),   j = wn * WN + 32 ni + (l & 31)
-template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M, int PLANES>
+template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M_>
 struct GtTile {
   static constexpr int BM = BM_, BN = BN_;
-  static constexpr int WAVES_N = 8 / WAVES_M;
+  static constexpr int WAVES_M = WAVES_M_, WAVES_N = 4 / WAVES_M;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
   static constexpr int MI = WM / 32, NI = WN / 32;
   typedef GtSide<T, BM, OA> SideA;
   typedef GtSide<T, BN, OB> SideB;
+  static constexpr int BK = SideA::BK;
   static constexpr int kBuf = SideA::kBytes + SideB::kBytes;
   static constexpr int kLds = 2 * kBuf;
-  static constexpr int kPairs = PLANES == 3 ? 6 : 1;
-  static constexpr int kLoadsA = SideA::kPieces / 8, kLoadsB = SideB::kPieces / 8;
-  typedef typename GtVec<T>::type V8;
-  static_assert(MI >= 1 && NI >= 1 && kLoadsB >= 1 && (PLANES == 1 || PLANES == 3), "tile");
+  typedef typename GtFrag<T>::type Frag;
+  static_assert(MI >= 1 && NI >= 1, "tile");
 
-  // acc += A[m0.., k0..k1) B[n0.., k0..k1)^T; k0, k1 multiples of 64.  Every thread of the
+  // acc += A[m0.., k0..k1) B[n0.., k0..k1)^T; k0 a multiple of a block.  Every thread of the
   // workgroup calls it; all LDS reads are done when it returns.
   __device__ static void run(const GtOperand& A, const GtOperand& B, int64_t m0, int64_t n0,
                              int64_t k0, int64_t k1, char* lds, gt_f32x16 (&acc)[MI][NI]) {
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    typename SideA::Source sa[kLoadsA];
-    typename SideB::Source sb[kLoadsB];
-#pragma unroll
-    for (int i = 0; i < kLoadsA; ++i) sa[i] = SideA::source(A, wave * kLoadsA + i, lane, m0, k0);
-#pragma unroll
-    for (int i = 0; i < kLoadsB; ++i) sb[i] = SideB::source(B, wave * kLoadsB + i, lane, n0, k0);
+    if (k1 <= k0) return;
+    const int lane = threadIdx.x & 63;
+    typename SideA::Loader ga;
+    typename SideB::Loader gb;
+    ga.init(A, m0, k0, k1);
+    gb.init(B, n0, k0, k1);
     typename SideA::template Reader<MI> ra;
     typename SideB::template Reader<NI> rb;
-    ra.init(lane, (wave / WAVES_N) * WM);
-    rb.init(lane, (wave % WAVES_N) * WN);
-    const int nk = int((k1 - k0) / kGtK), total = nk * kPairs;
-    auto stage = [&](int it, int buf) {
-      int kb = it, pa = 0, pb = 0;
-      if (kPairs > 1) {
-        const int pair = it / nk;
-        kb = it - pair * nk;
-        // (l,h) (h,l) (m,m) (m,h) (h,m) (h,h)
-        pa = pair == 0 ? 2 : (pair == 2 || pair == 3) ? 1 : 0;
-        pb = pair == 1 ? 2 : (pair == 2 || pair == 4) ? 1 : 0;
-      }
-      char* da = lds + buf * kBuf + wave * kLoadsA * 1024;
-      char* db = lds + buf * kBuf + SideA::kBytes + wave * kLoadsB * 1024;
+    ra.init(lane, wave_m() * WM);
+    rb.init(lane, wave_n() * WN);
+    const int nk = int((k1 - k0 + BK - 1) / BK);
+    gt_u32x4 va[SideA::kLoads], vb[SideB::kLoads];
+    Frag a[2][MI], b[2][NI];
+    auto fetch = [&](const char* block, int ks, int f) {
 #pragma unroll
-      for (int i = 0; i < kLoadsA; ++i)
-        __builtin_amdgcn_global_load_lds((gt_glb_ptr)(sa[i].at(kb, pa * A.plane * 2)),
-                                         (gt_lds_ptr)(da + i * 1024), 16, 0, 0);
+      for (int i = 0; i < MI; ++i) a[f][i] = ra.read(block, i, ks, lane);
 #pragma unroll
-      for (int i = 0; i < kLoadsB; ++i)
-        __builtin_amdgcn_global_load_lds((gt_glb_ptr)(sb[i].at(kb, pb * B.plane * 2)),
-                                         (gt_lds_ptr)(db + i * 1024), 16, 0, 0);
+      for (int j = 0; j < NI; ++j) b[f][j] = rb.read(block + SideA::kBytes, j, ks, lane);
     };
-    if (total > 0) stage(0, 0);
-    for (int it = 0; it < total; ++it) {
-      const int buf = it & 1;
-      // this wave's pieces of the block landed, then everyone's; and every wave has read the
-      // other buffer (its reads fed MFMAs that were issued before the barrier)
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      const char* la = lds + buf * kBuf;
-      const char* lb = la + SideA::kBytes;
-      constexpr int KS = kGtK / 16;
-      if constexpr (OA == kAcrossK || OB == kAcrossK) {
-        // all of the block's fragments are read before the next block's loads are issued: the
-        // compiler waits for every load in flight before a transposed read
-        V8 a[KS][MI], b[KS][NI];
+    auto multiply = [&](int f) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+      for (int i = 0; i < MI; ++i)
 #pragma unroll
-          for (int i = 0; i < MI; ++i) a[ks][i] = ra.read(la, i, ks, lane);
-#pragma unroll
-          for (int j = 0; j < NI; ++j) b[ks][j] = rb.read(lb, j, ks, lane);
-        }
-        if (it + 1 < total) stage(it + 1, buf ^ 1);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = gt_mfma(a[ks][i], b[ks][j], acc[i][j]);
-      } else {
-        if (it + 1 < total) stage(it + 1, buf ^ 1);
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          V8 a[MI], b[NI];
-#pragma unroll
-          for (int i = 0; i < MI; ++i) a[i] = ra.read(la, i, ks, lane);
-#pragma unroll
-          for (int j = 0; j < NI; ++j) b[j] = rb.read(lb, j, ks, lane);
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = gt_mfma(a[i], b[j], acc[i][j]);
-        }
+        for (int j = 0; j < NI; ++j) acc[i][j] = gt_mfma(a[f][i], b[f][j], acc[i][j]);
+    };
+    ga.load(va);
+    gb.load(vb);
+    ga.store(lds, va);
+    gb.store(lds + SideA::kBytes, vb);
+    __syncthreads();
+    fetch(lds, 0, 0);
+    for (int it = 0; it < nk; ++it) {
+      const char* cur = lds + (it & 1) * kBuf;
+      char* nxt = lds + ((it + 1) & 1) * kBuf;
+      const bool more = it + 1 < nk;
+      if (more) {
+        ga.load(va);
+        gb.load(vb);
       }
+      fetch(cur, 1, 1);
+      multiply(0);
+      fetch(cur, 2, 0);
+      multiply(1);
+      fetch(cur, 3, 1);
+      multiply(0);
+      if (more) {
+        ga.store(nxt, va);
+        gb.store(nxt + SideA::kBytes, vb);
+        // every wave has read this block and written its part of the next
+        __syncthreads();
+        fetch(nxt, 0, 0);
+      }
+      multiply(1);
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    __syncthreads();
   }
 
   __device__ static int wave_m() { return (threadIdx.x >> 6) / WAVES_N; }

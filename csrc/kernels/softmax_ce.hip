@@ -20,8 +20,6 @@ namespace kern {
 
 namespace {
 
-constexpr int kBM = 256;  // rows of a tile's first operand (classes, or rows in dx)
-
 // exp(d) for d <= 0 (or a little above): v_exp_f32 of d log2(e).  The difference is formed
 // first, in fp32: scaling both terms before it would lose |z| 2^-24 of the exponent.
 __device__ inline float exp_of(float d) {
@@ -29,46 +27,28 @@ __device__ inline float exp_of(float d) {
 }
 
 // ------------------------------------------------------------------------------ operand images
-// fp32 as three bf16 planes whose sum is the value to 2^-24 (each remainder is exact)
-template <int PLANES, typename T>
-__device__ inline void planes_of(float v, T (&out)[PLANES]) {
-  out[0] = static_cast<T>(v);
-  if constexpr (PLANES == 3) {
-    const float r = v - static_cast<float>(out[0]);
-    out[1] = static_cast<T>(r);
-    out[2] = static_cast<T>(r - static_cast<float>(out[1]));
-  }
-}
-
-// dst[row][plane][dp] = planes of src[row][0..dim), zero beyond dim and in rows that are left
-// out (target == ignore, or bias == -inf): an infinity or NaN there must not meet a coefficient
-// of zero in the gradients' products
-template <typename S, typename T, int PLANES>
-__global__ __launch_bounds__(256) void oap_ce_pack(const S* __restrict__ src, int64_t ld,
+// dst[row][dp] = src[row][0..dim), zero beyond dim and in rows that are left out (target ==
+// ignore, or bias == -inf): an infinity or NaN there must not meet a coefficient of zero in the
+// gradients' products
+template <typename T>
+__global__ __launch_bounds__(256) void oap_ce_pack(const T* __restrict__ src, int64_t ld,
                                                    int64_t rows, int dim, int dp,
                                                    const int64_t* __restrict__ target,
                                                    int64_t ignore,
                                                    const float* __restrict__ bias,
                                                    T* __restrict__ dst) {
-  const int per = dp / 8;
+  constexpr int CH = gt_chunk<T>();
+  const int per = dp / CH;
   const int64_t total = rows * per;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total;
        i += int64_t(gridDim.x) * 256) {
     const int64_t row = i / per;
-    const int c = int(i - row * per) * 8;
+    const int c = int(i - row * per) * CH;
     const bool out = target ? target[row] == ignore : bias && bias[row] == -INFINITY;
-    Vec16<T> o[PLANES];
+    Vec16<T> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      T p[PLANES];
-      const bool in = !out && c + j < dim;
-      planes_of<PLANES, T>(in ? static_cast<float>(src[row * ld + c + j]) : 0.f, p);
-#pragma unroll
-      for (int q = 0; q < PLANES; ++q) o[q].v[j] = p[q];
-    }
-#pragma unroll
-    for (int q = 0; q < PLANES; ++q)
-      *reinterpret_cast<Vec16<T>*>(dst + (row * PLANES + q) * dp + c) = o[q];
+    for (int j = 0; j < CH; ++j) o.v[j] = !out && c + j < dim ? src[row * ld + c + j] : T(0.f);
+    *reinterpret_cast<Vec16<T>*>(dst + row * dp + c) = o;
   }
 }
 
@@ -89,7 +69,7 @@ struct LogitArgs {
   const float2* stat;  // [n] the row's (max, sum)
   const float* coef;   // [n] upstream gradient over its largest magnitude, 0: no loss
   float pscale;
-  void* dz;            // [npad][PLANES][vp]
+  void* dz;            // [npad][vp]
   int64_t vp;
   float* dbpart;       // [row tile][vp] sums of dz over the tile's rows, or null
 };
@@ -102,32 +82,43 @@ __device__ inline int xcd_tile(int total) {
   return x * per + (x < rest ? x : rest) + i;
 }
 
+// Tiles in runs of 8 class tiles by all row tiles, the class tile fastest: the 32 workgroups that
+// an XCD runs at a time then share 8 + 4 operand panels in its L2.
+__device__ inline void tile_at(int t, int mtiles, int ntiles, int& mt, int& nt) {
+  const int run = t / (8 * ntiles), first = run * 8;
+  const int wide = mtiles - first < 8 ? mtiles - first : 8;
+  const int r = t - first * ntiles;
+  mt = first + r % wide;
+  nt = r / wide;
+}
+
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
 // over the tile's classes is mostly within the lane.
-template <typename T, int BN, int WAVES_M, int PLANES, bool GRAD>
-__global__ __launch_bounds__(kGtThreads) void oap_ce_logits(LogitArgs a) {
-  typedef GtTile<T, kBM, kAlongK, BN, kAlongK, WAVES_M, PLANES> Tile;
-  static_assert(BN * kBM * 2 <= Tile::kLds, "the dz tile fits the staging buffers");
+template <typename T, int BM, int BN, int WAVES_M, bool GRAD>
+__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
+  typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M> Tile;
+  static_assert(BN * BM * 2 <= Tile::kLds, "a 16-bit dz tile fits the staging buffers");
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float sbias[kBM];
+  __shared__ float sbias[BM];
   __shared__ float2 smerge[WAVES_M][BN];
   __shared__ int left_out;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int t = xcd_tile(a.vtiles * a.ntiles);
-  const int vt = t / a.ntiles, nt = t - vt * a.ntiles;
-  const int v0 = vt * kBM, n0 = nt * BN;
+  int vt, nt;
+  tile_at(xcd_tile(a.vtiles * a.ntiles), a.vtiles, a.ntiles, vt, nt);
+  const int v0 = vt * BM, n0 = nt * BN;
   if (tid == 0) left_out = 0;
   __syncthreads();
-  if (tid < kBM) {
-    const float b = v0 + tid >= a.w.rows ? -INFINITY : a.bias ? a.bias[v0 + tid] : 0.f;
-    sbias[tid] = b;
+  for (int i = tid; i < BM; i += kGtThreads) {
+    const float b = v0 + i >= a.w.rows ? -INFINITY : a.bias ? a.bias[v0 + i] : 0.f;
+    sbias[i] = b;
     if (b == -INFINITY) left_out = 1;
   }
+  __syncthreads();
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
   Tile::run(a.w, a.x, v0, n0, 0, a.dp, lds, acc);
   const int i0 = Tile::row0(), j0 = Tile::col0();
-  const bool masked = left_out != 0;  // (written before run()'s barriers)
+  const bool masked = left_out != 0;
 #pragma unroll
   for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
@@ -201,19 +192,19 @@ __global__ __launch_bounds__(kGtThreads) void oap_ce_logits(LogitArgs a) {
   }
   if constexpr (!GRAD) {
     __syncthreads();
-    if (tid < BN) {
+    for (int j = tid; j < BN; j += kGtThreads) {
       float m = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < WAVES_M; ++k) m = fmaxf(m, smerge[k][tid].x);
+      for (int k = 0; k < WAVES_M; ++k) m = fmaxf(m, smerge[k][j].x);
       const float ref = m > -INFINITY ? m : 0.f;
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < WAVES_M; ++k) s += smerge[k][tid].y * exp_of(smerge[k][tid].x - ref);
-      a.part[int64_t(vt) * a.npad + n0 + tid] = make_float2(m, s);
+      for (int k = 0; k < WAVES_M; ++k) s += smerge[k][j].y * exp_of(smerge[k][j].x - ref);
+      a.part[int64_t(vt) * a.npad + n0 + j] = make_float2(m, s);
     }
   } else {
     if (a.dbpart) {
-      float* sdb = reinterpret_cast<float*>(lds);  // [wave column][kBM]
+      float* sdb = reinterpret_cast<float*>(lds);  // [wave column][BM]
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
@@ -223,20 +214,36 @@ __global__ __launch_bounds__(kGtThreads) void oap_ce_logits(LogitArgs a) {
           for (int ni = 0; ni < Tile::NI; ++ni) v += acc[mi][ni][e];
 #pragma unroll
           for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-          if ((lane & 31) == 0) sdb[Tile::wave_n() * kBM + i0 + Tile::row_of(mi, e)] = v;
+          if ((lane & 31) == 0) sdb[Tile::wave_n() * BM + i0 + Tile::row_of(mi, e)] = v;
         }
       __syncthreads();
-      if (tid < kBM) {
+      for (int i = tid; i < BM; i += kGtThreads) {
         float v = 0.f;
-        for (int k = 0; k < Tile::WAVES_N; ++k) v += sdb[k * kBM + tid];
-        a.dbpart[int64_t(nt) * a.vp + v0 + tid] = v;
+        for (int k = 0; k < Tile::WAVES_N; ++k) v += sdb[k * BM + i];
+        a.dbpart[int64_t(nt) * a.vp + v0 + i] = v;
       }
     }
-    // dz through LDS, plane by plane: [row][256 classes], the 16-byte chunk c of row j at slot
-    // c ^ (j & 31), then out in whole rows
     T* out = static_cast<T*>(a.dz);
+    if constexpr (sizeof(T) == 4) {
+      // four consecutive classes of a row per lane and store
 #pragma unroll
-    for (int q = 0; q < PLANES; ++q) {
+      for (int ni = 0; ni < Tile::NI; ++ni)
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float4 v;
+            v.x = acc[mi][ni][4 * g + 0];
+            v.y = acc[mi][ni][4 * g + 1];
+            v.z = acc[mi][ni][4 * g + 2];
+            v.w = acc[mi][ni][4 * g + 3];
+            *reinterpret_cast<float4*>(out + (int64_t(n0) + j0 + 32 * ni) * a.vp + v0 + i0 +
+                                       Tile::row_of(mi, 4 * g)) = v;
+          }
+    } else {
+      // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & 15),
+      // then out in whole rows
+      constexpr int CPR = BM / 8;  // chunks of a row
       __syncthreads();
 #pragma unroll
       for (int ni = 0; ni < Tile::NI; ++ni)
@@ -248,21 +255,17 @@ __global__ __launch_bounds__(kGtThreads) void oap_ce_logits(LogitArgs a) {
               T v[4];
             } f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // the plane, and in its place what it leaves for the next
-              const float v = acc[mi][ni][4 * g + e] * (q == 0 ? a.pscale : 1.f);
-              f.v[e] = static_cast<T>(v);
-              if (PLANES > 1) acc[mi][ni][4 * g + e] = v - static_cast<float>(f.v[e]);
-            }
+            for (int e = 0; e < 4; ++e)
+              f.v[e] = static_cast<T>(acc[mi][ni][4 * g + e] * a.pscale);
             const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
-            *reinterpret_cast<Four*>(lds + j * (kBM * 2) + (((i >> 3) ^ (j & 31)) << 4) +
+            *reinterpret_cast<Four*>(lds + j * (BM * 2) + (((i >> 3) ^ (j & 15)) << 4) +
                                      ((i & 4) << 1)) = f;
           }
       __syncthreads();
-      for (int c = tid; c < BN * (kBM / 8); c += kGtThreads) {
-        const int j = c >> 5, k = c & 31;
-        *reinterpret_cast<float4*>(out + ((int64_t(n0) + j) * PLANES + q) * a.vp + v0 + k * 8) =
-            *reinterpret_cast<const float4*>(lds + j * (kBM * 2) + ((k ^ (j & 31)) << 4));
+      for (int c = tid; c < BN * CPR; c += kGtThreads) {
+        const int j = c / CPR, k = c % CPR;
+        *reinterpret_cast<float4*>(out + (int64_t(n0) + j) * a.vp + v0 + k * 8) =
+            *reinterpret_cast<const float4*>(lds + j * (BM * 2) + ((k ^ (j & 15)) << 4));
       }
     }
   }
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(1024) void oap_ce_coef(const float* __restrict__ gr
 // ------------------------------------------------------------------------------------- products
 struct ProdArgs {
   GtOperand a, b;
-  int64_t k;           // extent, a multiple of 64
+  int64_t k;           // extent
   int64_t m, n;        // valid rows / columns of the result
   int mtiles, ntiles, splits;
   void* out;           // dW: [m][n] elements; dx: fp32 slabs [split][m][n]
@@ -395,32 +398,39 @@ struct ProdArgs {
 
 // dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
 // part to the same elements, so the order of the sums is fixed.
-template <typename T, int BN, int WAVES_M, int PLANES>
-__global__ __launch_bounds__(kGtThreads) void oap_ce_dx(ProdArgs a) {
-  typedef GtTile<T, kBM, kAlongK, BN, kAcrossK, WAVES_M, PLANES> Tile;
+template <typename T, int BM, int BN, int WAVES_M>
+__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_dx(ProdArgs a) {
+  typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = xcd_tile(a.mtiles * a.ntiles * a.splits);
   const int sp = t / (a.mtiles * a.ntiles), u = t - sp * a.mtiles * a.ntiles;
-  const int mt = u / a.ntiles, nt = u - mt * a.ntiles;
-  const int64_t blocks = a.k / kGtK;
-  const int64_t k0 = blocks * sp / a.splits * kGtK, k1 = blocks * (sp + 1) / a.splits * kGtK;
+  int mt, nt;
+  tile_at(u, a.mtiles, a.ntiles, mt, nt);
+  const int64_t blocks = (a.k + Tile::BK - 1) / Tile::BK;
+  const int64_t k0 = blocks * sp / a.splits * Tile::BK;
+  const int64_t k1 = sp + 1 == a.splits ? a.k : blocks * (sp + 1) / a.splits * Tile::BK;
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
-  Tile::run(a.a, a.b, mt * kBM, nt * BN, k0, k1, lds, acc);
-  float* out = static_cast<float*>(a.out) + int64_t(sp) * a.m * a.n;
-  const int64_t i0 = int64_t(mt) * kBM + Tile::row0(), j0 = nt * BN + Tile::col0();
+  Tile::run(a.a, a.b, mt * BM, nt * BN, k0, k1, lds, acc);
+  const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
+  float* out = static_cast<float*>(a.out) + (int64_t(sp) * a.m + i0) * a.n + j0;
 #pragma unroll
-  for (int ni = 0; ni < Tile::NI; ++ni)
+  for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-    for (int mi = 0; mi < Tile::MI; ++mi)
+    for (int g = 0; g < 4; ++g) {
+      // (four rows at a time, from an address that is not kept for the others)
+      float* q = out + Tile::row_of(mi, 4 * g) * a.n;
+      asm volatile("" : "+v"(q)::"memory");
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t i = i0 + Tile::row_of(mi, e), j = j0 + 32 * ni;
-        if (i < a.m && j < a.n) {
-          float* o = out + i * a.n + j;
-          *o = a.add ? *o + acc[mi][ni][e] : acc[mi][ni][e];
-        }
-      }
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int ni = 0; ni < Tile::NI; ++ni)
+          if (i0 + Tile::row_of(mi, 4 * g + e) < a.m && j0 + 32 * ni < a.n) {
+            float* o = q + e * a.n + 32 * ni;
+            const float v = acc[mi][ni][4 * g + e];
+            *o = a.add ? *o + v : v;
+          }
+    }
 }
 
 template <typename S>
@@ -437,18 +447,18 @@ __global__ __launch_bounds__(256) void oap_ce_dx_out(const float* __restrict__ s
   }
 }
 
-template <typename S, typename T, int BN, int WAVES_M, int PLANES>
-__global__ __launch_bounds__(kGtThreads) void oap_ce_dw(ProdArgs a) {
-  typedef GtTile<T, kBM, kAcrossK, BN, kAcrossK, WAVES_M, PLANES> Tile;
+template <typename T, int BM, int BN, int WAVES_M>
+__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_dw(ProdArgs a) {
+  typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int t = xcd_tile(a.mtiles * a.ntiles);
-  const int mt = t / a.ntiles, nt = t - mt * a.ntiles;
+  int mt, nt;
+  tile_at(xcd_tile(a.mtiles * a.ntiles), a.mtiles, a.ntiles, mt, nt);
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
-  Tile::run(a.a, a.b, mt * kBM, nt * BN, 0, a.k, lds, acc);
+  Tile::run(a.a, a.b, mt * BM, nt * BN, 0, a.k, lds, acc);
   const float g = *a.gscale * a.unscale;
-  S* out = static_cast<S*>(a.out);
-  const int64_t i0 = int64_t(mt) * kBM + Tile::row0(), j0 = nt * BN + Tile::col0();
+  T* out = static_cast<T*>(a.out);
+  const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
 #pragma unroll
   for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
@@ -459,7 +469,7 @@ __global__ __launch_bounds__(kGtThreads) void oap_ce_dw(ProdArgs a) {
 #pragma unroll
       for (int ni = 0; ni < Tile::NI; ++ni) {
         const int64_t j = j0 + 32 * ni;
-        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : acc[mi][ni][e] * g);
+        if (j < a.n) out[i * a.n + j] = static_cast<T>(out_of ? 0.f : acc[mi][ni][e] * g);
       }
     }
 }
@@ -483,53 +493,43 @@ __global__ __launch_bounds__(256) void oap_ce_fill0(S* __restrict__ p, int64_t c
 }
 
 // ------------------------------------------------------------------------------------- planning
-// Operand type and planes of an element type
-template <typename S>
-struct Operand {
-  typedef S T;
-  static constexpr int planes = 1;
-};
-template <>
-struct Operand<float> {
-  typedef __bf16 T;
-  static constexpr int planes = 3;
-};
-
 struct Plan {
-  int planes;
-  int64_t dp;             // dim to a multiple of 64
+  int64_t dp;               // features of an image's row, to a whole chunk
   bool x_direct, w_direct;  // the operand is read where it lies
-  int bn;                 // row tile of the logits
+  int bm, bn;               // class and row tile of the logits
   int64_t npad;
-  int64_t piece;          // classes per piece, a multiple of 256
-  int dbn;                // feature tile of dx and dW
+  int64_t piece;            // classes per piece, a multiple of 256
+  int dbm, dbn;             // row (or class) and feature tile of dx and dW
   int splits;
 };
 
 bool direct(const CeArgs& a, const void* p, int64_t ld) {
-  return a.elem != Elem::F32 && a.dim % kGtK == 0 && ld % 8 == 0 &&
-         reinterpret_cast<uintptr_t>(p) % 16 == 0;
+  const int ch = 16 / elem_size(a.elem);
+  return a.dim % ch == 0 && ld % ch == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0 &&
+         ld < (int64_t(1) << 20);
 }
 
 constexpr int64_t kPieceBytes = int64_t(1) << 29;  // of one dz image or one class image
 
 Plan make_plan(const CeArgs& a, bool grad) {
   Plan p;
-  p.planes = a.elem == Elem::F32 ? 3 : 1;
-  p.dp = int64_t(round_up(size_t(a.dim), kGtK));
+  const int es = elem_size(a.elem);
+  p.dp = int64_t(round_up(size_t(a.dim), size_t(16 / es)));
   // (the gradients read images in which the rows that are left out are zero)
   p.x_direct = !grad && direct(a, a.x, a.ldx);
   p.w_direct = direct(a, a.w, a.ldw) && !(grad && a.bias);
+  p.bm = 256;
   p.bn = a.n <= 64 ? 64 : 256;
   p.npad = int64_t(round_up(size_t(a.n), size_t(p.bn)));
-  const int64_t vpad = int64_t(round_up(size_t(a.classes), kBM));
+  const int64_t vpad = int64_t(round_up(size_t(a.classes), 256));
   int64_t per = p.dp;  // elements per class of the largest image
   if (grad) per = std::max(per, p.npad);
-  p.piece = kPieceBytes / (per * 2 * p.planes) / kBM * kBM;
-  p.piece = std::max<int64_t>(kBM, std::min(p.piece, vpad));
-  if (!grad && p.w_direct) p.piece = std::min<int64_t>(vpad, int64_t(1) << 22);
+  p.piece = kPieceBytes / (per * es) / 256 * 256;
+  if (!grad && p.w_direct) p.piece = vpad;
+  p.piece = std::max<int64_t>(256, std::min({p.piece, vpad, int64_t(1) << 20}));
+  p.dbm = 256;
   p.dbn = a.dim <= 128 ? 128 : 256;
-  const int64_t tiles = ceil_div(a.n, kBM) * ceil_div(a.dim, p.dbn);
+  const int64_t tiles = ceil_div(a.n, p.dbm) * ceil_div(a.dim, p.dbn);
   const int64_t by_k = std::max<int64_t>(1, p.piece / 1024);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(by_k, 512 / tiles)));
   return p;
@@ -563,38 +563,31 @@ unsigned stride_grid(int64_t threads) {
   return unsigned(std::max<int64_t>(1, std::min<int64_t>(ceil_div(threads, 256), 8192)));
 }
 
-template <typename S>
+template <typename T>
 struct Ce {
-  typedef typename Operand<S>::T T;
-  static constexpr int P = Operand<S>::planes;
-
-  static void pack(const S* src, int64_t ld, int64_t rows, int dim, int64_t dp,
+  static void pack(const void* src, int64_t ld, int64_t rows, int dim, int64_t dp,
                    const int64_t* target, int64_t ignore, const float* bias, T* dst,
                    hipStream_t s) {
-    oap_ce_pack<S, T, P><<<stride_grid(rows * dp / 8), 256, 0, s>>>(
-        src, ld, rows, dim, int(dp), target, ignore, bias, dst);
+    oap_ce_pack<T><<<stride_grid(rows * dp / gt_chunk<T>()), 256, 0, s>>>(
+        static_cast<const T*>(src), ld, rows, dim, int(dp), target, ignore, bias, dst);
     OAP_HIP_CHECK(hipGetLastError());
   }
 
-  static GtOperand image(const T* p, int64_t dp, int64_t rows) {
-    return {p, dp * P, rows, dp, dp};
+  template <int BM, int BN, int WAVES_M, bool GRAD>
+  static void logits_tile(const LogitArgs& l, hipStream_t s) {
+    auto k = oap_ce_logits<T, BM, BN, WAVES_M, GRAD>;
+    constexpr int lds = GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M>::kLds;
+    set_lds(k, lds);
+    k<<<dim3(unsigned(l.vtiles * l.ntiles)), kGtThreads, lds, s>>>(l);
+    OAP_HIP_CHECK(hipGetLastError());
   }
 
   template <bool GRAD>
   static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
-    const unsigned grid = unsigned(l.vtiles * l.ntiles);
-    if (p.bn == 64) {
-      auto k = oap_ce_logits<T, 64, 4, P, GRAD>;
-      constexpr int lds = GtTile<T, kBM, kAlongK, 64, kAlongK, 4, P>::kLds;
-      set_lds(k, lds);
-      k<<<dim3(grid), kGtThreads, lds, s>>>(l);
-    } else {
-      auto k = oap_ce_logits<T, 256, 2, P, GRAD>;
-      constexpr int lds = GtTile<T, kBM, kAlongK, 256, kAlongK, 2, P>::kLds;
-      set_lds(k, lds);
-      k<<<dim3(grid), kGtThreads, lds, s>>>(l);
-    }
-    OAP_HIP_CHECK(hipGetLastError());
+    if (p.bn == 64)
+      logits_tile<256, 64, 4, GRAD>(l, s);
+    else
+      logits_tile<256, 256, 2, GRAD>(l, s);
   }
 
   struct Work {
@@ -605,9 +598,9 @@ struct Ce {
 
   static size_t carve_forward(const CeArgs& a, const Plan& p, void* base, Work& w) {
     Carver c{static_cast<char*>(base)};
-    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp * P);
-    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp * P);
-    w.part = c.take<float2>(size_t(ceil_div(a.classes, kBM)) * p.npad);
+    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp);
+    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
+    w.part = c.take<float2>(size_t(ceil_div(a.classes, p.bm)) * p.npad);
     w.zt = c.take<float>(a.n);
     return c.used;
   }
@@ -615,11 +608,11 @@ struct Ce {
   static size_t carve_backward(const CeArgs& a, const Plan& p, void* base, bool dx, bool dw,
                                bool db, Work& w) {
     Carver c{static_cast<char*>(base)};
-    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp * P);
-    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp * P);
+    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp);
+    w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.coef = c.take<float>(a.n);
     w.gscale = c.take<float>(1);
-    w.dz = c.take<T>(size_t(p.npad) * P * p.piece);
+    w.dz = c.take<T>(size_t(p.npad) * p.piece);
     w.slab = dx ? c.take<float>(size_t(p.splits) * a.n * a.dim) : nullptr;
     w.dbpart = db ? c.take<float>(size_t(p.npad / p.bn) * p.piece) : nullptr;
     return c.used;
@@ -630,13 +623,12 @@ struct Ce {
     const Plan p = make_plan(a, false);
     Work w;
     carve_forward(a, p, work, w);
-    const S* x = static_cast<const S*>(a.x);
-    const S* wt = static_cast<const S*>(a.w);
+    const T* wt = static_cast<const T*>(a.w);
     LogitArgs l = {};
-    l.x = {a.x, a.ldx, a.n, p.dp, 0};
+    l.x = {a.x, a.ldx, a.n, p.dp};
     if (!p.x_direct) {
-      pack(x, a.ldx, a.n, a.dim, p.dp, nullptr, 0, nullptr, w.ximg, s);
-      l.x = image(w.ximg, p.dp, a.n);
+      pack(a.x, a.ldx, a.n, a.dim, p.dp, nullptr, 0, nullptr, w.ximg, s);
+      l.x = {w.ximg, p.dp, a.n, p.dp};
     }
     l.dp = p.dp;
     l.target = a.target;
@@ -646,18 +638,18 @@ struct Ce {
     l.zt = w.zt;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
-      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp, 0};
+      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp};
       if (!p.w_direct) {
         pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, nullptr, w.wimg, s);
-        l.w = image(w.wimg, p.dp, nc);
+        l.w = {w.wimg, p.dp, nc, p.dp};
       }
       l.bias = a.bias ? a.bias + c0 : nullptr;
       l.class0 = c0;
-      l.vtiles = int(ceil_div(nc, kBM));
-      l.part = w.part + c0 / kBM * p.npad;
+      l.vtiles = int(ceil_div(nc, p.bm));
+      l.part = w.part + c0 / p.bm * p.npad;
       logits<false>(p, l, s);
     }
-    const int vtiles = int(ceil_div(a.classes, kBM));
+    const int vtiles = int(ceil_div(a.classes, p.bm));
     int cols = 1;
     while (cols < 64 && cols < a.n) cols *= 2;
     oap_ce_rows<<<dim3(unsigned(ceil_div(a.n, cols))), 1024, 0, s>>>(
@@ -669,25 +661,24 @@ struct Ce {
     }
   }
 
-  template <int BN, int WAVES_M>
+  template <int BM, int BN, int WAVES_M>
   static void products(const CeArgs& a, const Plan& p, const Work& w, const LogitArgs& l,
                        int64_t nc, int64_t c0, float unscale, void* dx, void* dw,
                        hipStream_t s) {
-    constexpr int lds = GtTile<T, kBM, kAcrossK, BN, kAcrossK, WAVES_M, P>::kLds;
+    constexpr int lds = GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M>::kLds;
     ProdArgs g = {};
     g.ntiles = int(ceil_div(a.dim, BN));
     g.n = a.dim;
     g.gscale = w.gscale;
     g.unscale = unscale;
-    const int64_t ncp = int64_t(round_up(size_t(nc), kGtK));
+    g.a = {w.dz, p.piece, p.npad, p.piece};
     if (dx) {
-      auto k = oap_ce_dx<T, BN, WAVES_M, P>;
+      auto k = oap_ce_dx<T, BM, BN, WAVES_M>;
       set_lds(k, lds);
-      g.a = image(w.dz, p.piece, p.npad);
       g.b = l.w;
-      g.k = ncp;
+      g.k = nc;
       g.m = a.n;
-      g.mtiles = int(ceil_div(a.n, kBM));
+      g.mtiles = int(ceil_div(a.n, BM));
       g.splits = p.splits;
       g.out = w.slab;
       g.add = c0 > 0;
@@ -695,14 +686,13 @@ struct Ce {
       OAP_HIP_CHECK(hipGetLastError());
     }
     if (dw) {
-      auto k = oap_ce_dw<S, T, BN, WAVES_M, P>;
+      auto k = oap_ce_dw<T, BM, BN, WAVES_M>;
       set_lds(k, lds);
-      g.a = image(w.dz, p.piece, p.npad);
       g.b = l.x;
-      g.k = int64_t(round_up(size_t(a.n), kGtK));
+      g.k = a.n;
       g.m = nc;
-      g.mtiles = int(ceil_div(nc, kBM));
-      g.out = static_cast<S*>(dw) + c0 * a.dim;
+      g.mtiles = int(ceil_div(nc, BM));
+      g.out = static_cast<T*>(dw) + c0 * a.dim;
       g.bias = a.bias ? a.bias + c0 : nullptr;
       k<<<dim3(unsigned(g.mtiles * g.ntiles)), kGtThreads, lds, s>>>(g);
       OAP_HIP_CHECK(hipGetLastError());
@@ -714,18 +704,17 @@ struct Ce {
     const Plan p = make_plan(a, true);
     Work w;
     carve_backward(a, p, work, dx, dw, db, w);
-    const S* x = static_cast<const S*>(a.x);
-    const S* wt = static_cast<const S*>(a.w);
+    const T* wt = static_cast<const T*>(a.w);
     // fp16 images hold dz times 2^14: |dz| <= 1 stays finite and 2^-28 is still a normal number
     const float pscale = a.elem == Elem::F16 ? 0x1p14f : 1.f;
     oap_ce_coef<<<1, 1024, 0, s>>>(grad, per_row, mean, a.target, a.ignore, a.classes, a.n,
                                    w.coef, w.gscale);
     OAP_HIP_CHECK(hipGetLastError());
     LogitArgs l = {};
-    l.x = {a.x, a.ldx, a.n, p.dp, 0};
+    l.x = {a.x, a.ldx, a.n, p.dp};
     if (!p.x_direct) {
-      pack(x, a.ldx, a.n, a.dim, p.dp, a.target, a.ignore, nullptr, w.ximg, s);
-      l.x = image(w.ximg, p.dp, a.n);
+      pack(a.x, a.ldx, a.n, a.dim, p.dp, a.target, a.ignore, nullptr, w.ximg, s);
+      l.x = {w.ximg, p.dp, a.n, p.dp};
     }
     l.dp = p.dp;
     l.target = a.target;
@@ -741,19 +730,19 @@ struct Ce {
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
       const float* bias = a.bias ? a.bias + c0 : nullptr;
-      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp, 0};
+      l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp};
       if (!p.w_direct) {
         pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, bias, w.wimg, s);
-        l.w = image(w.wimg, p.dp, nc);
+        l.w = {w.wimg, p.dp, nc, p.dp};
       }
       l.bias = bias;
       l.class0 = c0;
-      l.vtiles = int(ceil_div(nc, kBM));
+      l.vtiles = int(ceil_div(nc, p.bm));
       logits<true>(p, l, s);
       if (p.dbn == 128)
-        products<128, 4>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+        products<256, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
       else
-        products<256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+        products<256, 256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
       if (db) {
         oap_ce_db<<<dim3(unsigned(ceil_div(nc, 256))), 256, 0, s>>>(w.dbpart, l.ntiles, p.piece,
                                                                      nc, w.gscale, db + c0);
@@ -761,16 +750,16 @@ struct Ce {
       }
     }
     if (dx) {
-      oap_ce_dx_out<S><<<stride_grid(a.n * a.dim), 256, 0, s>>>(
-          w.slab, p.splits, a.n * a.dim, w.gscale, 1.f / pscale, static_cast<S*>(dx));
+      oap_ce_dx_out<T><<<stride_grid(a.n * a.dim), 256, 0, s>>>(
+          w.slab, p.splits, a.n * a.dim, w.gscale, 1.f / pscale, static_cast<T*>(dx));
       OAP_HIP_CHECK(hipGetLastError());
     }
   }
 
   static void zeros(const CeArgs& a, void* dx, void* dw, float* db, hipStream_t s) {
     const int64_t nx = a.n * a.dim, nw = a.classes * a.dim;
-    if (dx && nx) oap_ce_fill0<S><<<stride_grid(nx), 256, 0, s>>>(static_cast<S*>(dx), nx);
-    if (dw && nw) oap_ce_fill0<S><<<stride_grid(nw), 256, 0, s>>>(static_cast<S*>(dw), nw);
+    if (dx && nx) oap_ce_fill0<T><<<stride_grid(nx), 256, 0, s>>>(static_cast<T*>(dx), nx);
+    if (dw && nw) oap_ce_fill0<T><<<stride_grid(nw), 256, 0, s>>>(static_cast<T*>(dw), nw);
     if (db && a.classes)
       oap_ce_fill0<float><<<stride_grid(a.classes), 256, 0, s>>>(db, a.classes);
     OAP_HIP_CHECK(hipGetLastError());
@@ -778,11 +767,11 @@ struct Ce {
 };
 
 void check(const CeArgs& a) {
-  OAP_CHECK(a.n >= 0 && a.n < (int64_t(1) << 31) - kBM && a.classes >= 1 &&
-                a.classes < (int64_t(1) << 31) - kBM && a.dim >= 1 && a.dim <= (1 << 20) &&
+  OAP_CHECK(a.n >= 0 && a.n < (int64_t(1) << 31) - 256 && a.classes >= 1 &&
+                a.classes < (int64_t(1) << 31) - 256 && a.dim >= 1 && a.dim <= (1 << 20) &&
                 a.ldx >= a.dim && a.ldw >= a.dim,
             "softmax_cross_entropy: bad shape");
-  OAP_CHECK(ceil_div(a.n, 64) * ceil_div(a.classes, kBM) < (int64_t(1) << 31),
+  OAP_CHECK(ceil_div(a.n, 64) * ceil_div(a.classes, 64) < (int64_t(1) << 31),
             "softmax_cross_entropy: " << a.n << " x " << a.classes << " tiles are too many");
 }
 

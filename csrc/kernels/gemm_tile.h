@@ -10,8 +10,8 @@
 // registers while this one is multiplied, and written to the other buffer before the last of
 // its four steps; one barrier a block, and behind it the last step's MFMAs cover the first reads
 // of the next block.
-//  * kAlongK: 128 bytes of each row; the 16-byte chunk c of row r lies at slot c ^ (r & 7), so
-//    the eight rows that a fragment read (ds_read_b128) touches at once use different banks.
+//  * kAlongK: 128 bytes of each row; the 16-byte chunk c of row r lies at slot c ^ ((r >> 1) & 7),
+//    so the 16 rows that a fragment read (ds_read_b128) touches at once use all 64 banks.
 //  * kAcrossK, 16 bits: 64 rows of k, read by ds_read_b64_tr_b16: the 16 lanes of a group pass
 //    the addresses of 4 x 16 elements (4 of k, 16 of r) and get them transposed, lane i the four
 //    k of r = i.  Two reads make a fragment.  The 64-byte granule of a row is xor-ed with bits
@@ -96,6 +96,8 @@ struct GtSide {
   static constexpr int kChunks = R / CH;                // chunks of a k row (kAcrossK)
   static constexpr int kRowBytes = R * int(sizeof(T));  // of a k row (kAcrossK)
   static constexpr int kStep = ORDER == kAlongK ? kGtThreads / 8 : kGtThreads / kChunks;
+  // LDS reads of a fragment
+  static constexpr int kReads = ORDER == kAlongK ? 1 : sizeof(T) == 4 ? 4 : 2;
   typedef typename GtFrag<T>::type Frag;
   static_assert(kLoads >= 1, "a thread stages at least 16 bytes of each operand");
 
@@ -128,7 +130,7 @@ struct GtSide {
         }
         left = int((k1 < o.cols ? k1 : o.cols) - k0);
         sub = chunk * CH;
-        lds = r * 128 + ((chunk ^ (r & 7)) << 4);
+        lds = r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
       } else {
         const int k = t / kChunks, chunk = t % kChunks;
         base = static_cast<const char*>(o.p) + k0 * o.ld * sizeof(T) + r0 * sizeof(T);
@@ -170,11 +172,11 @@ struct GtSide {
   struct Reader {
     static constexpr int kOffs = ORDER == kAcrossK && sizeof(T) == 2 ? N : 1;
     int off[kOffs][2];
-    int r7;
+    int x7;
     __device__ void init(int lane, int base) {
       if (ORDER == kAlongK) {
         off[0][0] = (base + (lane & 31)) * 128;
-        r7 = lane & 7;
+        x7 = (lane >> 1) & 7;
       } else if (sizeof(T) == 4) {
         off[0][0] = 4 * (lane >> 5) * kRowBytes + (base + (lane & 31)) * 4;
       } else {
@@ -191,7 +193,7 @@ struct GtSide {
     }
     __device__ Frag read(const char* block, int i, int ks, int lane) const {
       if constexpr (ORDER == kAlongK) {
-        const int slot = ((2 * ks + (lane >> 5)) ^ r7) << 4;
+        const int slot = ((2 * ks + (lane >> 5)) ^ x7) << 4;
         return *reinterpret_cast<const Frag*>(block + off[0][0] + slot + i * 32 * 128);
       } else if constexpr (sizeof(T) == 4) {
         const char* p = block + off[0][0] + ks * 8 * kRowBytes + i * 32 * 4;
@@ -225,6 +227,28 @@ struct GtTile {
   static constexpr int kLds = 2 * kBuf;
   typedef typename GtFrag<T>::type Frag;
   static_assert(MI >= 1 && NI >= 1, "tile");
+
+  // Order of one step: the next step's fragment reads, and the step's share of global loads or
+  // LDS writes, are spread over its MFMAs, so the reads are in flight from the step's beginning;
+  // left to itself the compiler reads a fragment just before its use and waits for it.
+  template <bool LOADS, bool STORES>
+  __device__ static void interleave() {
+    constexpr int kMfmas = MI * NI * (sizeof(T) == 4 ? 4 : 1);
+    constexpr int kReads = SideA::kReads * MI + SideB::kReads * NI;
+    constexpr int kMoves = SideA::kLoads + SideB::kLoads;
+    constexpr int G = kMfmas < 8 ? kMfmas : 8;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      // the reads in the first half of the step, LDS writes in the second
+      constexpr int kR = STORES ? (2 * kReads + G - 1) / G : (kReads + G - 1) / G;
+      if (!STORES || g < G / 2) __builtin_amdgcn_sched_group_barrier(0x100, kR, 0);
+      if (LOADS) __builtin_amdgcn_sched_group_barrier(0x020, (kMoves + G - 1) / G, 0);
+      if (STORES && g >= G / 2)
+        __builtin_amdgcn_sched_group_barrier(0x200, (2 * kMoves + G - 1) / G, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kMfmas / G, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  }
 
   // acc += A[m0.., k0..k1) B[n0.., k0..k1)^T; k0 a multiple of a block.  Every thread of the
   // workgroup calls it; all LDS reads are done when it returns.
@@ -264,25 +288,25 @@ struct GtTile {
     for (int it = 0; it < nk; ++it) {
       const char* cur = lds + (it & 1) * kBuf;
       char* nxt = lds + ((it + 1) & 1) * kBuf;
-      const bool more = it + 1 < nk;
-      if (more) {
-        ga.load(va);
-        gb.load(vb);
-      }
+      // (the last turn loads zeros from beyond the range and stages them unread: no branch)
+      ga.load(va);
+      gb.load(vb);
       fetch(cur, 1, 1);
       multiply(0);
+      interleave<true, false>();
       fetch(cur, 2, 0);
       multiply(1);
+      interleave<false, false>();
       fetch(cur, 3, 1);
       multiply(0);
-      if (more) {
-        ga.store(nxt, va);
-        gb.store(nxt + SideA::kBytes, vb);
-        // every wave has read this block and written its part of the next
-        __syncthreads();
-        fetch(nxt, 0, 0);
-      }
+      ga.store(nxt, va);
+      gb.store(nxt + SideA::kBytes, vb);
+      interleave<false, true>();
+      // every wave has read this block and written its part of the next
+      __syncthreads();
+      fetch(nxt, 0, 0);
       multiply(1);
+      interleave<false, false>();
     }
     __syncthreads();
   }

@@ -64,6 +64,8 @@ __device__ inline gt_f32x16 gt_mfma(gt_f32x4 a, gt_f32x4 b, gt_f32x16 c) {
 }
 
 constexpr int kGtThreads = 256;  // 4 waves
+// waves per SIMD that a tile's registers allow
+constexpr int gt_occupancy(int bm, int bn) { return bm * bn <= 128 * 128 ? 2 : 1; }
 
 // elements of k per block, and per 16-byte chunk
 template <typename T>
@@ -225,6 +227,9 @@ struct GtTile {
   static constexpr int BK = SideA::BK;
   static constexpr int kBuf = SideA::kBytes + SideB::kBytes;
   static constexpr int kLds = 2 * kBuf;
+  // the last block apart, with only its occupied steps (the largest tiles' registers do not have
+  // room for a second copy of the loop's body, and their k is long)
+  static constexpr bool kTail = gt_occupancy(BM, BN) > 1;
   typedef typename GtFrag<T>::type Frag;
   static_assert(MI >= 1 && NI >= 1, "tile");
 
@@ -285,10 +290,10 @@ struct GtTile {
     gb.store(lds + SideA::kBytes, vb);
     __syncthreads();
     fetch(lds, 0, 0);
-    for (int it = 0; it < nk; ++it) {
+    // (the loads beyond the range give zeros that are staged unread: no branch)
+    for (int it = 0; it < (kTail ? nk - 1 : nk); ++it) {
       const char* cur = lds + (it & 1) * kBuf;
       char* nxt = lds + ((it + 1) & 1) * kBuf;
-      // (the last turn loads zeros from beyond the range and stages them unread: no branch)
       ga.load(va);
       gb.load(vb);
       fetch(cur, 1, 1);
@@ -308,6 +313,27 @@ struct GtTile {
       multiply(1);
       interleave<false, false>();
     }
+    if constexpr (!kTail) {
+      __syncthreads();
+      return;
+    }
+    // the last block: only the steps that hold any k
+    const char* cur = lds + ((nk - 1) & 1) * kBuf;
+    const int steps = int((k1 - k0 - int64_t(nk - 1) * BK + BK / 4 - 1) / (BK / 4));
+    fetch(cur, 1, 1);
+    multiply(0);
+    interleave<false, false>();
+    if (steps > 1) {
+      fetch(cur, 2, 0);
+      multiply(1);
+      interleave<false, false>();
+    }
+    if (steps > 2) {
+      fetch(cur, 3, 1);
+      multiply(0);
+      interleave<false, false>();
+    }
+    if (steps > 3) multiply(1);
     __syncthreads();
   }
 

@@ -7,6 +7,7 @@
 #include "kernels/softmax_ce.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <mutex>
 #include <set>
@@ -20,10 +21,26 @@ namespace kern {
 
 namespace {
 
-// exp(d) for d <= 0 (or a little above): v_exp_f32 of d log2(e).  The difference is formed
-// first, in fp32: scaling both terms before it would lose |z| 2^-24 of the exponent.
-__device__ inline float exp_of(float d) {
-  return __builtin_amdgcn_exp2f(d * 1.44269504088896340736f);
+// Logits are kept in units of ln 2, z log2(e), so that a power is one v_exp_f32 of a difference.
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f;
+__device__ inline float pow2(float d) { return __builtin_amdgcn_exp2f(d); }
+
+// Sum of the 32 lanes of each half wave, in all of them: VALU only (an LDS exchange a step would
+// cost more than the additions)
+template <int CTRL>
+__device__ inline float dpp_add(float v) {
+  const int o = __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true);
+  return v + __int_as_float(o);
+}
+__device__ inline float half_wave_sum(float v) {
+  v = dpp_add<0xB1>(v);   // quad_perm [1,0,3,2]
+  v = dpp_add<0x4E>(v);   // quad_perm [2,3,0,1]
+  v = dpp_add<0x141>(v);  // row_half_mirror
+  v = dpp_add<0x140>(v);  // row_mirror
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false,
+                                                  false);
+  return __int_as_float(p[0]) + __int_as_float(p[1]);
 }
 
 // ------------------------------------------------------------------------------ operand images
@@ -95,9 +112,9 @@ __device__ inline void tile_at(int t, int mtiles, int ntiles, int& mt, int& nt) 
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
 // over the tile's classes is mostly within the lane.
 template <typename T, int BM, int BN, int WAVES_M, bool GRAD>
-__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
+__global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logits(LogitArgs a) {
   typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M> Tile;
-  static_assert(BN * BM * 2 <= Tile::kLds, "a 16-bit dz tile fits the staging buffers");
+  static_assert(BN * BM * int(sizeof(T)) <= Tile::kLds, "the dz tile fits the staging buffers");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float sbias[BM];
   __shared__ float2 smerge[WAVES_M][BN];
@@ -109,7 +126,9 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
   if (tid == 0) left_out = 0;
   __syncthreads();
   for (int i = tid; i < BM; i += kGtThreads) {
-    const float b = v0 + i >= a.w.rows ? -INFINITY : a.bias ? a.bias[v0 + i] : 0.f;
+    float b = v0 + i >= a.w.rows ? -INFINITY : a.bias ? a.bias[v0 + i] : 0.f;
+    // (finite biases stay finite: the type's lowest value is no exclusion)
+    if (b > -INFINITY) b = fmaxf(b * kLog2e, -FLT_MAX);
     sbias[i] = b;
     if (b == -INFINITY) left_out = 1;
   }
@@ -118,19 +137,24 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
   Tile::clear(acc);
   Tile::run(a.w, a.x, v0, n0, 0, a.dp, lds, acc);
   const int i0 = Tile::row0(), j0 = Tile::col0();
-  const bool masked = left_out != 0;
+  const bool masked = left_out != 0, plain = !masked && !a.bias;
+  if (!plain) {
 #pragma unroll
-  for (int mi = 0; mi < Tile::MI; ++mi)
+    for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float b = sbias[i0 + Tile::row_of(mi, e)];
+      for (int e = 0; e < 16; ++e) {
+        const float b = sbias[i0 + Tile::row_of(mi, e)];
 #pragma unroll
-      for (int ni = 0; ni < Tile::NI; ++ni) {
-        const float z = acc[mi][ni][e] + b;
-        // (a class that is left out has no logit, whatever its weights hold)
-        acc[mi][ni][e] = masked && b == -INFINITY ? -INFINITY : z;
+        for (int ni = 0; ni < Tile::NI; ++ni) {
+          const float z = __builtin_fmaf(acc[mi][ni][e], kLog2e, b);
+          // (a class that is left out has no logit, whatever its weights hold)
+          acc[mi][ni][e] = masked && b == -INFINITY ? -INFINITY : z;
+        }
       }
-    }
+  }
+  // acc: the logits in units of ln 2, or (plain) of 1; one multiply-add takes either to its
+  // distance from a row's maximum
+  const float unit = plain ? kLog2e : 1.f;
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
     const int j = j0 + 32 * ni;
@@ -144,12 +168,13 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
         for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[mi][ni][e]);
+      m *= unit;
       float sum = 0.f;
       const float ref = m > -INFINITY ? m : 0.f;
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += exp_of(acc[mi][ni][e] - ref);
+        for (int e = 0; e < 16; ++e) sum += pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref));
       if (__ballot(tgt >= 0)) {
         float zt = 0.f;
         bool mine = false;
@@ -161,25 +186,24 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
             zt = hit ? acc[mi][ni][e] : zt;
             mine |= hit;
           }
-        if (mine) a.zt[n] = zt;
+        if (mine) a.zt[n] = zt * unit;
       }
       const float mo = __shfl_xor(m, 32, 64), so = __shfl_xor(sum, 32, 64);
       const float mm = fmaxf(m, mo), mr = mm > -INFINITY ? mm : 0.f;
       // (a part that is -inf throughout has the sum 0; NaN stays in the sums)
-      const float st = sum * exp_of(m - mr) + so * exp_of(mo - mr);
+      const float st = sum * pow2(m - mr) + so * pow2(mo - mr);
       if (lane < 32) smerge[Tile::wave_m()][j] = make_float2(mm, st);
     } else {
       const float2 st = n < a.n ? a.stat[n] : make_float2(0.f, 0.f);
       const float c = n < a.n ? a.coef[n] : 0.f;
-      const float cs = st.y == 0.f ? 0.f : c / st.y;
+      const float cs = c == 0.f || st.y == 0.f ? 0.f : c / st.y;
+      // (a row without a loss has no gradient, whatever its logits are)
+      const float ref = c == 0.f ? INFINITY : st.x > -INFINITY ? st.x : 0.f;
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float z = acc[mi][ni][e];
-          // (a row without a loss has no gradient, whatever its logits are)
-          acc[mi][ni][e] = z == -INFINITY || c == 0.f ? 0.f : exp_of(z - st.x) * cs;
-        }
+        for (int e = 0; e < 16; ++e)
+          acc[mi][ni][e] = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref)) * cs;
       if (__ballot(tgt >= 0)) {
         const int hit = tgt >= 0 && sbias[i0 + tgt] == -INFINITY ? -1 : tgt;
 #pragma unroll
@@ -199,7 +223,7 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
       const float ref = m > -INFINITY ? m : 0.f;
       float s = 0.f;
 #pragma unroll
-      for (int k = 0; k < WAVES_M; ++k) s += smerge[k][j].y * exp_of(smerge[k][j].x - ref);
+      for (int k = 0; k < WAVES_M; ++k) s += smerge[k][j].y * pow2(smerge[k][j].x - ref);
       a.part[int64_t(vt) * a.npad + n0 + j] = make_float2(m, s);
     }
   } else {
@@ -212,8 +236,7 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
           float v = 0.f;
 #pragma unroll
           for (int ni = 0; ni < Tile::NI; ++ni) v += acc[mi][ni][e];
-#pragma unroll
-          for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
+          v = half_wave_sum(v);
           if ((lane & 31) == 0) sdb[Tile::wave_n() * BM + i0 + Tile::row_of(mi, e)] = v;
         }
       __syncthreads();
@@ -224,50 +247,132 @@ __global__ __launch_bounds__(kGtThreads, 1) void oap_ce_logits(LogitArgs a) {
       }
     }
     T* out = static_cast<T*>(a.dz);
-    if constexpr (sizeof(T) == 4) {
-      // four consecutive classes of a row per lane and store
+    // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & 15), then
+    // out in whole rows
+    constexpr int CH = gt_chunk<T>(), CPR = BM / CH, ROW = BM * int(sizeof(T));
+    __syncthreads();
 #pragma unroll
-      for (int ni = 0; ni < Tile::NI; ++ni)
+    for (int ni = 0; ni < Tile::NI; ++ni)
 #pragma unroll
-        for (int mi = 0; mi < Tile::MI; ++mi)
+      for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float4 v;
-            v.x = acc[mi][ni][4 * g + 0];
-            v.y = acc[mi][ni][4 * g + 1];
-            v.z = acc[mi][ni][4 * g + 2];
-            v.w = acc[mi][ni][4 * g + 3];
-            *reinterpret_cast<float4*>(out + (int64_t(n0) + j0 + 32 * ni) * a.vp + v0 + i0 +
-                                       Tile::row_of(mi, 4 * g)) = v;
-          }
-    } else {
-      // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & 15),
-      // then out in whole rows
-      constexpr int CPR = BM / 8;  // chunks of a row
-      __syncthreads();
+        for (int g = 0; g < 4; ++g) {
+          struct alignas(4 * sizeof(T)) Four {
+            T v[4];
+          } f;
 #pragma unroll
-      for (int ni = 0; ni < Tile::NI; ++ni)
+          for (int e = 0; e < 4; ++e)
+            f.v[e] = static_cast<T>(acc[mi][ni][4 * g + e] * a.pscale);
+          const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
+          *reinterpret_cast<Four*>(lds + j * ROW + (((i / CH) ^ (j & 15)) << 4) +
+                                   (i % CH) * int(sizeof(T))) = f;
+        }
+    __syncthreads();
+    for (int c = tid; c < BN * CPR; c += kGtThreads) {
+      const int j = c / CPR, k = c % CPR;
+      *reinterpret_cast<float4*>(out + (int64_t(n0) + j) * a.vp + v0 + k * CH) =
+          *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & 15)) << 4));
+    }
+  }
+}
+
+// A few rows (one, or up to four): the class rows are read once from memory and that is what
+// bounds it, so they go straight into registers.  G lanes share a class, four 16-byte chunks
+// each; the rows of x stay in registers; every group keeps its own (max, sum) and the workgroup
+// joins them.  The chip streams classes with enough loads in flight: two classes per lane group.
+struct FewArgs {
+  const void *w, *x;
+  int64_t ldw, ldx, classes;
+  int n, dim;
+  const float* bias;
+  const int64_t* target;
+  float2* part;  // [workgroup][n]
+  float* zt;
+};
+
+constexpr int kFewBlocks = 2048;
+constexpr int kFewRows = 4;
+constexpr int kFewIters = 4;
+
+template <typename T, int N, int G>
+__global__ __launch_bounds__(256) void oap_ce_few(FewArgs a) {
+  constexpr int CH = gt_chunk<T>(), GROUPS = 256 / G;
+  __shared__ float2 red[N][GROUPS];
+  const int q = threadIdx.x & (G - 1), g = threadIdx.x / G;
+  float x[N][kFewIters][CH];
 #pragma unroll
-        for (int mi = 0; mi < Tile::MI; ++mi)
+  for (int r = 0; r < N; ++r)
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            struct alignas(8) Four {
-              T v[4];
-            } f;
+    for (int i = 0; i < kFewIters; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              f.v[e] = static_cast<T>(acc[mi][ni][4 * g + e] * a.pscale);
-            const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
-            *reinterpret_cast<Four*>(lds + j * (BM * 2) + (((i >> 3) ^ (j & 15)) << 4) +
-                                     ((i & 4) << 1)) = f;
-          }
-      __syncthreads();
-      for (int c = tid; c < BN * CPR; c += kGtThreads) {
-        const int j = c / CPR, k = c % CPR;
-        *reinterpret_cast<float4*>(out + (int64_t(n0) + j) * a.vp + v0 + k * 8) =
-            *reinterpret_cast<const float4*>(lds + j * (BM * 2) + ((k ^ (j & 15)) << 4));
+      for (int j = 0; j < CH; ++j) {
+        const int k = (q + i * G) * CH + j;
+        x[r][i][j] = r < a.n && k < a.dim
+                         ? static_cast<float>(static_cast<const T*>(a.x)[r * a.ldx + k])
+                         : 0.f;
+      }
+  int64_t tgt[N];
+  float m[N], s[N];
+#pragma unroll
+  for (int r = 0; r < N; ++r) {
+    tgt[r] = r < a.n ? a.target[r] : -1;
+    m[r] = -INFINITY;
+    s[r] = 0.f;
+  }
+  const T* w = static_cast<const T*>(a.w);
+  const int64_t step = int64_t(gridDim.x) * GROUPS;
+  for (int64_t c0 = int64_t(blockIdx.x) * GROUPS + g; c0 < a.classes; c0 += 2 * step) {
+    Vec16<T> v[2][kFewIters];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t c = c0 + u * step < a.classes ? c0 + u * step : c0;
+#pragma unroll
+      for (int i = 0; i < kFewIters; ++i) {
+        v[u][i] = {};
+        if ((q + i * G) * CH < a.dim)
+          v[u][i] = *reinterpret_cast<const Vec16<T>*>(w + c * a.ldw + (q + i * G) * CH);
       }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t c = c0 + u * step;
+      if (c >= a.classes) break;  // (uniform in the group)
+      float b = a.bias ? a.bias[c] : 0.f;
+      const bool out = b == -INFINITY;
+      if (!out) b = fmaxf(b * kLog2e, -FLT_MAX);
+#pragma unroll
+      for (int r = 0; r < N; ++r) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < kFewIters; ++i)
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            z = __builtin_fmaf(x[r][i][j], static_cast<float>(v[u][i].v[j]), z);
+#pragma unroll
+        for (int k = G / 2; k >= 1; k >>= 1) z += __shfl_xor(z, k, 64);
+        z = out ? -INFINITY : __builtin_fmaf(z, kLog2e, b);
+        if (c == tgt[r] && q == 0) a.zt[r] = z;
+        // (NaN stays in the sum)
+        const float mm = fmaxf(m[r], z), ref = mm > -INFINITY ? mm : 0.f;
+        s[r] = s[r] * pow2(m[r] - ref) + pow2(z - ref);
+        m[r] = mm;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < N; ++r)
+    if (q == 0) red[r][g] = make_float2(m[r], s[r]);
+  __syncthreads();
+  if (threadIdx.x < unsigned(a.n)) {
+    const int r = threadIdx.x;
+    float mm = -INFINITY, ss = 0.f;
+    for (int k = 0; k < GROUPS; ++k) {
+      const float2 p = red[r][k];
+      const float t = fmaxf(mm, p.x), ref = t > -INFINITY ? t : 0.f;
+      ss = ss * pow2(mm - ref) + p.y * pow2(p.x - ref);
+      mm = t;
+    }
+    a.part[int64_t(blockIdx.x) * a.n + r] = make_float2(mm, ss);
   }
 }
 
@@ -289,7 +394,7 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(const float2* __restrict__ p
     for (int t = r0; t < vtiles; t += nr) {
       const float2 p = part[int64_t(t) * npad + row];
       const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
-      s = s * exp_of(m - ref) + p.y * exp_of(p.x - ref);
+      s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
       m = mm;
     }
   }
@@ -299,7 +404,7 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(const float2* __restrict__ p
     if (r0 < h) {
       const float2 p = red[threadIdx.x + h * cols];
       const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
-      s = s * exp_of(m - ref) + p.y * exp_of(p.x - ref);
+      s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
       m = mm;
       red[threadIdx.x] = make_float2(m, s);
     }
@@ -312,7 +417,7 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(const float2* __restrict__ p
     else if (t < 0 || t >= classes)
       loss[row] = NAN;
     else
-      loss[row] = zt[row] == -INFINITY ? INFINITY : logf(s) + (m - zt[row]);
+      loss[row] = zt[row] == -INFINITY ? INFINITY : kLn2 * (log2f(s) + (m - zt[row]));
   }
 }
 
@@ -399,7 +504,7 @@ struct ProdArgs {
 // dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
 // part to the same elements, so the order of the sums is fixed.
 template <typename T, int BM, int BN, int WAVES_M>
-__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_dx(ProdArgs a) {
+__global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dx(ProdArgs a) {
   typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int t = xcd_tile(a.mtiles * a.ntiles * a.splits);
@@ -448,7 +553,7 @@ __global__ __launch_bounds__(256) void oap_ce_dx_out(const float* __restrict__ s
 }
 
 template <typename T, int BM, int BN, int WAVES_M>
-__global__ __launch_bounds__(kGtThreads, 1) void oap_ce_dw(ProdArgs a) {
+__global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dw(ProdArgs a) {
   typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   int mt, nt;
@@ -509,7 +614,18 @@ bool direct(const CeArgs& a, const void* p, int64_t ld) {
          ld < (int64_t(1) << 20);
 }
 
-constexpr int64_t kPieceBytes = int64_t(1) << 29;  // of one dz image or one class image
+// Of one dz image or one class image.  Smaller pieces stay in the last-level cache, but their
+// products fill the chip less evenly and dx's slabs are added to more often: 2^28, 2^29, 2^30
+// took 17.7, 16.9, 16.6 ms at 8192 x 131072 x 2048 bf16 and 18.6, 18.0, 17.6 ms at 1024 x 2M x 100
+// fp32.
+constexpr int64_t kPieceBytes = int64_t(1) << 30;
+
+// Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps
+// another's MFMAs, but a byte from LDS feeds half as many.  fp32 MFMAs are slow enough for LDS at
+// any size (1024 x 2M x 100: 19.9 against 24.4 ms); in 16 bits the small ones are faster while
+// the epilogue weighs (forward and gradients, bf16: 3000 x 20000 x 784 0.66 against 0.68 ms,
+// 4096 x 65536 x 512 1.44 against 1.52 ms; 8192 x 131072 x 2048 18.9 against 16.6 ms).
+bool small_tiles(const CeArgs& a) { return a.elem == Elem::F32 || a.dim <= 1024; }
 
 Plan make_plan(const CeArgs& a, bool grad) {
   Plan p;
@@ -518,8 +634,9 @@ Plan make_plan(const CeArgs& a, bool grad) {
   // (the gradients read images in which the rows that are left out are zero)
   p.x_direct = !grad && direct(a, a.x, a.ldx);
   p.w_direct = direct(a, a.w, a.ldw) && !(grad && a.bias);
-  p.bm = 256;
-  p.bn = a.n <= 64 ? 64 : 256;
+  const bool narrow = small_tiles(a);
+  p.bm = a.n > 64 && narrow ? 128 : 256;
+  p.bn = a.n <= 64 ? 64 : narrow ? 128 : 256;
   p.npad = int64_t(round_up(size_t(a.n), size_t(p.bn)));
   const int64_t vpad = int64_t(round_up(size_t(a.classes), 256));
   int64_t per = p.dp;  // elements per class of the largest image
@@ -527,12 +644,18 @@ Plan make_plan(const CeArgs& a, bool grad) {
   p.piece = kPieceBytes / (per * es) / 256 * 256;
   if (!grad && p.w_direct) p.piece = vpad;
   p.piece = std::max<int64_t>(256, std::min({p.piece, vpad, int64_t(1) << 20}));
-  p.dbm = 256;
-  p.dbn = a.dim <= 128 ? 128 : 256;
+  p.dbm = narrow ? 128 : 256;
+  p.dbn = a.dim <= 128 || narrow ? 128 : 256;
   const int64_t tiles = ceil_div(a.n, p.dbm) * ceil_div(a.dim, p.dbn);
-  const int64_t by_k = std::max<int64_t>(1, p.piece / 1024);
+  const int64_t by_k = std::max<int64_t>(1, p.piece / 256);  // at least 256 classes a split
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(by_k, 512 / tiles)));
   return p;
+}
+
+// Features that the lane groups of oap_ce_few cover
+bool few_rows(const CeArgs& a) {
+  return a.n <= kFewRows && a.dim <= 64 * kFewIters * 16 / elem_size(a.elem) &&
+         direct(a, a.w, a.ldw);
 }
 
 struct Carver {
@@ -586,7 +709,9 @@ struct Ce {
   static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
     if (p.bn == 64)
       logits_tile<256, 64, 4, GRAD>(l, s);
-    else
+    else if (p.bn == 128)
+      logits_tile<128, 128, 2, GRAD>(l, s);
+    else if constexpr (sizeof(T) == 2)
       logits_tile<256, 256, 2, GRAD>(l, s);
   }
 
@@ -598,6 +723,12 @@ struct Ce {
 
   static size_t carve_forward(const CeArgs& a, const Plan& p, void* base, Work& w) {
     Carver c{static_cast<char*>(base)};
+    w = {};
+    if (few_rows(a)) {
+      w.part = c.take<float2>(size_t(kFewBlocks) * a.n);
+      w.zt = c.take<float>(a.n);
+      return c.used;
+    }
     w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp);
     w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.part = c.take<float2>(size_t(ceil_div(a.classes, p.bm)) * p.npad);
@@ -623,6 +754,11 @@ struct Ce {
     const Plan p = make_plan(a, false);
     Work w;
     carve_forward(a, p, work, w);
+    if (few_rows(a)) {
+      const int blocks = few(a, w, s);
+      rows(a, w, blocks, a.n, loss, stat, total, mean, s);
+      return;
+    }
     const T* wt = static_cast<const T*>(a.w);
     LogitArgs l = {};
     l.x = {a.x, a.ldx, a.n, p.dp};
@@ -649,16 +785,54 @@ struct Ce {
       l.part = w.part + c0 / p.bm * p.npad;
       logits<false>(p, l, s);
     }
-    const int vtiles = int(ceil_div(a.classes, p.bm));
+    rows(a, w, int(ceil_div(a.classes, p.bm)), p.npad, loss, stat, total, mean, s);
+  }
+
+  // (few rows of many class tiles: fewer rows per workgroup, at least one per CU)
+  static void rows(const CeArgs& a, const Work& w, int tiles, int64_t npad, float* loss,
+                   float2* stat, float* total, bool mean, hipStream_t s) {
     int cols = 1;
-    while (cols < 64 && cols < a.n) cols *= 2;
+    while (cols < 64 && cols * 256 < a.n) cols *= 2;
+    if (a.n >= 8) cols = std::max(cols, 8);
     oap_ce_rows<<<dim3(unsigned(ceil_div(a.n, cols))), 1024, 0, s>>>(
-        w.part, vtiles, p.npad, a.n, cols, a.target, a.ignore, a.classes, w.zt, loss, stat);
+        w.part, tiles, npad, a.n, cols, a.target, a.ignore, a.classes, w.zt, loss, stat);
     OAP_HIP_CHECK(hipGetLastError());
     if (total) {
       oap_ce_total<<<1, 1024, 0, s>>>(loss, a.target, a.ignore, a.n, mean, total);
       OAP_HIP_CHECK(hipGetLastError());
     }
+  }
+
+  template <int N, int G>
+  static int few_launch(const FewArgs& f, hipStream_t s) {
+    const int blocks =
+        int(std::max<int64_t>(1, std::min<int64_t>(kFewBlocks, ceil_div(f.classes, 256 / G))));
+    oap_ce_few<T, N, G><<<dim3(unsigned(blocks)), 256, 0, s>>>(f);
+    OAP_HIP_CHECK(hipGetLastError());
+    return blocks;
+  }
+  template <int N>
+  static int few_lanes(const FewArgs& f, hipStream_t s) {
+    const int per = kFewIters * gt_chunk<T>();  // features of a lane
+    if (f.dim <= 8 * per) return few_launch<N, 8>(f, s);
+    if (f.dim <= 16 * per) return few_launch<N, 16>(f, s);
+    if (f.dim <= 32 * per) return few_launch<N, 32>(f, s);
+    return few_launch<N, 64>(f, s);
+  }
+  static int few(const CeArgs& a, const Work& w, hipStream_t s) {
+    FewArgs f = {};
+    f.w = a.w;
+    f.x = a.x;
+    f.ldw = a.ldw;
+    f.ldx = a.ldx;
+    f.classes = a.classes;
+    f.n = int(a.n);
+    f.dim = a.dim;
+    f.bias = a.bias;
+    f.target = a.target;
+    f.part = w.part;
+    f.zt = w.zt;
+    return a.n == 1 ? few_lanes<1>(f, s) : few_lanes<kFewRows>(f, s);
   }
 
   template <int BM, int BN, int WAVES_M>
@@ -739,10 +913,14 @@ struct Ce {
       l.class0 = c0;
       l.vtiles = int(ceil_div(nc, p.bm));
       logits<true>(p, l, s);
-      if (p.dbn == 128)
-        products<256, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
-      else
-        products<256, 256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      if (p.dbm == 128)
+        products<128, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      else if constexpr (sizeof(T) == 2) {
+        if (p.dbn == 128)
+          products<256, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+        else
+          products<256, 256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      }
       if (db) {
         oap_ce_db<<<dim3(unsigned(ceil_div(nc, 256))), 256, 0, s>>>(w.dbpart, l.ntiles, p.piece,
                                                                      nc, w.gscale, db + c0);

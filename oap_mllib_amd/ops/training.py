@@ -28,7 +28,7 @@ def _float_tensor(name: str, t, dim: int | None = None):
         raise ValueError(f"{name}: expected a tensor, got {type(t).__name__}")
     if t.dtype not in _ELEM:
         raise ValueError(f"{name}: expected float32, bfloat16 or float16, got {t.dtype}")
-    if t.device.type not in ("cuda", "cpu") or t.layout != torch.strided:
+    if not (t.is_cuda or t.is_cpu) or t.layout != torch.strided:
         raise ValueError(f"{name}: expected a dense CPU or GPU tensor")
     if dim is not None and t.dim() != dim:
         raise ValueError(f"{name}: expected a {dim}-D tensor, got shape {tuple(t.shape)}")
@@ -61,7 +61,9 @@ def _ptr(t) -> int:
 def _where(t) -> tuple[int, int]:
     """(device, stream) of a native call; (-1, 0) is the host engine."""
     if t.is_cuda:
-        return t.device.index, torch.cuda.current_stream(t.device).cuda_stream
+        index = t.get_device()
+        # (the handle itself: a Stream object costs as much as a small op's launch)
+        return index, torch._C._cuda_getCurrentRawStream(index)
     return -1, 0
 
 
@@ -78,9 +80,16 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         wr, ldw = _rows(weight)
         n, d = x.shape
         v = weight.shape[0]
-        f32 = dict(dtype=torch.float32, device=x.device)
-        loss, stat = torch.empty(n, **f32), torch.empty((n, 2), **f32)
-        total = torch.empty((), **f32) if reduction != "none" else None
+        # per row: max and sum for the gradients, and the loss
+        rows = torch.empty(3 * n, dtype=torch.float32, device=x.device)
+        stat, loss = rows, rows.data_ptr() + 8 * n
+        out = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32,
+                          device=x.device)
+        total = 0
+        if reduction == "none":
+            loss = out.data_ptr()
+        else:
+            total = out.data_ptr()
         elem = _ELEM[x.dtype]
         dev, stream = _where(x)
         head = (elem, _ptr(xr), ldx, _ptr(wr), ldw, _ptr(bias))
@@ -88,11 +97,10 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         if dev >= 0:
             work = _work(native.softmax_ce_forward_bytes(*head, n, v, d), x)
         native.softmax_ce_forward(dev, stream, *head, _ptr(target), ignore_index, n, v, d,
-                                  _ptr(loss), _ptr(stat), _ptr(total), reduction == "mean",
-                                  _ptr(work))
+                                  loss, _ptr(stat), total, reduction == "mean", _ptr(work))
         ctx.save_for_backward(x, weight, bias, target, stat)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
-        return loss if total is None else total
+        return out
 
     @staticmethod
     @once_differentiable
@@ -131,7 +139,8 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
     ``target`` (n integers) holds the class of each row; rows with ``ignore_index`` have no loss
     and no gradient, whatever ``x`` holds there.  A class whose bias is ``-inf`` is left out: it
     has no probability and no gradient, whatever ``weight`` holds there, and a row whose target
-    it is has the loss ``inf`` and the gradient of the classes that are left.  A target that is
+    it is has the loss ``inf`` and the gradient of the classes that are left (finite biases below
+    -2.3e38 exclude nothing and count as equal).  A target that is
     no class and not ``ignore_index`` gives its row the loss NaN and no gradient.
 
     ``reduction``: "mean" over the rows that are not ignored (0 if all are), "sum" or "none"
@@ -150,10 +159,12 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
     if bias is not None:
         _float_tensor("bias", bias, 1)
         _same("bias", bias, x, (v,))
-        bias = bias.float().contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction: expected 'mean', 'sum' or 'none', got {reduction!r}")
-    target = target.detach().long().contiguous()
+    if target.dtype != torch.int64 or not target.is_contiguous():
+        target = target.long().contiguous()
     if not x.is_cuda and x.dtype != torch.float32:
         x, weight = x.float(), weight.float()
     return _SoftmaxCrossEntropy.apply(x, weight, bias, target, int(ignore_index), reduction)
@@ -161,7 +172,7 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
 
 # ----------------------------------------------------------------------------------- dropout
 def _drop(x, residual, p, seed, offset):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     dev, stream = _where(x)
     tensor = isinstance(seed, torch.Tensor)
     _loader.load().dropout(dev, stream, _ELEM[x.dtype], _ptr(x), _ptr(residual), _ptr(y),

@@ -48,24 +48,30 @@ __device__ inline float half_wave_sum(float v) {
 // ignore, or bias == -inf): an infinity or NaN there must not meet a coefficient of zero in the
 // gradients' products
 template <typename T>
-__global__ __launch_bounds__(256) void oap_ce_pack(const T* __restrict__ src, int64_t ld,
-                                                   int64_t rows, int dim, int dp,
-                                                   const int64_t* __restrict__ target,
-                                                   int64_t ignore,
-                                                   const float* __restrict__ bias,
-                                                   T* __restrict__ dst) {
+struct PackArgs {
+  const T* src;  // null: nothing to do
+  int64_t ld, rows;
+  int dim, dp;
+  const int64_t* target;
+  int64_t ignore;
+  const float* bias;
+  T* dst;
+};
+
+template <typename T>
+__device__ inline void pack_rows(const PackArgs<T>& a, int64_t first, int64_t stride) {
   constexpr int CH = gt_chunk<T>();
-  const int per = dp / CH;
-  const int64_t total = rows * per;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total;
-       i += int64_t(gridDim.x) * 256) {
+  const int per = a.dp / CH;
+  const int64_t total = a.rows * per;
+  for (int64_t i = first; i < total; i += stride) {
     const int64_t row = i / per;
     const int c = int(i - row * per) * CH;
-    const bool out = target ? target[row] == ignore : bias && bias[row] == -INFINITY;
+    const bool out = a.target ? a.target[row] == a.ignore : a.bias && a.bias[row] == -INFINITY;
     Vec16<T> o;
 #pragma unroll
-    for (int j = 0; j < CH; ++j) o.v[j] = !out && c + j < dim ? src[row * ld + c + j] : T(0.f);
-    *reinterpret_cast<Vec16<T>*>(dst + row * dp + c) = o;
+    for (int j = 0; j < CH; ++j)
+      o.v[j] = !out && c + j < a.dim ? a.src[row * a.ld + c + j] : T(0.f);
+    *reinterpret_cast<Vec16<T>*>(a.dst + row * a.dp + c) = o;
   }
 }
 
@@ -247,9 +253,10 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       }
     }
     T* out = static_cast<T*>(a.dz);
-    // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & 15), then
+    // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & SW), then
     // out in whole rows
     constexpr int CH = gt_chunk<T>(), CPR = BM / CH, ROW = BM * int(sizeof(T));
+    constexpr int SW = CPR < 16 ? CPR - 1 : 15;
     __syncthreads();
 #pragma unroll
     for (int ni = 0; ni < Tile::NI; ++ni)
@@ -264,14 +271,14 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
           for (int e = 0; e < 4; ++e)
             f.v[e] = static_cast<T>(acc[mi][ni][4 * g + e] * a.pscale);
           const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
-          *reinterpret_cast<Four*>(lds + j * ROW + (((i / CH) ^ (j & 15)) << 4) +
+          *reinterpret_cast<Four*>(lds + j * ROW + (((i / CH) ^ (j & SW)) << 4) +
                                    (i % CH) * int(sizeof(T))) = f;
         }
     __syncthreads();
     for (int c = tid; c < BN * CPR; c += kGtThreads) {
       const int j = c / CPR, k = c % CPR;
       *reinterpret_cast<float4*>(out + (int64_t(n0) + j) * a.vp + v0 + k * CH) =
-          *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & 15)) << 4));
+          *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & SW)) << 4));
     }
   }
 }
@@ -379,62 +386,25 @@ __global__ __launch_bounds__(256) void oap_ce_few(FewArgs a) {
 // Rows: (max, sum) of every class tile into the row's and the loss, log(sum) + (max - z_t): the
 // difference is formed first, so logits of any size keep the loss's own precision.  A workgroup
 // takes `cols` rows (a power of two) and shares the class tiles of each among its other threads.
-__global__ __launch_bounds__(1024) void oap_ce_rows(const float2* __restrict__ part, int vtiles,
-                                                    int64_t npad, int64_t n, int cols,
-                                                    const int64_t* __restrict__ target,
-                                                    int64_t ignore, int64_t classes,
-                                                    const float* __restrict__ zt,
-                                                    float* __restrict__ loss,
-                                                    float2* __restrict__ stat) {
-  __shared__ float2 red[1024];
-  const int c = threadIdx.x & (cols - 1), r0 = threadIdx.x / cols, nr = 1024 / cols;
-  const int64_t row = int64_t(blockIdx.x) * cols + c;
-  float m = -INFINITY, s = 0.f;
-  if (row < n) {
-    for (int t = r0; t < vtiles; t += nr) {
-      const float2 p = part[int64_t(t) * npad + row];
-      const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
-      s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
-      m = mm;
-    }
-  }
-  red[threadIdx.x] = make_float2(m, s);
-  for (int h = nr / 2; h >= 1; h >>= 1) {
-    __syncthreads();
-    if (r0 < h) {
-      const float2 p = red[threadIdx.x + h * cols];
-      const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
-      s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
-      m = mm;
-      red[threadIdx.x] = make_float2(m, s);
-    }
-  }
-  if (r0 == 0 && row < n) {
-    stat[row] = make_float2(m, s);
-    const int64_t t = target[row];
-    if (t == ignore)
-      loss[row] = 0.f;
-    else if (t < 0 || t >= classes)
-      loss[row] = NAN;
-    else
-      loss[row] = zt[row] == -INFINITY ? INFINITY : kLn2 * (log2f(s) + (m - zt[row]));
-  }
-}
+// A single workgroup goes over all rows and forms the total as well.
+struct RowArgs {
+  const float2* part;
+  int tiles;
+  int64_t npad, n;
+  int cols;
+  const int64_t* target;
+  int64_t ignore, classes;
+  const float* zt;
+  float* loss;
+  float2* stat;
+  float* total;  // null: none, or in a launch of its own
+  int mean;
+};
 
-// Sum (or mean over the rows that have a loss) in a fixed order, in fp64.
-__global__ __launch_bounds__(1024) void oap_ce_total(const float* __restrict__ loss,
-                                                     const int64_t* __restrict__ target,
-                                                     int64_t ignore, int64_t n, int mean,
-                                                     float* __restrict__ total) {
+// (sum, count) of the workgroup's threads in a fixed order, in fp64; into *total
+__device__ inline void total_of(double s, unsigned long long k, int mean, float* total) {
   __shared__ double red[1024];
   __shared__ unsigned long long cnt[1024];
-  double s = 0.0;
-  unsigned long long k = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024)
-    if (target[i] != ignore) {
-      s += double(loss[i]);
-      ++k;
-    }
   red[threadIdx.x] = s;
   cnt[threadIdx.x] = k;
   for (int h = 512; h >= 1; h >>= 1) {
@@ -447,23 +417,90 @@ __global__ __launch_bounds__(1024) void oap_ce_total(const float* __restrict__ l
   if (threadIdx.x == 0) *total = float(mean ? red[0] / double(cnt[0] ? cnt[0] : 1) : red[0]);
 }
 
+__global__ __launch_bounds__(1024) void oap_ce_rows(RowArgs a) {
+  __shared__ float2 red[1024];
+  const int cols = a.cols, c = threadIdx.x & (cols - 1), r0 = threadIdx.x / cols;
+  const int nr = 1024 / cols;
+  double sum = 0.0;
+  unsigned long long count = 0;
+  for (int64_t first = int64_t(blockIdx.x) * cols; first < a.n;
+       first += int64_t(gridDim.x) * cols) {
+    const int64_t row = first + c;
+    float m = -INFINITY, s = 0.f;
+    if (row < a.n) {
+      for (int t = r0; t < a.tiles; t += nr) {
+        const float2 p = a.part[int64_t(t) * a.npad + row];
+        const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
+        s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
+        m = mm;
+      }
+    }
+    __syncthreads();
+    red[threadIdx.x] = make_float2(m, s);
+    for (int h = nr / 2; h >= 1; h >>= 1) {
+      __syncthreads();
+      if (r0 < h) {
+        const float2 p = red[threadIdx.x + h * cols];
+        const float mm = fmaxf(m, p.x), ref = mm > -INFINITY ? mm : 0.f;
+        s = s * pow2(m - ref) + p.y * pow2(p.x - ref);
+        m = mm;
+        red[threadIdx.x] = make_float2(m, s);
+      }
+    }
+    if (r0 == 0 && row < a.n) {
+      a.stat[row] = make_float2(m, s);
+      const int64_t t = a.target[row];
+      float l;
+      if (t == a.ignore)
+        l = 0.f;
+      else if (t < 0 || t >= a.classes)
+        l = NAN;
+      else
+        l = a.zt[row] == -INFINITY ? INFINITY : kLn2 * (log2f(s) + (m - a.zt[row]));
+      a.loss[row] = l;
+      if (t != a.ignore) {
+        sum += double(l);
+        ++count;
+      }
+    }
+  }
+  if (gridDim.x == 1 && a.total) total_of(sum, count, a.mean, a.total);
+}
+
+// Sum (or mean over the rows that have a loss)
+__global__ __launch_bounds__(1024) void oap_ce_total(RowArgs a) {
+  double s = 0.0;
+  unsigned long long k = 0;
+  for (int64_t i = threadIdx.x; i < a.n; i += 1024)
+    if (a.target[i] != a.ignore) {
+      s += double(a.loss[i]);
+      ++k;
+    }
+  total_of(s, k, a.mean, a.total);
+}
+
 // Upstream gradient of every row as g_n = gscale * coef_n with |coef_n| <= 1: products of the
 // coefficient with a probability then fit 16 bits.  Rows without a loss (or with a target that
 // is no class) get the coefficient 0.
-__global__ __launch_bounds__(1024) void oap_ce_coef(const float* __restrict__ grad, int per_row,
-                                                    int mean, const int64_t* __restrict__ target,
-                                                    int64_t ignore, int64_t classes, int64_t n,
-                                                    float* __restrict__ coef,
-                                                    float* __restrict__ gscale) {
+struct CoefArgs {
+  const float* grad;  // null: nothing to do
+  int per_row, mean;
+  const int64_t* target;
+  int64_t ignore, classes, n;
+  float* coef;
+  float* gscale;
+};
+
+__device__ inline void coefficients(const CoefArgs& a) {
   __shared__ float red[1024];
   __shared__ unsigned long long cnt[1024];
   float m = 0.f;
   unsigned long long k = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    const int64_t t = target[i];
-    k += t != ignore;
-    if (per_row && t >= 0 && t < classes && t != ignore) {
-      const float g = fabsf(grad[i]);
+  for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+    const int64_t t = a.target[i];
+    k += t != a.ignore;
+    if (a.per_row && t >= 0 && t < a.classes && t != a.ignore) {
+      const float g = fabsf(a.grad[i]);
       m = g <= m ? m : g;  // (a NaN is kept)
     }
   }
@@ -480,12 +517,29 @@ __global__ __launch_bounds__(1024) void oap_ce_coef(const float* __restrict__ gr
   __syncthreads();
   const float top = red[0];
   if (threadIdx.x == 0)
-    *gscale = per_row ? top : mean ? grad[0] / float(cnt[0] ? cnt[0] : 1) : grad[0];
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    const int64_t t = target[i];
-    const bool has = t >= 0 && t < classes && t != ignore;
-    coef[i] = !has ? 0.f : per_row ? (top == 0.f ? 0.f : grad[i] / top) : 1.f;
+    *a.gscale =
+        a.per_row ? top : a.mean ? a.grad[0] / float(cnt[0] ? cnt[0] : 1) : a.grad[0];
+  for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
+    const int64_t t = a.target[i];
+    const bool has = t >= 0 && t < a.classes && t != a.ignore;
+    a.coef[i] = !has ? 0.f : a.per_row ? (top == 0.f ? 0.f : a.grad[i] / top) : 1.f;
   }
+}
+
+// What a launch of logits reads: the rows' coefficients (workgroup 0), the image of x and that
+// of the piece's classes (shares of the other workgroups), in one launch.
+template <typename T>
+__global__ __launch_bounds__(1024) void oap_ce_prepare(CoefArgs coef, PackArgs<T> x,
+                                                       PackArgs<T> w) {
+  if (coef.grad && blockIdx.x == 0) {
+    coefficients(coef);
+    return;
+  }
+  const int skip = coef.grad ? 1 : 0;
+  const int64_t first = int64_t(blockIdx.x - skip) * 1024 + threadIdx.x;
+  const int64_t stride = int64_t(gridDim.x - skip) * 1024;
+  if (x.src) pack_rows(x, first, stride);
+  if (w.src) pack_rows(w, first, stride);
 }
 
 // ------------------------------------------------------------------------------------- products
@@ -538,17 +592,39 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dx(Pr
     }
 }
 
-template <typename S>
-__global__ __launch_bounds__(256) void oap_ce_dx_out(const float* __restrict__ slab, int splits,
-                                                     int64_t count,
-                                                     const float* __restrict__ gscale,
-                                                     float unscale, S* __restrict__ dx) {
-  const float g = *gscale * unscale;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count;
-       i += int64_t(gridDim.x) * 256) {
+// What is left of a piece: db of its classes (the first workgroups), and after the last piece the
+// slabs of dx into the result.
+template <typename T>
+struct FinishArgs {
+  const float* gscale;
+  const float* dbpart;  // [row tile][vp], or null
+  int rtiles;
+  int64_t vp, classes;
+  float* db;
+  const float* slab;  // [split][count], or null
+  int splits;
+  int64_t count;
+  float unscale;
+  T* dx;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void oap_ce_finish(FinishArgs<T> a) {
+  const int dbblocks = a.dbpart ? int((a.classes + 255) / 256) : 0;
+  const float g = *a.gscale;
+  if (int(blockIdx.x) < dbblocks) {
+    const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (v >= a.classes) return;
+    float s = 0.f;
+    for (int t = 0; t < a.rtiles; ++t) s += a.dbpart[int64_t(t) * a.vp + v];
+    a.db[v] = s * g;
+    return;
+  }
+  for (int64_t i = int64_t(blockIdx.x - dbblocks) * 256 + threadIdx.x; i < a.count;
+       i += int64_t(gridDim.x - dbblocks) * 256) {
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += slab[int64_t(s) * count + i];
-    dx[i] = static_cast<S>(v * g);
+    for (int s = 0; s < a.splits; ++s) v += a.slab[int64_t(s) * a.count + i];
+    a.dx[i] = static_cast<T>(v * (g * a.unscale));
   }
 }
 
@@ -579,17 +655,6 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dw(Pr
     }
 }
 
-__global__ __launch_bounds__(256) void oap_ce_db(const float* __restrict__ part, int ntiles,
-                                                 int64_t vp, int64_t classes,
-                                                 const float* __restrict__ gscale,
-                                                 float* __restrict__ db) {
-  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (v >= classes) return;
-  float s = 0.f;
-  for (int t = 0; t < ntiles; ++t) s += part[int64_t(t) * vp + v];
-  db[v] = s * *gscale;
-}
-
 template <typename S>
 __global__ __launch_bounds__(256) void oap_ce_fill0(S* __restrict__ p, int64_t count) {
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count;
@@ -604,7 +669,7 @@ struct Plan {
   int bm, bn;               // class and row tile of the logits
   int64_t npad;
   int64_t piece;            // classes per piece, a multiple of 256
-  int dbm, dbn;             // row (or class) and feature tile of dx and dW
+  int xtile, wtile;         // square tiles of dx and dW
   int splits;
 };
 
@@ -625,7 +690,11 @@ constexpr int64_t kPieceBytes = int64_t(1) << 30;
 // any size (1024 x 2M x 100: 19.9 against 24.4 ms); in 16 bits the small ones are faster while
 // the epilogue weighs (forward and gradients, bf16: 3000 x 20000 x 784 0.66 against 0.68 ms,
 // 4096 x 65536 x 512 1.44 against 1.52 ms; 8192 x 131072 x 2048 18.9 against 16.6 ms).
-bool small_tiles(const CeArgs& a) { return a.elem == Elem::F32 || a.dim <= 1024; }
+// Where tiles of 128 leave CUs empty, tiles of 64 finish sooner.
+int tile_of(const CeArgs& a, int64_t rows, int64_t cols) {
+  if (ceil_div(rows, 128) * ceil_div(cols, 128) < 192) return 64;
+  return a.elem == Elem::F32 || a.dim <= 1024 ? 128 : 256;
+}
 
 Plan make_plan(const CeArgs& a, bool grad) {
   Plan p;
@@ -634,9 +703,9 @@ Plan make_plan(const CeArgs& a, bool grad) {
   // (the gradients read images in which the rows that are left out are zero)
   p.x_direct = !grad && direct(a, a.x, a.ldx);
   p.w_direct = direct(a, a.w, a.ldw) && !(grad && a.bias);
-  const bool narrow = small_tiles(a);
-  p.bm = a.n > 64 && narrow ? 128 : 256;
-  p.bn = a.n <= 64 ? 64 : narrow ? 128 : 256;
+  p.bm = tile_of(a, a.classes, a.n);
+  p.bn = a.n <= 64 ? 64 : p.bm;
+  if (p.bn == 64 && p.bm > 64) p.bm = 256;  // few rows of many classes
   p.npad = int64_t(round_up(size_t(a.n), size_t(p.bn)));
   const int64_t vpad = int64_t(round_up(size_t(a.classes), 256));
   int64_t per = p.dp;  // elements per class of the largest image
@@ -644,10 +713,16 @@ Plan make_plan(const CeArgs& a, bool grad) {
   p.piece = kPieceBytes / (per * es) / 256 * 256;
   if (!grad && p.w_direct) p.piece = vpad;
   p.piece = std::max<int64_t>(256, std::min({p.piece, vpad, int64_t(1) << 20}));
-  p.dbm = narrow ? 128 : 256;
-  p.dbn = a.dim <= 128 || narrow ? 128 : 256;
-  const int64_t tiles = ceil_div(a.n, p.dbm) * ceil_div(a.dim, p.dbn);
-  const int64_t by_k = std::max<int64_t>(1, p.piece / 256);  // at least 256 classes a split
+  p.wtile = tile_of(a, std::min(p.piece, a.classes), a.dim);
+  // dx: two workgroups per CU between the tiles and the splits of k, of at least 256 classes (128
+  // where even so there are few)
+  p.xtile = a.elem == Elem::F32 || a.dim <= 1024 ? 128 : 256;
+  int64_t tiles = ceil_div(a.n, p.xtile) * ceil_div(a.dim, p.xtile), by_k = p.piece / 256;
+  if (a.n <= 64 || tiles * by_k < 192) {
+    p.xtile = 64;
+    tiles = ceil_div(a.n, 64) * ceil_div(a.dim, 64);
+    by_k = p.piece / 128;
+  }
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>(by_k, 512 / tiles)));
   return p;
 }
@@ -688,11 +763,17 @@ unsigned stride_grid(int64_t threads) {
 
 template <typename T>
 struct Ce {
-  static void pack(const void* src, int64_t ld, int64_t rows, int dim, int64_t dp,
-                   const int64_t* target, int64_t ignore, const float* bias, T* dst,
-                   hipStream_t s) {
-    oap_ce_pack<T><<<stride_grid(rows * dp / gt_chunk<T>()), 256, 0, s>>>(
-        static_cast<const T*>(src), ld, rows, dim, int(dp), target, ignore, bias, dst);
+  static PackArgs<T> pack(const void* src, int64_t ld, int64_t rows, const CeArgs& a, int64_t dp,
+                          const int64_t* target, const float* bias, T* dst) {
+    return {static_cast<const T*>(src), ld, rows, a.dim, int(dp), target, a.ignore, bias, dst};
+  }
+  static void prepare(const CoefArgs& coef, const PackArgs<T>& x, const PackArgs<T>& w,
+                      hipStream_t s) {
+    if (!coef.grad && !x.src && !w.src) return;
+    const int64_t items = std::max(x.src ? x.rows * x.dp : 0, w.src ? w.rows * w.dp : 0);
+    const int64_t blocks = std::min<int64_t>(ceil_div(items, 1024 * gt_chunk<T>()), 2048);
+    oap_ce_prepare<T><<<dim3(unsigned(std::max<int64_t>(1, blocks + (coef.grad ? 1 : 0)))), 1024,
+                        0, s>>>(coef, x, w);
     OAP_HIP_CHECK(hipGetLastError());
   }
 
@@ -707,7 +788,9 @@ struct Ce {
 
   template <bool GRAD>
   static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
-    if (p.bn == 64)
+    if (p.bm == 64)
+      logits_tile<64, 64, 2, GRAD>(l, s);
+    else if (p.bn == 64)
       logits_tile<256, 64, 4, GRAD>(l, s);
     else if (p.bn == 128)
       logits_tile<128, 128, 2, GRAD>(l, s);
@@ -761,9 +844,10 @@ struct Ce {
     }
     const T* wt = static_cast<const T*>(a.w);
     LogitArgs l = {};
+    PackArgs<T> px = {}, pw = {};
     l.x = {a.x, a.ldx, a.n, p.dp};
     if (!p.x_direct) {
-      pack(a.x, a.ldx, a.n, a.dim, p.dp, nullptr, 0, nullptr, w.ximg, s);
+      px = pack(a.x, a.ldx, a.n, a, p.dp, nullptr, nullptr, w.ximg);
       l.x = {w.ximg, p.dp, a.n, p.dp};
     }
     l.dp = p.dp;
@@ -776,9 +860,11 @@ struct Ce {
       const int64_t nc = std::min(p.piece, a.classes - c0);
       l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp};
       if (!p.w_direct) {
-        pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, nullptr, w.wimg, s);
+        pw = pack(wt + c0 * a.ldw, a.ldw, nc, a, p.dp, nullptr, nullptr, w.wimg);
         l.w = {w.wimg, p.dp, nc, p.dp};
       }
+      prepare({}, px, pw, s);
+      px.src = nullptr;
       l.bias = a.bias ? a.bias + c0 : nullptr;
       l.class0 = c0;
       l.vtiles = int(ceil_div(nc, p.bm));
@@ -788,17 +874,19 @@ struct Ce {
     rows(a, w, int(ceil_div(a.classes, p.bm)), p.npad, loss, stat, total, mean, s);
   }
 
-  // (few rows of many class tiles: fewer rows per workgroup, at least one per CU)
+  // One workgroup for little work (the total needs no launch of its own then), else at least one
+  // per CU.
   static void rows(const CeArgs& a, const Work& w, int tiles, int64_t npad, float* loss,
                    float2* stat, float* total, bool mean, hipStream_t s) {
-    int cols = 1;
-    while (cols < 64 && cols * 256 < a.n) cols *= 2;
-    if (a.n >= 8) cols = std::max(cols, 8);
-    oap_ce_rows<<<dim3(unsigned(ceil_div(a.n, cols))), 1024, 0, s>>>(
-        w.part, tiles, npad, a.n, cols, a.target, a.ignore, a.classes, w.zt, loss, stat);
+    RowArgs r = {w.part, tiles, npad, a.n,  1,     a.target, a.ignore, a.classes,
+                 w.zt,   loss,  stat, total, mean};
+    const bool one = a.n * tiles <= 16384;
+    while (r.cols < 64 && r.cols * (one ? 1 : 256) < a.n) r.cols *= 2;
+    if (a.n >= 8) r.cols = std::max(r.cols, 8);
+    oap_ce_rows<<<dim3(one ? 1 : unsigned(ceil_div(a.n, r.cols))), 1024, 0, s>>>(r);
     OAP_HIP_CHECK(hipGetLastError());
-    if (total) {
-      oap_ce_total<<<1, 1024, 0, s>>>(loss, a.target, a.ignore, a.n, mean, total);
+    if (total && !one && ceil_div(a.n, r.cols) > 1) {
+      oap_ce_total<<<1, 1024, 0, s>>>(r);
       OAP_HIP_CHECK(hipGetLastError());
     }
   }
@@ -835,41 +923,62 @@ struct Ce {
     return a.n == 1 ? few_lanes<1>(f, s) : few_lanes<kFewRows>(f, s);
   }
 
-  template <int BM, int BN, int WAVES_M>
+  template <int B>
+  static void dx_tile(const ProdArgs& g, hipStream_t s) {
+    constexpr int lds = GtTile<T, B, kAlongK, B, kAcrossK, 2>::kLds;
+    auto k = oap_ce_dx<T, B, B, 2>;
+    set_lds(k, lds);
+    k<<<dim3(unsigned(g.mtiles * g.ntiles * g.splits)), kGtThreads, lds, s>>>(g);
+    OAP_HIP_CHECK(hipGetLastError());
+  }
+  template <int B>
+  static void dw_tile(const ProdArgs& g, hipStream_t s) {
+    constexpr int lds = GtTile<T, B, kAcrossK, B, kAcrossK, 2>::kLds;
+    auto k = oap_ce_dw<T, B, B, 2>;
+    set_lds(k, lds);
+    k<<<dim3(unsigned(g.mtiles * g.ntiles)), kGtThreads, lds, s>>>(g);
+    OAP_HIP_CHECK(hipGetLastError());
+  }
+
   static void products(const CeArgs& a, const Plan& p, const Work& w, const LogitArgs& l,
                        int64_t nc, int64_t c0, float unscale, void* dx, void* dw,
                        hipStream_t s) {
-    constexpr int lds = GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M>::kLds;
     ProdArgs g = {};
-    g.ntiles = int(ceil_div(a.dim, BN));
     g.n = a.dim;
     g.gscale = w.gscale;
     g.unscale = unscale;
     g.a = {w.dz, p.piece, p.npad, p.piece};
     if (dx) {
-      auto k = oap_ce_dx<T, BM, BN, WAVES_M>;
-      set_lds(k, lds);
       g.b = l.w;
       g.k = nc;
       g.m = a.n;
-      g.mtiles = int(ceil_div(a.n, BM));
+      g.mtiles = int(ceil_div(a.n, p.xtile));
+      g.ntiles = int(ceil_div(a.dim, p.xtile));
       g.splits = p.splits;
       g.out = w.slab;
       g.add = c0 > 0;
-      k<<<dim3(unsigned(g.mtiles * g.ntiles * g.splits)), kGtThreads, lds, s>>>(g);
-      OAP_HIP_CHECK(hipGetLastError());
+      if (p.xtile == 64)
+        dx_tile<64>(g, s);
+      else if (p.xtile == 128)
+        dx_tile<128>(g, s);
+      else if constexpr (sizeof(T) == 2)
+        dx_tile<256>(g, s);
     }
     if (dw) {
-      auto k = oap_ce_dw<T, BM, BN, WAVES_M>;
-      set_lds(k, lds);
       g.b = l.x;
       g.k = a.n;
       g.m = nc;
-      g.mtiles = int(ceil_div(nc, BM));
+      g.mtiles = int(ceil_div(nc, p.wtile));
+      g.ntiles = int(ceil_div(a.dim, p.wtile));
+      g.splits = 1;
       g.out = static_cast<T*>(dw) + c0 * a.dim;
       g.bias = a.bias ? a.bias + c0 : nullptr;
-      k<<<dim3(unsigned(g.mtiles * g.ntiles)), kGtThreads, lds, s>>>(g);
-      OAP_HIP_CHECK(hipGetLastError());
+      if (p.wtile == 64)
+        dw_tile<64>(g, s);
+      else if (p.wtile == 128)
+        dw_tile<128>(g, s);
+      else if constexpr (sizeof(T) == 2)
+        dw_tile<256>(g, s);
     }
   }
 
@@ -881,15 +990,11 @@ struct Ce {
     const T* wt = static_cast<const T*>(a.w);
     // fp16 images hold dz times 2^14: |dz| <= 1 stays finite and 2^-28 is still a normal number
     const float pscale = a.elem == Elem::F16 ? 0x1p14f : 1.f;
-    oap_ce_coef<<<1, 1024, 0, s>>>(grad, per_row, mean, a.target, a.ignore, a.classes, a.n,
-                                   w.coef, w.gscale);
-    OAP_HIP_CHECK(hipGetLastError());
+    const CoefArgs coef = {grad, per_row, mean, a.target, a.ignore, a.classes, a.n, w.coef,
+                           w.gscale};
     LogitArgs l = {};
-    l.x = {a.x, a.ldx, a.n, p.dp};
-    if (!p.x_direct) {
-      pack(a.x, a.ldx, a.n, a.dim, p.dp, a.target, a.ignore, nullptr, w.ximg, s);
-      l.x = {w.ximg, p.dp, a.n, p.dp};
-    }
+    PackArgs<T> px = pack(a.x, a.ldx, a.n, a, p.dp, a.target, nullptr, w.ximg), pw = {};
+    l.x = {w.ximg, p.dp, a.n, p.dp};
     l.dp = p.dp;
     l.target = a.target;
     l.n = a.n;
@@ -903,34 +1008,43 @@ struct Ce {
     l.dbpart = w.dbpart;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
+      const bool last = c0 + nc == a.classes;
       const float* bias = a.bias ? a.bias + c0 : nullptr;
       l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp};
       if (!p.w_direct) {
-        pack(wt + c0 * a.ldw, a.ldw, nc, a.dim, p.dp, nullptr, 0, bias, w.wimg, s);
+        pw = pack(wt + c0 * a.ldw, a.ldw, nc, a, p.dp, nullptr, bias, w.wimg);
         l.w = {w.wimg, p.dp, nc, p.dp};
       }
+      prepare(c0 ? CoefArgs{} : coef, px, pw, s);
+      px.src = nullptr;
       l.bias = bias;
       l.class0 = c0;
       l.vtiles = int(ceil_div(nc, p.bm));
       logits<true>(p, l, s);
-      if (p.dbm == 128)
-        products<128, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
-      else if constexpr (sizeof(T) == 2) {
-        if (p.dbn == 128)
-          products<256, 128, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
-        else
-          products<256, 256, 2>(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
-      }
+      products(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
+      FinishArgs<T> f = {};
+      f.gscale = w.gscale;
+      int64_t blocks = 0;
       if (db) {
-        oap_ce_db<<<dim3(unsigned(ceil_div(nc, 256))), 256, 0, s>>>(w.dbpart, l.ntiles, p.piece,
-                                                                     nc, w.gscale, db + c0);
+        f.dbpart = w.dbpart;
+        f.rtiles = l.ntiles;
+        f.vp = p.piece;
+        f.classes = nc;
+        f.db = db + c0;
+        blocks = ceil_div(nc, 256);
+      }
+      if (dx && last) {
+        f.slab = w.slab;
+        f.splits = p.splits;
+        f.count = a.n * a.dim;
+        f.unscale = 1.f / pscale;
+        f.dx = static_cast<T*>(dx);
+        blocks += stride_grid(f.count);
+      }
+      if (blocks > 0) {
+        oap_ce_finish<T><<<dim3(unsigned(blocks)), 256, 0, s>>>(f);
         OAP_HIP_CHECK(hipGetLastError());
       }
-    }
-    if (dx) {
-      oap_ce_dx_out<T><<<stride_grid(a.n * a.dim), 256, 0, s>>>(
-          w.slab, p.splits, a.n * a.dim, w.gscale, 1.f / pscale, static_cast<T*>(dx));
-      OAP_HIP_CHECK(hipGetLastError());
     }
   }
 

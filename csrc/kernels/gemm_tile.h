@@ -1,8 +1,8 @@
 // Tile core of the products of the softmax cross entropy: C[m, n] = sum_k A(m, k) B(n, k) on the
-// matrix units, in bf16 or fp16 (v_mfma_f32_32x32x16) or fp32 (v_mfma_f32_32x32x2), with fp32
-// sums.  Each operand lies in memory either with k along its rows (kAlongK: element (r, k) at
-// r * ld + k) or with k across them (kAcrossK: at k * ld + r), so no operand is ever transposed
-// in memory.
+// matrix units, in bf16 or fp16 (v_mfma_f32_32x32x16), in fp32 (v_mfma_f32_32x32x2) or in fp32 as
+// two fp16 numbers (GtSplit), with fp32 sums.  Each operand lies in memory either with k along its
+// rows (kAlongK: element (r, k) at r * ld + k) or with k across them (kAcrossK: at k * ld + r), so
+// no operand is ever transposed in memory.
 //
 // A workgroup of 4 waves, one per SIMD, owns a BM x BN tile; a wave's part of up to 128 x 128
 // keeps 256 accumulators, so a byte read from LDS feeds the most MFMAs.  k advances in blocks of
@@ -17,6 +17,13 @@
 //    k of r = i.  Two reads make a fragment.  The 64-byte granule of a row is xor-ed with bits
 //    of k, so the four k rows of a read use different banks.
 //  * kAcrossK, fp32: 32 rows of k, read by ds_read_b32 (32 lanes along a row).
+//
+// GtSplit: a matrix scaled by a power of two so that its largest magnitude lies in [2^14, 2^15),
+// each number the sum of two fp16, h + l.  A product is l h + h l + h h: it leaves out l l and
+// the rounding of l, each below 2^-22 of the product, and numbers below 2^-15 of the matrix's
+// largest keep an absolute error of 2^-40 of that.  Three 16-bit MFMAs take a fifth of the time
+// of the fp32 ones.  A row lies as runs of 32 numbers, their 32 h and then their 32 l, so 128
+// bytes of a row hold 32 k in either order of k.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -50,6 +57,16 @@ template <>
 struct GtFrag<float> {
   typedef gt_f32x4 type;
 };
+struct GtSplit {
+  _Float16 h, l;
+};
+struct gt_split8 {
+  gt_f16x8 h, l;
+};
+template <>
+struct GtFrag<GtSplit> {
+  typedef gt_split8 type;
+};
 
 __device__ inline gt_f32x16 gt_mfma(gt_bf16x8 a, gt_bf16x8 b, gt_f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -62,6 +79,21 @@ __device__ inline gt_f32x16 gt_mfma(gt_f32x4 a, gt_f32x4 b, gt_f32x16 c) {
   for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
   return c;
 }
+
+__device__ inline gt_f32x16 gt_mfma(const gt_split8& a, const gt_split8& b, gt_f32x16 c) {
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, b.h, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.l, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+}
+template <typename T>
+constexpr bool gt_is_split = false;
+template <>
+constexpr bool gt_is_split<GtSplit> = true;
+// steps of k per block, and MFMAs of a step's 32 x 32 product
+template <typename T>
+constexpr int gt_steps = gt_is_split<T> ? 2 : 4;
+template <typename T>
+constexpr int gt_mfmas = gt_is_split<T> ? 3 : sizeof(T) == 4 ? 4 : 1;
 
 constexpr int kGtThreads = 256;  // 4 waves
 // waves per SIMD that a tile's registers allow
@@ -77,10 +109,10 @@ constexpr int gt_chunk() {
   return 16 / int(sizeof(T));
 }
 
-// `rows` x `cols` elements in memory, row stride `ld`; cols and ld are multiples of a chunk and
-// p is 16-byte aligned.  256 rows span less than 2^31 bytes.  k beyond the extent of the operand
-// reads as 0; rows beyond `rows` (kAlongK) or columns beyond `cols` (kAcrossK) read as some
-// others, and the results they belong to are the caller's to leave out.
+// `rows` x `cols` elements in memory, row stride `ld`; cols and ld are multiples of a chunk
+// (GtSplit: of 32) and p is 16-byte aligned.  256 rows span less than 2^31 bytes.  k beyond the
+// extent of the operand reads as 0; rows beyond `rows` (kAlongK) or columns beyond `cols`
+// (kAcrossK) read as some others, and the results they belong to are the caller's to leave out.
 struct GtOperand {
   const void* p;
   int64_t ld;
@@ -98,15 +130,17 @@ struct GtSide {
   static constexpr int kChunks = R / CH;                // chunks of a k row (kAcrossK)
   static constexpr int kRowBytes = R * int(sizeof(T));  // of a k row (kAcrossK)
   static constexpr int kStep = ORDER == kAlongK ? kGtThreads / 8 : kGtThreads / kChunks;
+  static constexpr bool kSplit = gt_is_split<T>;
+  static constexpr bool kTransposed = ORDER == kAcrossK && (sizeof(T) == 2 || kSplit);
   // LDS reads of a fragment
-  static constexpr int kReads = ORDER == kAlongK ? 1 : sizeof(T) == 4 ? 4 : 2;
+  static constexpr int kReads = (ORDER == kAlongK ? 1 : kTransposed ? 2 : 4) * (kSplit ? 2 : 1);
   typedef typename GtFrag<T>::type Frag;
   static_assert(kLoads >= 1, "a thread stages at least 16 bytes of each operand");
 
   // xor on the chunk index of k row r
   __device__ static int swizzle(int r) {
-    if (sizeof(T) == 4) return 0;
-    return R >= 256 ? (r & 7) << 2 : R == 128 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
+    if (!kTransposed) return 0;
+    return kRowBytes >= 512 ? (r & 7) << 2 : kRowBytes == 256 ? (r & 3) << 2 : ((r >> 1) & 1) << 2;
   }
 
   // The thread's loads: rows r, r + kStep, ... of a block (rows of the tile, or rows of k)
@@ -131,7 +165,7 @@ struct GtSide {
           off[i] = uint32_t(q < last ? q : last) * ldb + chunk * 16;
         }
         left = int((k1 < o.cols ? k1 : o.cols) - k0);
-        sub = chunk * CH;
+        sub = kSplit ? 0 : chunk * CH;
         lds = r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
       } else {
         const int k = t / kChunks, chunk = t % kChunks;
@@ -172,43 +206,65 @@ struct GtSide {
   // Fragments of the rows base + 32 i
   template <int N>
   struct Reader {
-    static constexpr int kOffs = ORDER == kAcrossK && sizeof(T) == 2 ? N : 1;
-    int off[kOffs][2];
+    static constexpr int kOffs = kTransposed ? N : 1, kPlanes = kSplit ? 2 : 1;
+    int off[kOffs][kPlanes][2];
     int x7;
     __device__ void init(int lane, int base) {
       if (ORDER == kAlongK) {
-        off[0][0] = (base + (lane & 31)) * 128;
+        off[0][0][0] = (base + (lane & 31)) * 128;
         x7 = (lane >> 1) & 7;
-      } else if (sizeof(T) == 4) {
-        off[0][0] = 4 * (lane >> 5) * kRowBytes + (base + (lane & 31)) * 4;
+      } else if (!kTransposed) {
+        off[0][0][0] = 4 * (lane >> 5) * kRowBytes + (base + (lane & 31)) * 4;
       } else {
         const int g = lane >> 4, s = lane & 15;
 #pragma unroll
         for (int i = 0; i < kOffs; ++i)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int k = 8 * (g >> 1) + (s >> 2) + 4 * q;
-            const int chunk = (base + 32 * i + 16 * (g & 1)) / 8 + ((s & 3) >> 1);
-            off[i][q] = k * kRowBytes + ((chunk ^ swizzle(k)) << 4) + (s & 1) * 8;
-          }
+          for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int k = 8 * (g >> 1) + (s >> 2) + 4 * q;
+              const int first = (base + 32 * i) / 8 * kPlanes + 4 * p;  // chunk of the run
+              const int chunk = first + 2 * (g & 1) + ((s & 3) >> 1);
+              off[i][p][q] = k * kRowBytes + ((chunk ^ swizzle(k)) << 4) + (s & 1) * 8;
+            }
       }
+    }
+    template <typename V>
+    __device__ static V transposed(const char* lo, const char* hi) {
+      const gt_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)lo);
+      const gt_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)hi);
+      const gt_s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      return __builtin_bit_cast(V, v);
     }
     __device__ Frag read(const char* block, int i, int ks, int lane) const {
       if constexpr (ORDER == kAlongK) {
-        const int slot = ((2 * ks + (lane >> 5)) ^ x7) << 4;
-        return *reinterpret_cast<const Frag*>(block + off[0][0] + slot + i * 32 * 128);
-      } else if constexpr (sizeof(T) == 4) {
-        const char* p = block + off[0][0] + ks * 8 * kRowBytes + i * 32 * 4;
+        const char* p = block + off[0][0][0] + i * 32 * 128;
+        const int c = 2 * ks + (lane >> 5);
+        if constexpr (kSplit) {
+          Frag f;
+          f.h = *reinterpret_cast<const gt_f16x8*>(p + ((c ^ x7) << 4));
+          f.l = *reinterpret_cast<const gt_f16x8*>(p + (((c + 4) ^ x7) << 4));
+          return f;
+        } else {
+          return *reinterpret_cast<const Frag*>(p + ((c ^ x7) << 4));
+        }
+      } else if constexpr (!kTransposed) {
+        const char* p = block + off[0][0][0] + ks * 8 * kRowBytes + i * 32 * 4;
         Frag f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(p + j * kRowBytes);
         return f;
       } else {
         const char* p = block + ks * 16 * kRowBytes;
-        const gt_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)(p + off[i][0]));
-        const gt_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gt_lds_s16x4)(p + off[i][1]));
-        const gt_s16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        return __builtin_bit_cast(Frag, v);
+        if constexpr (kSplit) {
+          Frag f;
+          f.h = transposed<gt_f16x8>(p + off[i][0][0], p + off[i][0][1]);
+          f.l = transposed<gt_f16x8>(p + off[i][1][0], p + off[i][1][1]);
+          return f;
+        } else {
+          return transposed<Frag>(p + off[i][0][0], p + off[i][0][1]);
+        }
       }
     }
   };
@@ -229,7 +285,7 @@ struct GtTile {
   static constexpr int kLds = 2 * kBuf;
   // the last block apart, with only its occupied steps (the largest tiles' registers do not have
   // room for a second copy of the loop's body, and their k is long)
-  static constexpr bool kTail = gt_occupancy(BM, BN) > 1;
+  static constexpr bool kTail = gt_occupancy(BM, BN) > 1 && !gt_is_split<T>;
   typedef typename GtFrag<T>::type Frag;
   static_assert(MI >= 1 && NI >= 1, "tile");
 
@@ -238,7 +294,7 @@ struct GtTile {
   // left to itself the compiler reads a fragment just before its use and waits for it.
   template <bool LOADS, bool STORES>
   __device__ static void interleave() {
-    constexpr int kMfmas = MI * NI * (sizeof(T) == 4 ? 4 : 1);
+    constexpr int kMfmas = MI * NI * gt_mfmas<T>;
     constexpr int kReads = SideA::kReads * MI + SideB::kReads * NI;
     constexpr int kMoves = SideA::kLoads + SideB::kLoads;
     constexpr int G = kMfmas < 8 ? kMfmas : 8;
@@ -288,8 +344,32 @@ struct GtTile {
     gb.load(vb);
     ga.store(lds, va);
     gb.store(lds + SideA::kBytes, vb);
+    if constexpr (gt_is_split<T>) {
+      ga.load(va);
+      gb.load(vb);
+    }
     __syncthreads();
     fetch(lds, 0, 0);
+    if constexpr (gt_is_split<T>) {
+      // two short steps a block: the loads are issued behind the barrier, a block ahead
+      for (int it = 0; it < nk; ++it) {
+        const char* cur = lds + (it & 1) * kBuf;
+        char* nxt = lds + ((it + 1) & 1) * kBuf;
+        fetch(cur, 1, 1);
+        multiply(0);
+        ga.store(nxt, va);
+        gb.store(nxt + SideA::kBytes, vb);
+        interleave<false, true>();
+        __syncthreads();
+        fetch(nxt, 0, 0);
+        ga.load(va);
+        gb.load(vb);
+        multiply(1);
+        interleave<true, false>();
+      }
+      __syncthreads();
+      return;
+    }
     // (the loads beyond the range give zeros that are staged unread: no branch)
     for (int it = 0; it < (kTail ? nk - 1 : nk); ++it) {
       const char* cur = lds + (it & 1) * kBuf;

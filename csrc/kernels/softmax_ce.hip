@@ -62,7 +62,26 @@ struct PackArgs {
   int64_t ignore;
   const float* bias;
   void* dst;
+  int lanes;  // log2 of the lanes of a row
+  bool vec;   // rows of src are 16-byte aligned
 };
+
+// Eight numbers of a row from column c on, zero beyond its end
+template <typename T>
+__device__ inline void load8(const PackArgs<T>& a, int64_t row, int c, T (&v)[8]) {
+  const T* p = a.src + row * a.ld + c;
+  if (a.vec && c + 8 <= a.dim) {
+#pragma unroll
+    for (int q = 0; q < 8; q += Vec16<T>::n) {
+      const Vec16<T> o = *reinterpret_cast<const Vec16<T>*>(p + q);
+#pragma unroll
+      for (int j = 0; j < Vec16<T>::n; ++j) v[q + j] = o.v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < a.dim ? p[j] : T(0.f);
+  }
+}
 
 template <typename T>
 __device__ inline bool left_out_row(const PackArgs<T>& a, int64_t row) {
@@ -82,16 +101,19 @@ __device__ inline int scale_exponent(float top) {
 
 template <typename T>
 __device__ inline float largest(const PackArgs<T>& a, int block, int blocks) {
-  // a wave per row and turn
-  const int lane = threadIdx.x & 63;
-  const int64_t w0 = (int64_t(block) * blockDim.x + threadIdx.x) >> 6;
-  const int64_t ws = (int64_t(blocks) * blockDim.x) >> 6;
+  const int64_t t = int64_t(block) * blockDim.x + threadIdx.x;
+  const int lane = int(t & ((1 << a.lanes) - 1));
   float m = 0.f;
-  for (int64_t row = w0; row < a.rows; row += ws) {
+  for (int64_t row = t >> a.lanes; row < a.rows; row += int64_t(blocks) * blockDim.x >> a.lanes) {
     if (left_out_row(a, row)) continue;
-    for (int c = lane; c < a.dim; c += 64) {
-      const float v = fabsf(static_cast<float>(a.src[row * a.ld + c]));
-      m = v > m && v < INFINITY ? v : m;
+    for (int c = lane * 8; c < a.dim; c += 8 << a.lanes) {
+      T v[8];
+      load8(a, row, c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = fabsf(static_cast<float>(v[j]));
+        m = x > m && x < INFINITY ? x : m;
+      }
     }
   }
   return m;
@@ -124,34 +146,37 @@ __global__ __launch_bounds__(1024) void oap_ce_largest(PackArgs<T> x, PackArgs<T
   }
 }
 
+// the share of thread t of `threads`
 template <typename T, typename I>
-__device__ inline void pack_rows(const PackArgs<T>& a, float scale, int64_t first,
-                                 int64_t stride) {
-  constexpr int CH = gt_is_split<I> ? 8 : gt_chunk<T>();
-  const int per = a.dp / CH;
-  const int64_t total = a.rows * per;
-  for (int64_t i = first; i < total; i += stride) {
-    const int64_t row = i / per;
-    const int c = int(i - row * per) * CH;
+__device__ inline void pack_rows(const PackArgs<T>& a, float scale, int64_t t, int64_t threads) {
+  const int lane = int(t & ((1 << a.lanes) - 1));
+  for (int64_t row = t >> a.lanes; row < a.rows; row += threads >> a.lanes) {
     const bool out = left_out_row(a, row);
-    if constexpr (gt_is_split<I>) {
-      Vec16<_Float16> h, l;
+    for (int c = lane * 8; c < a.dp; c += 8 << a.lanes) {
+      T v[8];
+      load8(a, row, c, v);
+      if constexpr (gt_is_split<I>) {
+        Vec16<_Float16> h, l;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = !out && c + j < a.dim ? a.src[row * a.ld + c + j] * scale : 0.f;
-        h.v[j] = static_cast<_Float16>(v);
-        l.v[j] = static_cast<_Float16>(v - static_cast<float>(h.v[j]));
+        for (int j = 0; j < 8; ++j) {
+          const float x = out ? 0.f : v[j] * scale;
+          h.v[j] = static_cast<_Float16>(x);
+          l.v[j] = static_cast<_Float16>(x - static_cast<float>(h.v[j]));
+        }
+        // runs of 32 numbers: their h, then their l
+        _Float16* d = static_cast<_Float16*>(a.dst) + 2 * (row * a.dp + (c & ~31)) + (c & 31);
+        *reinterpret_cast<Vec16<_Float16>*>(d) = h;
+        *reinterpret_cast<Vec16<_Float16>*>(d + 32) = l;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 8; q += Vec16<T>::n) {
+          Vec16<T> o;
+#pragma unroll
+          for (int j = 0; j < Vec16<T>::n; ++j) o.v[j] = out ? T(0.f) : v[q + j];
+          if (c + q < a.dp)  // (an fp32 row may end inside the eight)
+            *reinterpret_cast<Vec16<T>*>(static_cast<T*>(a.dst) + row * a.dp + c + q) = o;
+        }
       }
-      // runs of 32 numbers: their h, then their l
-      _Float16* d = static_cast<_Float16*>(a.dst) + 2 * (row * a.dp + (c & ~31)) + (c & 31);
-      *reinterpret_cast<Vec16<_Float16>*>(d) = h;
-      *reinterpret_cast<Vec16<_Float16>*>(d + 32) = l;
-    } else {
-      Vec16<T> o;
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        o.v[j] = !out && c + j < a.dim ? a.src[row * a.ld + c + j] : T(0.f);
-      *reinterpret_cast<Vec16<T>*>(static_cast<T*>(a.dst) + row * a.dp + c) = o;
     }
   }
 }
@@ -173,7 +198,7 @@ struct LogitArgs {
   // gradient
   const float2* stat;  // [n] the row's (max, sum)
   const float* coef;   // [n] upstream gradient over its largest magnitude, 0: no loss
-  float pscale;
+  float pscale, unscale;  // of the dz image (powers of two)
   void* dz;            // [npad][vp]
   int64_t vp;
   float* dbpart;       // [row tile][vp] sums of dz over the tile's rows, or null
@@ -245,11 +270,18 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       for (int e = 0; e < 16; ++e) {
         const float b = sbias[i0 + Tile::row_of(mi, e)];
 #pragma unroll
-        for (int ni = 0; ni < Tile::NI; ++ni) {
-          const float z = __builtin_fmaf(acc[mi][ni][e], per, b);
-          // (a class that is left out has no logit, whatever its weights hold)
-          acc[mi][ni][e] = masked && b == -INFINITY ? -INFINITY : z;
-        }
+        for (int ni = 0; ni < Tile::NI; ++ni)
+          acc[mi][ni][e] = __builtin_fmaf(acc[mi][ni][e], per, b);
+      }
+  }
+  if (masked) {  // a class that is left out has no logit, whatever its weights hold
+#pragma unroll
+    for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const bool out = sbias[i0 + Tile::row_of(mi, e)] == -INFINITY;
+#pragma unroll
+        for (int ni = 0; ni < Tile::NI; ++ni) acc[mi][ni][e] = out ? -INFINITY : acc[mi][ni][e];
       }
   }
   // acc: the logits in units of ln 2, or (plain) the sums; one multiply-add takes either to its
@@ -295,7 +327,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       if (lane < 32) smerge[Tile::wave_m()][j] = make_float2(mm, st);
     } else {
       const float2 st = n < a.n ? a.stat[n] : make_float2(0.f, 0.f);
-      const float c = n < a.n ? a.coef[n] : 0.f;
+      const float c = n < a.n ? a.coef[n] * a.pscale : 0.f;  // (the image's scale in it)
       const float cs = c == 0.f || st.y == 0.f ? 0.f : c / st.y;
       // (a row without a loss has no gradient, whatever its logits are)
       const float ref = c == 0.f ? INFINITY : st.x > -INFINITY ? st.x : 0.f;
@@ -343,7 +375,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       for (int i = tid; i < BM; i += kGtThreads) {
         float v = 0.f;
         for (int k = 0; k < Tile::WAVES_N; ++k) v += sdb[k * BM + i];
-        a.dbpart[int64_t(nt) * a.vp + v0 + i] = v;
+        a.dbpart[int64_t(nt) * a.vp + v0 + i] = v * a.unscale;
       }
     }
     // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & SW), then
@@ -370,7 +402,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
             Four l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = acc[mi][ni][4 * g + e] * a.pscale;
+              const float v = acc[mi][ni][4 * g + e];
               f.v[e] = static_cast<H>(v);
               l.v[e] = static_cast<H>(v - static_cast<float>(f.v[e]));
             }
@@ -379,17 +411,23 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
             *at(j, byte + 64) = l;
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e] * a.pscale);
+            for (int e = 0; e < 4; ++e) f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e]);
             *at(j, i * int(sizeof(T))) = f;
           }
         }
     __syncthreads();
-    char* out = static_cast<char*>(a.dz);
-    for (int c = tid; c < BN * CPR; c += kGtThreads) {
-      const int j = c / CPR, k = c % CPR;
-      *reinterpret_cast<float4*>(out + ((int64_t(n0) + j) * a.vp + v0) * int(sizeof(T)) + k * 16) =
+    // (a thread's chunk k of rows j, j + RS, ...: one address that advances)
+    constexpr int RS = kGtThreads / CPR;
+    const int k = tid % CPR, j1 = tid / CPR;
+    const int64_t pitch = a.vp * int64_t(sizeof(T));
+    char* out = static_cast<char*>(a.dz) + (int64_t(n0) + j1) * pitch + v0 * int64_t(sizeof(T)) +
+                k * 16;
+#pragma unroll
+    for (int it = 0; it < BN / RS; ++it) {
+      const int j = j1 + it * RS;
+      *reinterpret_cast<float4*>(out) =
           *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & SW)) << 4));
+      out += RS * pitch;
     }
   }
 }
@@ -910,7 +948,11 @@ struct Ce {
 
   static PackArgs<S> pack(const void* src, int64_t ld, int64_t rows, const CeArgs& a, int64_t dp,
                           const int64_t* target, const float* bias, T* dst) {
-    return {static_cast<const S*>(src), ld, rows, a.dim, int(dp), target, a.ignore, bias, dst};
+    PackArgs<S> r = {static_cast<const S*>(src), ld, rows, a.dim, int(dp), target, a.ignore, bias,
+                     dst, 0, false};
+    while (r.lanes < 6 && (8 << r.lanes) < dp) ++r.lanes;
+    r.vec = ld % gt_chunk<S>() == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
+    return r;
   }
   static void prepare(const CoefArgs& coef, const PackArgs<S>& x, const PackArgs<S>& w,
                       const Work& k, hipStream_t s) {
@@ -919,8 +961,8 @@ struct Ce {
       oap_ce_largest<S><<<kMaxBlocks, 1024, 0, s>>>(x, w, k.largest);
       OAP_HIP_CHECK(hipGetLastError());
     }
-    const int64_t items = std::max(x.src ? x.rows * x.dp : 0, w.src ? w.rows * w.dp : 0);
-    const int64_t blocks = std::min<int64_t>(ceil_div(items, 1024 * 8), 2048);
+    const int64_t items = std::max(x.src ? x.rows << x.lanes : 0, w.src ? w.rows << w.lanes : 0);
+    const int64_t blocks = std::min<int64_t>(ceil_div(items, 1024), 2048);
     oap_ce_prepare<S, T><<<dim3(unsigned(std::max<int64_t>(1, blocks) + (coef.grad ? 1 : 0))),
                            1024, 0, s>>>(coef, x, w, k.largest, k.scale);
     OAP_HIP_CHECK(hipGetLastError());
@@ -1155,6 +1197,7 @@ struct Ce {
     l.stat = stat;
     l.coef = w.coef;
     l.pscale = pscale;
+    l.unscale = 1.f / pscale;
     l.dz = w.dz;
     l.vp = p.piece;
     l.dbpart = w.dbpart;

@@ -13,7 +13,6 @@
 
 #include <algorithm>
 #include <cfloat>
-#include <cstdlib>
 #include <cmath>
 #include <mutex>
 #include <set>
@@ -834,6 +833,7 @@ struct Plan {
   bool split;               // fp32 operands as two fp16 numbers
   int64_t dp;               // features of an image's row, to a whole chunk
   bool x_direct, w_direct;  // the operand is read where it lies
+  int64_t rows;             // rows per turn of the forward pass
   int bm, bn;               // class and row tile of the logits
   int64_t npad;
   int64_t piece;            // classes per piece, a multiple of 256
@@ -853,7 +853,11 @@ bool direct(const CeArgs& a, const void* p, int64_t ld) {
 // fp32.
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
-const double kSplitWork = getenv("CE_SPLIT") ? atof(getenv("CE_SPLIT")) : 1e9;
+// fp32 problems of at least this many products take the split operands: their images cost two
+// launches and a pass over the weights (1024 x 20000 x 128: 181 against 259 us with gradients,
+// 2048 x 20000 x 1000 1.09 against 2.45 ms; 300 x 5000 x 512 147 against 130 us, 200 x 20000 x 300
+// without gradients 52 against 47 us).
+constexpr double kSplitWork = 1.5e9;
 
 // Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps
 // another's MFMAs, but a byte from LDS feeds half as many.  fp32 MFMAs are slow enough for LDS at
@@ -881,7 +885,14 @@ Plan make_plan(const CeArgs& a, bool grad) {
   p.bm = tile_of(a, a.classes, a.n);
   p.bn = a.n <= 64 ? 64 : p.bm;
   if (p.bn == 64 && p.bm > 64) p.bm = 256;  // few rows of many classes
-  p.npad = int64_t(round_up(size_t(a.n), size_t(p.bn)));
+  // the forward pass keeps 8 bytes of each row and class tile: as many rows at a time as take
+  // 1 GiB, at least 4096
+  p.rows = a.n;
+  if (!grad) {
+    const int64_t fit = (int64_t(1) << 30) / 8 / ceil_div(a.classes, p.bm) / p.bn * p.bn;
+    p.rows = std::min<int64_t>(a.n, std::max<int64_t>(fit, 4096));
+  }
+  p.npad = int64_t(round_up(size_t(p.rows), size_t(p.bn)));
   const int64_t vpad = int64_t(round_up(size_t(a.classes), 256));
   int64_t per = p.dp;  // elements per class of the largest image
   if (grad) per = std::max(per, p.npad);
@@ -997,10 +1008,10 @@ struct Ce {
       w.zt = c.take<float>(a.n);
       return c.used;
     }
-    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(a.n) * p.dp);
+    w.ximg = p.x_direct ? nullptr : c.take<T>(size_t(p.rows) * p.dp);
     w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.part = c.take<float2>(size_t(ceil_div(a.classes, p.bm)) * p.npad);
-    w.zt = c.take<float>(a.n);
+    w.zt = c.take<float>(p.rows);
     w.largest = c.take<float>(2 * kMaxBlocks);
     w.scale = c.take<int>(2);
     return c.used;
@@ -1022,16 +1033,30 @@ struct Ce {
     return c.used;
   }
 
-  static void forward(const CeArgs& a, float* loss, float2* stat, float* total, bool mean,
+  static void forward(const CeArgs& all, float* loss, float2* stat, float* total, bool mean,
                       void* work, hipStream_t s) {
-    const Plan p = make_plan(a, false);
+    const Plan p = make_plan(all, false);
     Work w;
-    carve_forward(a, p, work, w);
-    if (few_rows(a)) {
-      const int blocks = few(a, w, s);
-      rows(a, w, blocks, a.n, loss, stat, total, mean, s);
+    carve_forward(all, p, work, w);
+    if (few_rows(all)) {
+      const int blocks = few(all, w, s);
+      rows(all, w, blocks, all.n, loss, stat, total, mean, s);
       return;
     }
+    for (int64_t r0 = 0; r0 < all.n; r0 += p.rows) {
+      CeArgs a = all;
+      a.n = std::min(p.rows, all.n - r0);
+      a.x = static_cast<const S*>(all.x) + r0 * all.ldx;
+      a.target = all.target + r0;
+      forward_rows(a, p, w, s);
+      rows(a, w, int(ceil_div(a.classes, p.bm)), p.npad, loss + r0, stat + r0,
+           p.rows == all.n ? total : nullptr, mean, s);
+    }
+    if (total && p.rows < all.n) sum_losses(all, loss, total, mean, s);
+  }
+
+  // (max, sum) of all class tiles for the rows of a
+  static void forward_rows(const CeArgs& a, const Plan& p, const Work& w, hipStream_t s) {
     const S* wt = static_cast<const S*>(a.w);
     LogitArgs l = {};
     PackArgs<S> px = {}, pw = {};
@@ -1044,7 +1069,7 @@ struct Ce {
     l.scale = w.scale;
     l.target = a.target;
     l.n = a.n;
-    l.ntiles = int(p.npad / p.bn);
+    l.ntiles = int(ceil_div(a.n, p.bn));
     l.npad = p.npad;
     l.zt = w.zt;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
@@ -1062,7 +1087,6 @@ struct Ce {
       l.part = w.part + c0 / p.bm * p.npad;
       logits<false>(p, l, s);
     }
-    rows(a, w, int(ceil_div(a.classes, p.bm)), p.npad, loss, stat, total, mean, s);
   }
 
   // One workgroup for little work (the total needs no launch of its own then), else at least one
@@ -1076,10 +1100,19 @@ struct Ce {
     if (a.n >= 8) r.cols = std::max(r.cols, 8);
     oap_ce_rows<<<dim3(one ? 1 : unsigned(ceil_div(a.n, r.cols))), 1024, 0, s>>>(r);
     OAP_HIP_CHECK(hipGetLastError());
-    if (total && !one && ceil_div(a.n, r.cols) > 1) {
-      oap_ce_total<<<1, 1024, 0, s>>>(r);
-      OAP_HIP_CHECK(hipGetLastError());
-    }
+    if (total && !one && ceil_div(a.n, r.cols) > 1) sum_losses(a, loss, total, mean, s);
+  }
+  static void sum_losses(const CeArgs& a, const float* loss, float* total, bool mean,
+                         hipStream_t s) {
+    RowArgs r = {};
+    r.n = a.n;
+    r.target = a.target;
+    r.ignore = a.ignore;
+    r.loss = const_cast<float*>(loss);
+    r.total = total;
+    r.mean = mean;
+    oap_ce_total<<<1, 1024, 0, s>>>(r);
+    OAP_HIP_CHECK(hipGetLastError());
   }
 
   template <int N, int G>

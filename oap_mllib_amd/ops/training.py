@@ -259,11 +259,14 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, weights, indices)
         ctx.args = (k, sigmoid, renormalize, scale)
         ctx.mark_non_differentiable(indices, counts)
+        ctx.set_materialize_grads(False)  # (no zeros for the integers' gradients)
         return weights, indices, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _indices, _counts):
+        if grad is None:
+            return (None,) * 8
         logits, weights, indices = ctx.saved_tensors
         k, sigmoid, renormalize, scale = ctx.args
         z, ld = _rows(logits)

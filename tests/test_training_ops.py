@@ -282,6 +282,66 @@ def test_ce_pieces_gpu():
             assert (err <= tol).all(), (dtype, (err / tol).max())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1.0, 1e-18, 1e18])
+def test_ce_large_fp32_gpu(scale):
+    """fp32 problems large enough for the split operands: sizes off every tile, rows and classes
+    that are left out, magnitudes far from one (x and weight scaled against each other).  What the
+    split leaves out, 2^-40 of an operand's largest entry and 2^-39 of the largest coefficient, is
+    below 2^-23 of the sums of magnitudes here: every row of x and weight holds an entry within
+    2^-3 of the largest, and the smallest dz is above 2^-15 of the largest."""
+    n, v, d = 333, 15_013, 301
+    x, w = rand((n, d), 1, device="cuda"), rand((v, d), 2, device="cuda", scale=0.5 / math.sqrt(d))
+    x, w = x * scale, w / scale
+    b = rand((v,), 3, device="cuda", scale=0.3)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(4)).cuda()
+    ce_check(x, w, t, None)
+    t[7:200:5] = -100
+    x[7], x[12, 3] = math.nan, INF
+    b[100:9000:7] = -INF
+    w[100], w[107, 5] = math.nan, -INF
+    ce_check(x, w, t, b)
+    ce_check(x, w, t, b, "none", torch.rand(n, generator=torch.Generator().manual_seed(5)).cuda()
+             + 0.5)
+    z = torch.zeros_like(x)
+    loss = ops.softmax_cross_entropy(z, torch.zeros_like(w), t)
+    check(loss, torch.tensor(math.log(v)).double(), 8 * E32 * math.log(v), "zeros")
+
+
+@pytest.mark.gpu
+def test_ce_rows_in_turns_gpu():
+    """More rows than one turn of the forward pass keeps statistics for: every row's loss is that
+    of a call on its own part of the rows, but for the order in which 15625 tiles' sums are joined
+    (up to 31 additions and powers in a row of threads, 10 levels above them)."""
+    n, v, d = 9000, 2_000_000, 4
+    x, w = rand((n, d), 1, torch.bfloat16, "cuda"), rand((v, d), 2, torch.bfloat16, "cuda")
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    t[::7] = -100
+    whole = ops.softmax_cross_entropy(x, w, t, reduction="none")
+    parts = [ops.softmax_cross_entropy(x[a:a + 3000], w, t[a:a + 3000], reduction="none")
+             for a in range(0, n, 3000)]
+    parts = torch.cat(parts)
+    assert ((whole - parts).abs() <= 2 * 41 * 3 * E32 + 4 * E32 * parts.abs()).all()
+    mean = ops.softmax_cross_entropy(x, w, t)
+    ref = whole.double().sum() / (t != -100).sum()
+    assert abs(mean.item() - ref.item()) <= E32 * abs(ref.item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(1, 5000, 100), (3, 1000, 1024), (4, 999, 40), (4, 33, 2048),
+                                   (2, 70, 4096), (1, 1, 8), (5, 3000, 128)])
+def test_ce_few_rows_gpu(dtype, n, v, d):
+    """One row and a few: losses alone and with gradients, odd counts, every lane layout."""
+    x, w = rand((n, d), 1, dtype, "cuda"), rand((v, d), 2, dtype, "cuda", 2 / math.sqrt(d))
+    t = torch.arange(n, device="cuda") * 13 % v
+    b = rand((v,), 3, device="cuda")
+    b[v // 2 + 1::3] = -INF
+    for bias in (None, b):
+        ce_check(x, w, t, bias, "none", want=(False, False, False))
+        ce_check(x, w, t, bias)
+
+
 # ----------------------------------------------------------------------------------- dropout
 def philox_words(count, offset, seed):
     """Words of elements offset .. offset + count - 1, in plain integers."""

@@ -272,7 +272,10 @@ struct GtSide {
 
 // Element (row i, column j) of acc[mi][ni][e] in lane l of wave (wm, wn):
 //   i = wm * WM + 32 mi + 8 (e >> 2) + 4 (l >> 5) + (e & 3),   j = wn * WN + 32 ni + (l & 31)
-template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M_>
+//
+// SINGLE: one LDS buffer and two barriers a block.  Half the LDS lets a third workgroup share the
+// CU, which hides more than the second buffer does while k is short.
+template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M_, bool SINGLE = false>
 struct GtTile {
   static constexpr int BM = BM_, BN = BN_;
   static constexpr int WAVES_M = WAVES_M_, WAVES_N = 4 / WAVES_M;
@@ -282,7 +285,7 @@ struct GtTile {
   typedef GtSide<T, BN, OB> SideB;
   static constexpr int BK = SideA::BK;
   static constexpr int kBuf = SideA::kBytes + SideB::kBytes;
-  static constexpr int kLds = 2 * kBuf;
+  static constexpr int kLds = (SINGLE ? 1 : 2) * kBuf;
   // the last block apart, with only its occupied steps (the largest tiles' registers do not have
   // room for a second copy of the loop's body, and their k is long)
   static constexpr bool kTail = gt_occupancy(BM, BN) > 1 && !gt_is_split<T>;
@@ -340,6 +343,26 @@ struct GtTile {
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = gt_mfma(a[f][i], b[f][j], acc[i][j]);
     };
+    if constexpr (SINGLE) {
+      ga.load(va);
+      gb.load(vb);
+      for (int it = 0; it < nk; ++it) {
+        ga.store(lds, va);
+        gb.store(lds + SideA::kBytes, vb);
+        __syncthreads();
+        ga.load(va);
+        gb.load(vb);
+        fetch(lds, 0, 0);
+#pragma unroll
+        for (int ks = 0; ks < gt_steps<T>; ++ks) {
+          if (ks + 1 < gt_steps<T>) fetch(lds, ks + 1, (ks + 1) & 1);
+          multiply(ks & 1);
+          interleave<false, false>();
+        }
+        __syncthreads();
+      }
+      return;
+    }
     ga.load(va);
     gb.load(vb);
     ga.store(lds, va);

@@ -232,10 +232,9 @@ struct Store<GtSplit> {
 
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
 // over the tile's classes is mostly within the lane.
-template <typename T, int BM, int BN, int WAVES_M, bool GRAD>
+template <typename T, int BM, int BN, int WAVES_M, bool SINGLE, bool GRAD>
 __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logits(LogitArgs a) {
-  typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M> Tile;
-  static_assert(BN * BM * int(sizeof(T)) <= Tile::kLds, "the dz tile fits the staging buffers");
+  typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M, SINGLE> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float sbias[BM];
   __shared__ float2 smerge[WAVES_M][BN];
@@ -378,9 +377,13 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       }
     }
     // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & SW), then
-    // out in whole rows
+    // out in whole rows; in parts of 32 rows of every wave where the tile is larger than LDS
     constexpr int CPR = BM * int(sizeof(T)) / 16, ROW = BM * int(sizeof(T));
     constexpr int SW = CPR < 16 ? CPR - 1 : 15;
+    constexpr bool kWhole = BN * ROW <= Tile::kLds;
+    constexpr int PARTS = kWhole ? 1 : Tile::NI, NP = Tile::NI / PARTS;  // blocks of a part
+    constexpr int PW = Tile::WN / PARTS, PR = BN / PARTS;                // rows of it
+    static_assert(PR * ROW <= Tile::kLds, "a part of the dz tile fits the staging buffer");
     typedef typename Store<T>::type H;  // what is stored: T, or the two halves of a split number
     struct alignas(4 * sizeof(H)) Four {
       H v[4];
@@ -388,45 +391,49 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
     auto at = [&](int j, int byte) {
       return reinterpret_cast<Four*>(lds + j * ROW + (((byte >> 4) ^ (j & SW)) << 4) + (byte & 15));
     };
-    __syncthreads();
-#pragma unroll
-    for (int ni = 0; ni < Tile::NI; ++ni)
-#pragma unroll
-      for (int mi = 0; mi < Tile::MI; ++mi)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int j = j0 + 32 * ni, i = i0 + Tile::row_of(mi, 4 * g);
-          Four f;
-          if constexpr (gt_is_split<T>) {
-            Four l;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = acc[mi][ni][4 * g + e];
-              f.v[e] = static_cast<H>(v);
-              l.v[e] = static_cast<H>(v - static_cast<float>(f.v[e]));
-            }
-            const int byte = (i >> 5) * 128 + (i & 31) * 2;
-            *at(j, byte) = f;
-            *at(j, byte + 64) = l;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e]);
-            *at(j, i * int(sizeof(T))) = f;
-          }
-        }
-    __syncthreads();
-    // (a thread's chunk k of rows j, j + RS, ...: one address that advances)
+    // (a thread's chunk k of rows j1, j1 + RS, ... of a part)
     constexpr int RS = kGtThreads / CPR;
     const int k = tid % CPR, j1 = tid / CPR;
     const int64_t pitch = a.vp * int64_t(sizeof(T));
-    char* out = static_cast<char*>(a.dz) + (int64_t(n0) + j1) * pitch + v0 * int64_t(sizeof(T)) +
-                k * 16;
+    char* out = static_cast<char*>(a.dz) + int64_t(n0) * pitch + v0 * int64_t(sizeof(T)) + k * 16;
 #pragma unroll
-    for (int it = 0; it < BN / RS; ++it) {
-      const int j = j1 + it * RS;
-      *reinterpret_cast<float4*>(out) =
-          *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & SW)) << 4));
-      out += RS * pitch;
+    for (int part = 0; part < PARTS; ++part) {
+      __syncthreads();
+#pragma unroll
+      for (int np = 0; np < NP; ++np)
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int ni = part * NP + np;
+            const int j = Tile::wave_n() * PW + 32 * np + (lane & 31);
+            const int i = i0 + Tile::row_of(mi, 4 * g);
+            Four f;
+            if constexpr (gt_is_split<T>) {
+              Four l;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = acc[mi][ni][4 * g + e];
+                f.v[e] = static_cast<H>(v);
+                l.v[e] = static_cast<H>(v - static_cast<float>(f.v[e]));
+              }
+              const int byte = (i >> 5) * 128 + (i & 31) * 2;
+              *at(j, byte) = f;
+              *at(j, byte + 64) = l;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e]);
+              *at(j, i * int(sizeof(T))) = f;
+            }
+          }
+      __syncthreads();
+#pragma unroll
+      for (int it = 0; it < PR / RS; ++it) {
+        const int j = j1 + it * RS;
+        const int row = j / PW * Tile::WN + part * PW + j % PW;  // of the tile
+        *reinterpret_cast<float4*>(out + row * pitch) =
+            *reinterpret_cast<const float4*>(lds + j * ROW + ((k ^ (j & SW)) << 4));
+      }
     }
   }
 }
@@ -837,6 +844,7 @@ struct Plan {
   int bm, bn;               // class and row tile of the logits
   int64_t npad;
   int64_t piece;            // classes per piece, a multiple of 256
+  bool single;              // logits of 128 x 128 with one staging buffer
   int xtile, wtile;         // square tiles of dx and dW
   int splits;
 };
@@ -884,6 +892,11 @@ Plan make_plan(const CeArgs& a, bool grad) {
   p.w_direct = !p.split && direct(a, a.w, a.ldw) && !(grad && a.bias);
   p.bm = tile_of(a, a.classes, a.n);
   p.bn = a.n <= 64 ? 64 : p.bm;
+  // One buffer lets a third workgroup share the CU.  16 bits gain at every k that takes this tile
+  // (4096 x 200000 x 128 1.82 against 1.99 ms, 4096 x 65536 x 512 1.38 against 1.42 ms), split
+  // operands while k is short (1024 x 2M x 100 10.6 against 11.7 ms; 2048 x 20000 x 1000 1.10
+  // against 1.09 ms).  fp32 keeps two: that loop skips the empty steps of a short k.
+  p.single = es == 2 || (p.split && p.dp <= 512);
   if (p.bn == 64 && p.bm > 64) p.bm = 256;  // few rows of many classes
   // the forward pass keeps 8 bytes of each row and class tile: as many rows at a time as take
   // 1 GiB, at least 4096
@@ -979,10 +992,10 @@ struct Ce {
     OAP_HIP_CHECK(hipGetLastError());
   }
 
-  template <int BM, int BN, int WAVES_M, bool GRAD>
+  template <int BM, int BN, int WAVES_M, bool SINGLE, bool GRAD>
   static void logits_tile(const LogitArgs& l, hipStream_t s) {
-    auto k = oap_ce_logits<T, BM, BN, WAVES_M, GRAD>;
-    constexpr int lds = GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M>::kLds;
+    auto k = oap_ce_logits<T, BM, BN, WAVES_M, SINGLE, GRAD>;
+    constexpr int lds = GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M, SINGLE>::kLds;
     set_lds(k, lds);
     k<<<dim3(unsigned(l.vtiles * l.ntiles)), kGtThreads, lds, s>>>(l);
     OAP_HIP_CHECK(hipGetLastError());
@@ -991,13 +1004,15 @@ struct Ce {
   template <bool GRAD>
   static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
     if (p.bm == 64)
-      logits_tile<64, 64, 2, GRAD>(l, s);
+      logits_tile<64, 64, 2, false, GRAD>(l, s);
     else if (p.bn == 64)
-      logits_tile<256, 64, 4, GRAD>(l, s);
+      logits_tile<256, 64, 4, false, GRAD>(l, s);
+    else if (p.bn == 128 && p.single)
+      logits_tile<128, 128, 2, sizeof(T) == 2 || gt_is_split<T>, GRAD>(l, s);
     else if (p.bn == 128)
-      logits_tile<128, 128, 2, GRAD>(l, s);
+      logits_tile<128, 128, 2, sizeof(T) == 2, GRAD>(l, s);
     else if constexpr (sizeof(T) == 2)
-      logits_tile<256, 256, 2, GRAD>(l, s);
+      logits_tile<256, 256, 2, false, GRAD>(l, s);
   }
 
   static size_t carve_forward(const CeArgs& a, const Plan& p, void* base, Work& w) {

@@ -21,6 +21,7 @@ __all__ = ["dropout", "route", "softmax_cross_entropy"]
 
 _ELEM = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}
 _M64 = (1 << 64) - 1
+_F32 = torch.finfo(torch.float32)
 
 
 def _float_tensor(name: str, t, dim: int | None = None):
@@ -296,11 +297,13 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
 
     An expert whose logit is ``-inf`` or NaN, or whose bias is ``-inf`` or NaN, is left out; where
     fewer than ``k`` are left the last slots hold index -1 and weight 0.  At most 1024 experts,
-    32 choices and 64 groups.  The gradient goes from ``weights`` to ``logits``.
+    32 choices, 64 groups and 2^31 - 1 tokens.  The gradient goes from ``weights`` to ``logits``.
     """
     _float_tensor("logits", logits, 2)
     native = _loader.load()
-    e = logits.shape[1]
+    t, e = logits.shape
+    if t >= 1 << 31:
+        raise ValueError(f"logits: expected less than 2^31 tokens, got {t}")
     if not 1 <= e <= native.route_max_experts:
         raise ValueError(f"logits: expected 1 to {native.route_max_experts} experts, got {e}")
     k, groups = int(k), int(groups)
@@ -316,8 +319,8 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"score: expected 'softmax' or 'sigmoid', got {score!r}")
     scale = float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale: expected a positive number, got {scale}")
+    if not _F32.tiny <= scale <= _F32.max:
+        raise ValueError(f"scale: expected a positive float32 number, got {scale}")
     if bias is not None:
         _same("bias", bias, logits, (e,), torch.float32)
         bias = bias.detach().contiguous()

@@ -696,3 +696,97 @@ def test_other_stream_gives_the_same():
     s.synchronize()
     for a, b in zip(want, got):
         assert torch.equal(a, b)  # (fixed order of every sum)
+
+
+@pytest.mark.gpu
+def test_threads_at_once():
+    """Calls from several threads, each on a stream of its own."""
+    from concurrent.futures import ThreadPoolExecutor
+    x, leaves, t = step_inputs("cuda", torch.bfloat16, n=300, v=3000)
+
+    def run(seed):
+        loss, counts = step(x, *leaves, t, seed)
+        return [loss.detach(), counts, *torch.autograd.grad(loss, leaves)]
+
+    want = [run(s) for s in range(4)]
+    torch.cuda.synchronize()
+
+    def worker(seed):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [run(seed) for _ in range(5)]
+        stream.synchronize()
+        return all(torch.equal(a, b) for g in got for a, b in zip(g, want[seed]))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(worker, range(4)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 70])
+def test_ce_offsets_beyond_32_bits(n):
+    """Weights of more than 2^31 elements and 2^32 bytes.  All classes but the last 300 have zero
+    weights, so each adds exp(0) to a row's sum."""
+    v, d, tail = 1_200_000, 2000, 300
+    w = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    w[-tail:] = rand((tail, d), 1, torch.bfloat16, "cuda")
+    x = rand((n, d), 2, torch.bfloat16, "cuda", 0.2)
+    t = torch.randint(v - tail, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    loss = ops.softmax_cross_entropy(*leaves, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, leaves)
+    x64, w64, k = cpu64(x), cpu64(w[-tail:]), t.cpu() - (v - tail)
+    z = x64 @ w64.t()
+    lse = torch.logsumexp(torch.cat([z, torch.full((n, 1), math.log(v - tail))], 1), 1)
+    hot = torch.zeros_like(z)
+    hot[torch.arange(n), k] = 1
+    zerr = 2 * (d + 10) * E32 * (x64.abs() @ w64.abs().t()).max().item()
+    u = half_step(torch.bfloat16)
+    check(loss, (lse - z.gather(1, k[:, None])[:, 0]).sum(),
+          n * (zerr + 4 * E32 * (lse.abs().max() + 1)) * 2, "loss")
+    p, p0 = (z - lse[:, None]).exp(), (-lse).exp()
+    # (the classes of zero weights add nothing to a sum of dx, exactly)
+    rel = 2 * zerr + 16 * E32 + u + (max(tail, n) + 8) * E32
+    check(dx, (p - hot) @ w64, ((p + hot) @ w64.abs()) * (rel + u) + 1e-37, "dx")
+    check(dw[-tail:], (p - hot).t() @ x64, ((p + hot).t() @ x64.abs()) * (rel + u) + 1e-37,
+          "dw of the last")
+    head = dw[[0, v // 2, v - tail - 1]]
+    check(head, (p0 @ x64).expand(3, d), (p0 @ x64.abs()).expand(3, d) * (rel + u) + 1e-37,
+          "dw of the others")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 3])
+def test_dropout_offsets_beyond_32_bits(offset):
+    n = (1 << 31) + 1001
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = ops.dropout(x, 0.3, 9, offset=offset)
+    for i in (0, 1 << 30, n - 1001):
+        part = ops.dropout(x[:1001], 0.3, 9, offset=offset + i)
+        assert torch.equal(y[i:i + 1001], part)
+
+
+@pytest.mark.gpu
+def test_route_offsets_beyond_32_bits():
+    e, k, turns = 128, 4, 17000
+    base = rand((1000, e), 4, torch.bfloat16, "cuda").requires_grad_()
+    up = rand((1000, k), 5, torch.float32, "cuda")
+    w, i, c = ops.route(base, k)
+    g, = torch.autograd.grad(w, base, up)
+    big = base.detach().repeat(turns, 1).requires_grad_()
+    bw, bi, bc = ops.route(big, k)
+    assert torch.equal(bw.view(turns, 1000, k), w.expand(turns, 1000, k))
+    assert torch.equal(bi.view(turns, 1000, k), i.expand(turns, 1000, k))
+    assert torch.equal(bc, c * turns)
+    bg, = torch.autograd.grad(bw, big, up.repeat(turns, 1))
+    for t in (0, turns // 2, turns - 1):
+        assert torch.equal(bg.view(turns, 1000, e)[t], g)
+
+
+def test_route_limits():
+    z = torch.zeros(1, 4)
+    for scale in (1e39, 1e-39, 1e-60):  # not a normal fp32 number
+        with pytest.raises(ValueError, match="scale"):
+            ops.route(z, 2, scale=scale)
+    with pytest.raises(ValueError, match="tokens"):  # (the loads are 32-bit numbers)
+        ops.route(z.expand(1 << 31, 4), 2)

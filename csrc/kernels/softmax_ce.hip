@@ -9,6 +9,17 @@
 // piece's classes are then copied into split images at a power-of-two scale each, and dz, at most
 // 1 in magnitude, is stored split at the scale 2^14.  A product keeps 22 bits; |dz| below 2^-24
 // keeps an absolute 2^-39.
+//
+// Roundings: sums, statistics, losses and dx's slabs are fp32, and a result is rounded once.  With
+// 16-bit operands dz is rounded to their type (at most 2^-8 of it in bf16, 2^-11 in fp16) before
+// it meets W and x, whose own rounding is as large: that is what the matrix units take, and dz in
+// two parts would double the work of dX and dW.  db sums dz in fp32 before that rounding.
+//
+// What bounds it, at 8192 x 131072 x 2048 bf16 (16.6 ms for forward and gradients, 8 N V D
+// operations): the matrix units under the chip's power limit, 1.06 to 1.13 PF/s in each product
+// (a library product of the same shapes 1.23).  At 1024 x 2M x 100 fp32 (10.4 ms): k is short, so
+// each tile's epilogue and staging weigh as much as its MFMAs (21% busy), and dz, written once and
+// read twice, is 26 GB.
 #include "kernels/softmax_ce.h"
 
 #include <algorithm>
@@ -231,7 +242,8 @@ struct Store<GtSplit> {
 };
 
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
-// over the tile's classes is mostly within the lane.
+// over the tile's classes is mostly within the lane.  8192 x 131072 x 2048 bf16: 3.9 ms forward
+// (1.13 PF/s), 2.23 ms for each half of the classes with their dz (0.98 PF/s, 1 GiB written).
 template <typename T, int BM, int BN, int WAVES_M, bool SINGLE, bool GRAD>
 __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logits(LogitArgs a) {
   typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M, SINGLE> Tile;
@@ -442,6 +454,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 // bounds it, so they go straight into registers.  G lanes share a class, four 16-byte chunks
 // each; the rows of x stay in registers; every group keeps its own (max, sum) and the workgroup
 // joins them.  The chip streams classes with enough loads in flight: two classes per lane group.
+// One row, 2M x 100 fp32: 142 us, 5.9 TB/s.
 struct FewArgs {
   const void *w, *x;
   int64_t ldw, ldx, classes;
@@ -727,7 +740,8 @@ struct ProdArgs {
 };
 
 // dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
-// part to the same elements, so the order of the sums is fixed.
+// part to the same elements, so the order of the sums is fixed.  65536 classes of 8192 x 2048
+// bf16: 2.03 ms (1.08 PF/s); dW of them 2.07 ms (1.06 PF/s).
 template <typename T, int BM, int BN, int WAVES_M>
 __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dx(ProdArgs a) {
   typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M> Tile;
@@ -856,9 +870,9 @@ bool direct(const CeArgs& a, const void* p, int64_t ld) {
 }
 
 // Of one dz image or one class image.  Smaller pieces stay in the last-level cache, but their
-// products fill the chip less evenly and dx's slabs are added to more often: 2^28, 2^29, 2^30
-// took 17.7, 16.9, 16.6 ms at 8192 x 131072 x 2048 bf16 and 18.6, 18.0, 17.6 ms at 1024 x 2M x 100
-// fp32.
+// products fill the chip less evenly and dx's slabs are added to more often: 2^28, 2^29, 2^30, 2^31
+// took 18.2, 17.3, 16.9, 17.0 ms at 8192 x 131072 x 2048 bf16 and 11.5, 11.6, 10.7, 10.9 ms at
+// 1024 x 2M x 100 fp32.
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
 // fp32 problems of at least this many products take the split operands: their images cost two
@@ -869,9 +883,9 @@ constexpr double kSplitWork = 1.5e9;
 
 // Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps
 // another's MFMAs, but a byte from LDS feeds half as many.  fp32 MFMAs are slow enough for LDS at
-// any size (1024 x 2M x 100: 19.9 against 24.4 ms); in 16 bits the small ones are faster while
-// the epilogue weighs (forward and gradients, bf16: 3000 x 20000 x 784 0.66 against 0.68 ms,
-// 4096 x 65536 x 512 1.44 against 1.52 ms; 8192 x 131072 x 2048 18.9 against 16.6 ms).
+// any size (1024 x 2M x 100 in fp32 MFMAs: 19.9 against 24.4 ms); in 16 bits the small ones are
+// faster while the epilogue weighs (forward and gradients, bf16: 3000 x 20000 x 784 0.66 against
+// 0.68 ms, 4096 x 65536 x 512 1.44 against 1.52 ms; 8192 x 131072 x 2048 18.9 against 16.6 ms).
 // Where tiles of 128 leave CUs empty, tiles of 64 finish sooner.
 int tile_of(const CeArgs& a, int64_t rows, int64_t cols) {
   if (ceil_div(rows, 128) * ceil_div(cols, 128) < 192) return 64;

@@ -7,6 +7,10 @@ comes from torch's allocator for the length of the call.  A CPU tensor goes thro
 host engine (fp32 in, sums in fp64).  Float32, bfloat16 and float16 are taken; sums, softmax
 statistics and choices are held in 32 bits or more, and a result is rounded once.
 
+Before a backward pass is captured, what keeps an eager graph of the same leaves alive (its loss)
+has to go: torch ties a leaf's gradient to the stream of the first graph that uses the leaf, and
+a capture that waits for another stream fails.
+
 The ops are local to the process: with row shards every rank calls them on its own rows and
 reduces what it needs, as with any torch op.
 """

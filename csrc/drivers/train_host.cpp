@@ -1,5 +1,7 @@
 #include "drivers/train_host.h"
 
+#include <unistd.h>
+
 #include <algorithm>
 #include <cmath>
 #include <functional>
@@ -19,8 +21,14 @@ namespace {
 
 constexpr double kInf = std::numeric_limits<double>::infinity();
 
-// One pool for the process; a pool runs one loop at a time.
+// One pool for the process; a pool runs one loop at a time.  The child of a fork has none of the
+// pool's threads and runs alone.
 void parallel(int64_t n, const std::function<void(int64_t, int64_t)>& f) {
+  static const pid_t owner = getpid();
+  if (getpid() != owner) {
+    if (n > 0) f(0, n);
+    return;
+  }
   static std::mutex mu;
   static ThreadPool pool(
       int(std::min<unsigned>(std::max(1u, std::thread::hardware_concurrency()), 16)));
@@ -190,7 +198,8 @@ void ce_forward_host(const kern::CeArgs& a, float* loss, float2* stat, float* to
         z[j] = ce_logit(a, i, j);
         m = std::max(m, z[j]);
       }
-      const double ref = m > -kInf ? m : 0.0;
+      // (the sum refers to the maximum as it is kept)
+      const double ref = m > -kInf ? double(float(m)) : 0.0;
       for (int64_t j = 0; j < a.classes; ++j) s += std::exp(z[j] - ref);
       stat[i] = make_float2(float(m), float(s));
       if (a.target[i] == a.ignore)
@@ -198,7 +207,7 @@ void ce_forward_host(const kern::CeArgs& a, float* loss, float2* stat, float* to
       else if (!has_loss(a, i))
         loss[i] = std::numeric_limits<float>::quiet_NaN();
       else
-        loss[i] = float(z[a.target[i]] == -kInf ? kInf : std::log(s) + (m - z[a.target[i]]));
+        loss[i] = float(z[a.target[i]] == -kInf ? kInf : std::log(s) + (ref - z[a.target[i]]));
     }
   });
   if (!total) return;

@@ -790,3 +790,40 @@ def test_route_limits():
             ops.route(z, 2, scale=scale)
     with pytest.raises(ValueError, match="tokens"):  # (the loads are 32-bit numbers)
         ops.route(z.expand(1 << 31, 4), 2)
+
+
+def test_host_large_logits():
+    """Sums and probabilities refer to the stored maximum: logits of 1e5 keep their differences."""
+    x = torch.tensor([[100000.125]], requires_grad=True)
+    w = torch.tensor([[1.0], [1.00001], [0.99999]], requires_grad=True)
+    t = torch.tensor([0])
+    loss = ops.softmax_cross_entropy(x, w, t)
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    z = cpu64(x) @ cpu64(w).t()
+    p = torch.softmax(z, 1)
+    p[0, 0] -= 1
+    # sums in 64 bits; the sum of exponentials (2^-24) and the results are rounded to fp32
+    check(loss, (z.logsumexp(1) - z[:, 0])[0], 1e-6, "loss")
+    check(dw, p.t() @ cpu64(x), 4 * 2.0 ** -24 * 1e5, "dw")
+    check(dx, p @ cpu64(w), 4 * 2.0 ** -24 * 2, "dx")
+
+
+def test_host_engine_in_a_forked_child():
+    """The child of a fork has none of the host engine's threads."""
+    import multiprocessing
+    x = torch.ones(4096)
+    want = ops.dropout(x, 0.5, 7)
+    fork = multiprocessing.get_context("fork")
+
+    def child(out):
+        out.put(bool((ops.dropout(x, 0.5, 7).numpy() == want.numpy()).all()))
+
+    out = fork.Queue()
+    p = fork.Process(target=child, args=(out,))
+    p.start()
+    p.join(30)
+    alive = p.is_alive()
+    if alive:
+        p.kill()
+        p.join()
+    assert not alive and out.get(timeout=5)

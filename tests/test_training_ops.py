@@ -827,3 +827,16 @@ def test_host_engine_in_a_forked_child():
         p.kill()
         p.join()
     assert not alive and out.get(timeout=5)
+
+
+def test_second_derivatives_are_refused():
+    """A graph of the gradient gives the same gradient, and an error when it is differentiated."""
+    x = rand((5, 8), 1).requires_grad_()
+    up = rand((5, 2), 2)
+    for f in (lambda: (ops.dropout(x, 0.3, 4) ** 2).sum(),
+              lambda: (ops.route(x, 2)[0] * up).sum()):
+        plain, = torch.autograd.grad(f(), x)
+        g, = torch.autograd.grad(f(), x, create_graph=True)
+        assert torch.equal(plain, g.detach())
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)

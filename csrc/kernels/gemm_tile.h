@@ -97,7 +97,7 @@ constexpr int gt_mfmas = gt_is_split<T> ? 3 : sizeof(T) == 4 ? 4 : 1;
 
 constexpr int kGtThreads = 256;  // 4 waves
 // waves per SIMD that a tile's registers allow
-constexpr int gt_occupancy(int bm, int bn) { return bm * bn <= 128 * 128 ? 2 : 1; }
+constexpr int gt_occupancy(int bm, int bn) { return bm * bn <= 256 * 128 ? 2 : 1; }
 
 // elements of k per block, and per 16-byte chunk
 template <typename T>

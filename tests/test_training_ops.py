@@ -309,6 +309,24 @@ def test_ce_large_fp32_gpu(scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_ce_many_tiles_gpu(dtype, bias):
+    """Enough rows and classes for the wider tiles of 16-bit logits."""
+    n, v, d = 1100, 30001, 40
+    x, w = rand((n, d), 1, dtype, "cuda", 0.5), rand((v, d), 2, dtype, "cuda", 0.5)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    t[::7] = -100
+    b = None
+    if bias:
+        b = rand((v,), 4)
+        b[5::11] = -INF
+        b[t[t >= 0]] = 0.25
+        b = b.cuda()
+    ce_check(x, w, t.cuda(), b)
+
+
+@pytest.mark.gpu
 def test_ce_rows_in_turns_gpu():
     """More rows than one turn of the forward pass keeps statistics for: every row's loss is that
     of a call on its own part of the rows, but for the order in which 15625 tiles' sums are joined

@@ -187,6 +187,11 @@ bool has_loss(const kern::CeArgs& a, int64_t i) {
   return a.target[i] != a.ignore && a.target[i] >= 0 && a.target[i] < a.classes;
 }
 
+// (rows without a loss, or whose loss nobody asks the gradient of, take no part)
+bool has_gradient(const kern::CeArgs& a, const float* grad, bool per_row, int64_t i) {
+  return has_loss(a, i) && !(per_row && grad[i] == 0.f);
+}
+
 }  // namespace
 
 void ce_forward_host(const kern::CeArgs& a, float* loss, float2* stat, float* total, bool mean) {
@@ -240,7 +245,7 @@ void ce_backward_host(const kern::CeArgs& a, const float2* stat, const float* gr
       std::vector<double> acc(a.dim);
       for (int64_t i = b; i < end; ++i) {
         std::fill(acc.begin(), acc.end(), 0.0);
-        for (int64_t j = 0; has_loss(a, i) && j < a.classes; ++j) {
+        for (int64_t j = 0; has_gradient(a, grad, per_row, i) && j < a.classes; ++j) {
           const double d = dz(i, j);
           if (d != 0.0)
             for (int c = 0; c < a.dim; ++c) acc[c] += d * w[j * a.ldw + c];
@@ -255,7 +260,7 @@ void ce_backward_host(const kern::CeArgs& a, const float2* stat, const float* gr
         std::fill(acc.begin(), acc.end(), 0.0);
         double bias = 0.0;
         for (int64_t i = 0; i < a.n; ++i) {
-          if (!has_loss(a, i)) continue;
+          if (!has_gradient(a, grad, per_row, i)) continue;
           const double d = dz(i, j);
           bias += d;
           if (d != 0.0)

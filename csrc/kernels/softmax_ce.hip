@@ -6,9 +6,11 @@
 // stores its dz in the operand type and multiplies it into dx and dW while it is in cache.
 //
 // Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers: x and a
-// piece's classes are then copied into split images at a power-of-two scale each, and dz, at most
-// 1 in magnitude, is stored split at the scale 2^14.  A product keeps 22 bits; |dz| below 2^-24
-// keeps an absolute 2^-39.
+// piece's classes are then copied into split images at powers of two, and dz, at most 1 in
+// magnitude, is stored split at the scale 2^14.  A product keeps 22 bits; |dz| below 2^-24 keeps an
+// absolute 2^-39.  Every row of x has a scale of its own in the logits (a row is right whatever the
+// others hold), a piece's classes have one, and so have the rows in dW: there a number keeps an
+// absolute 2^-40 of the largest that takes part in the same sums.
 //
 // Roundings: sums, statistics, losses and dx's slabs are fp32, and a result is rounded once.  With
 // 16-bit operands dz is rounded to their type (at most 2^-8 of it in bf16, 2^-11 in fp16) before
@@ -60,18 +62,21 @@ __device__ inline float half_wave_sum(float v) {
 }
 
 // ------------------------------------------------------------------------------ operand images
-// dst[row][dp] = src[row][0..dim), zero beyond dim and in rows that are left out (target ==
-// ignore, or bias == -inf): an infinity or NaN there must not meet a coefficient of zero in the
-// gradients' products
+// dst[row][dp] = src[row][0..dim), zero beyond dim and in rows that are left out (no class as
+// target, an upstream gradient of zero, or bias == -inf): an infinity or NaN there must not meet a
+// coefficient of zero in the gradients' products, nor a large number set the others' scale.
+// Split images of x: dst at a scale per row, and dst2 at the scale of the largest.
 template <typename T>
 struct PackArgs {
   const T* src;  // null: nothing to do
   int64_t ld, rows;
   int dim, dp;
   const int64_t* target;
-  int64_t ignore;
+  int64_t ignore, classes;
+  const float* grad;  // upstream gradient per row, or null
   const float* bias;
-  void* dst;
+  void *dst, *dst2;
+  int* rowexp;  // exponents of dst's rows, or null: one scale for all
   int lanes;  // log2 of the lanes of a row
   bool vec;   // rows of src are 16-byte aligned
 };
@@ -95,11 +100,13 @@ __device__ inline void load8(const PackArgs<T>& a, int64_t row, int c, T (&v)[8]
 
 template <typename T>
 __device__ inline bool left_out_row(const PackArgs<T>& a, int64_t row) {
-  return a.target ? a.target[row] == a.ignore : a.bias && a.bias[row] == -INFINITY;
+  if (!a.target) return a.bias && a.bias[row] == -INFINITY;
+  const int64_t t = a.target[row];
+  return t == a.ignore || t < 0 || t >= a.classes || (a.grad && a.grad[row] == 0.f);
 }
 
 // Split images: the largest finite magnitude of each operand, by workgroup, and the exponent e
-// that takes it into [2^14, 2^15)
+// that takes a largest magnitude into [2^14, 2^15)
 constexpr int kMaxBlocks = 512;  // workgroups (and partial maxima) of an operand
 
 __device__ inline int scale_exponent(float top) {
@@ -107,6 +114,16 @@ __device__ inline int scale_exponent(float top) {
   int e;
   frexpf(top, &e);  // top = f 2^e, f in [0.5, 1)
   return min(max(15 - e, -126), 126);
+}
+
+template <typename T>
+__device__ inline float finite_max(float m, const T (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = fabsf(static_cast<float>(v[j]));
+    m = x > m && x < INFINITY ? x : m;
+  }
+  return m;
 }
 
 template <typename T>
@@ -119,11 +136,7 @@ __device__ inline float largest(const PackArgs<T>& a, int block, int blocks) {
     for (int c = lane * 8; c < a.dim; c += 8 << a.lanes) {
       T v[8];
       load8(a, row, c, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = fabsf(static_cast<float>(v[j]));
-        m = x > m && x < INFINITY ? x : m;
-      }
+      m = finite_max(m, v);
     }
   }
   return m;
@@ -141,12 +154,12 @@ __device__ inline float block_max(float v, float* red) {
   return v;
 }
 
-// part[0 .. kMaxBlocks): x, part[kMaxBlocks ..): w; every entry of a non-null operand is written
+// part[0 .. kMaxBlocks): x where one scale for all rows is wanted, part[kMaxBlocks ..): w
 template <typename T>
 __global__ __launch_bounds__(1024) void oap_ce_largest(PackArgs<T> x, PackArgs<T> w,
                                                        float* __restrict__ part) {
   __shared__ float red[16];
-  if (x.src) {
+  if (x.src && x.dst2) {
     const float m = block_max(largest(x, blockIdx.x, kMaxBlocks), red);
     if (threadIdx.x == 0) part[blockIdx.x] = m;
   }
@@ -156,27 +169,47 @@ __global__ __launch_bounds__(1024) void oap_ce_largest(PackArgs<T> x, PackArgs<T
   }
 }
 
+// Eight numbers from column c on, split: runs of 32 numbers, their h, then their l
+template <typename T>
+__device__ inline void store_split(void* dst, int64_t row, int dp, int c, const T (&v)[8],
+                                   float scale, bool out) {
+  Vec16<_Float16> h, l;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = out ? 0.f : static_cast<float>(v[j]) * scale;
+    h.v[j] = static_cast<_Float16>(x);
+    l.v[j] = static_cast<_Float16>(x - static_cast<float>(h.v[j]));
+  }
+  _Float16* d = static_cast<_Float16*>(dst) + 2 * (row * dp + (c & ~31)) + (c & 31);
+  *reinterpret_cast<Vec16<_Float16>*>(d) = h;
+  *reinterpret_cast<Vec16<_Float16>*>(d + 32) = l;
+}
+
 // the share of thread t of `threads`
 template <typename T, typename I>
 __device__ inline void pack_rows(const PackArgs<T>& a, float scale, int64_t t, int64_t threads) {
   const int lane = int(t & ((1 << a.lanes) - 1));
   for (int64_t row = t >> a.lanes; row < a.rows; row += threads >> a.lanes) {
     const bool out = left_out_row(a, row);
+    float first = scale;  // of dst
+    if (gt_is_split<I> && a.rowexp) {
+      float m = 0.f;
+      for (int c = lane * 8; c < a.dim; c += 8 << a.lanes) {
+        T v[8];
+        load8(a, row, c, v);
+        m = finite_max(m, v);
+      }
+      for (int k = 1 << a.lanes >> 1; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, 64));
+      const int e = scale_exponent(m);
+      if (lane == 0) a.rowexp[row] = e;
+      first = ldexpf(1.f, e);
+    }
     for (int c = lane * 8; c < a.dp; c += 8 << a.lanes) {
       T v[8];
       load8(a, row, c, v);
       if constexpr (gt_is_split<I>) {
-        Vec16<_Float16> h, l;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = out ? 0.f : v[j] * scale;
-          h.v[j] = static_cast<_Float16>(x);
-          l.v[j] = static_cast<_Float16>(x - static_cast<float>(h.v[j]));
-        }
-        // runs of 32 numbers: their h, then their l
-        _Float16* d = static_cast<_Float16*>(a.dst) + 2 * (row * a.dp + (c & ~31)) + (c & 31);
-        *reinterpret_cast<Vec16<_Float16>*>(d) = h;
-        *reinterpret_cast<Vec16<_Float16>*>(d + 32) = l;
+        store_split(a.dst, row, a.dp, c, v, first, out);
+        if (a.dst2) store_split(a.dst2, row, a.dp, c, v, scale, out);
       } else {
 #pragma unroll
         for (int q = 0; q < 8; q += Vec16<T>::n) {
@@ -196,7 +229,8 @@ struct LogitArgs {
   GtOperand w, x;      // rows: the piece's classes, all rows
   int64_t dp;          // k extent
   const float* bias;   // of the piece, or null
-  const int* scale;    // split images: exponents of x and of the piece's classes
+  const int* scale;    // split images: exponent of the piece's classes
+  const int* rowexp;   // and of every row
   const int64_t* target;
   int64_t class0;      // first class of the piece
   int64_t n;
@@ -270,9 +304,16 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
   Tile::run(a.w, a.x, v0, n0, 0, a.dp, lds, acc);
   const int i0 = Tile::row0(), j0 = Tile::col0();
   const bool masked = left_out != 0, plain = !masked && !a.bias;
-  // what takes a sum of products to the logit in units of ln 2
-  float per = kLog2e;
-  if constexpr (gt_is_split<T>) per = ldexpf(kLog2e, -(a.scale[0] + a.scale[1]));
+  // what takes a row's sums of products to logits in units of ln 2 (finite: a sum of 0 stays 0)
+  float per[Tile::NI];
+#pragma unroll
+  for (int ni = 0; ni < Tile::NI; ++ni) {
+    per[ni] = kLog2e;
+    if constexpr (gt_is_split<T>) {
+      const int64_t n = n0 + j0 + 32 * ni;
+      per[ni] = fminf(ldexpf(kLog2e, -(*a.scale + a.rowexp[n < a.n ? n : a.n - 1])), FLT_MAX);
+    }
+  }
   if (!plain) {
 #pragma unroll
     for (int mi = 0; mi < Tile::MI; ++mi)
@@ -281,7 +322,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
         const float b = sbias[i0 + Tile::row_of(mi, e)];
 #pragma unroll
         for (int ni = 0; ni < Tile::NI; ++ni)
-          acc[mi][ni][e] = __builtin_fmaf(acc[mi][ni][e], per, b);
+          acc[mi][ni][e] = __builtin_fmaf(acc[mi][ni][e], per[ni], b);
       }
   }
   if (masked) {  // a class that is left out has no logit, whatever its weights hold
@@ -296,11 +337,11 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
   }
   // acc: the logits in units of ln 2, or (plain) the sums; one multiply-add takes either to its
   // distance from a row's maximum
-  const float unit = plain ? per : 1.f;
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
     const int j = j0 + 32 * ni;
     const int64_t n = n0 + j;
+    const float unit = plain ? per[ni] : 1.f;
     const int64_t tg = n < a.n ? a.target[n] - a.class0 - v0 - i0 : -1;
     // the target's offset where it may be one of this lane's classes, else -1
     const int tgt = tg >= 0 && tg < Tile::WM ? int(tg) : -1;
@@ -696,7 +737,7 @@ __device__ inline void coefficients(const CoefArgs& a) {
 
 // What a launch of logits reads: the rows' coefficients (workgroup 0), the image of x and that
 // of the piece's classes (shares of the other workgroups), in one launch.  Split images: part
-// holds the partial maxima, and the exponents go to scale[0] (x) and scale[1] (classes).
+// holds the partial maxima, and the exponents go to scale[0] (x, dst2) and scale[1] (classes).
 template <typename T, typename I>
 __global__ __launch_bounds__(1024) void oap_ce_prepare(CoefArgs coef, PackArgs<T> x,
                                                        PackArgs<T> w, const float* part,
@@ -712,14 +753,14 @@ __global__ __launch_bounds__(1024) void oap_ce_prepare(CoefArgs coef, PackArgs<T
   if constexpr (gt_is_split<I>) {
     __shared__ float red[16];
     const int t = threadIdx.x;
-    const int ex = scale_exponent(block_max(t < kMaxBlocks ? part[t] : 0.f, red));
-    const int ew = scale_exponent(block_max(t < kMaxBlocks ? part[kMaxBlocks + t] : 0.f, red));
-    sx = ldexpf(1.f, ex);
-    sw = ldexpf(1.f, ew);
-    if (first == 0) {
-      scale[0] = ex;
-      scale[1] = ew;
+    if (x.src && x.dst2) {
+      const int e = scale_exponent(block_max(t < kMaxBlocks ? part[t] : 0.f, red));
+      if (first == 0) scale[0] = e;
+      sx = ldexpf(1.f, e);
     }
+    const int e = scale_exponent(block_max(t < kMaxBlocks ? part[kMaxBlocks + t] : 0.f, red));
+    if (first == 0) scale[1] = e;
+    sw = ldexpf(1.f, e);
   }
   if (x.src) pack_rows<T, I>(x, sx, first, stride);
   if (w.src) pack_rows<T, I>(w, sw, first, stride);
@@ -985,16 +1026,25 @@ unsigned stride_grid(int64_t threads) {
 template <typename S, typename T>
 struct Ce {
   struct Work {
-    T *ximg, *wimg, *dz;
+    T *ximg, *ximg2, *wimg, *dz;
     float2* part;
     float *zt, *coef, *gscale, *slab, *dbpart, *largest;
-    int* scale;
+    int *scale, *rowexp;
   };
 
   static PackArgs<S> pack(const void* src, int64_t ld, int64_t rows, const CeArgs& a, int64_t dp,
                           const int64_t* target, const float* bias, T* dst) {
-    PackArgs<S> r = {static_cast<const S*>(src), ld, rows, a.dim, int(dp), target, a.ignore, bias,
-                     dst, 0, false};
+    PackArgs<S> r = {};
+    r.src = static_cast<const S*>(src);
+    r.ld = ld;
+    r.rows = rows;
+    r.dim = a.dim;
+    r.dp = int(dp);
+    r.target = target;
+    r.ignore = a.ignore;
+    r.classes = a.classes;
+    r.bias = bias;
+    r.dst = dst;
     while (r.lanes < 6 && (8 << r.lanes) < dp) ++r.lanes;
     r.vec = ld % gt_chunk<S>() == 0 && reinterpret_cast<uintptr_t>(src) % 16 == 0;
     return r;
@@ -1052,6 +1102,7 @@ struct Ce {
     w.zt = c.take<float>(p.rows);
     w.largest = c.take<float>(2 * kMaxBlocks);
     w.scale = c.take<int>(2);
+    w.rowexp = p.split ? c.take<int>(p.rows) : nullptr;
     return c.used;
   }
 
@@ -1063,6 +1114,8 @@ struct Ce {
     w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.largest = c.take<float>(2 * kMaxBlocks);
     w.scale = c.take<int>(2);
+    w.rowexp = p.split ? c.take<int>(p.rows) : nullptr;
+    w.ximg2 = p.split && dw ? c.take<T>(size_t(a.n) * p.dp) : nullptr;
     w.coef = c.take<float>(a.n);
     w.gscale = c.take<float>(1);
     w.dz = c.take<T>(size_t(p.npad) * p.piece);
@@ -1100,11 +1153,13 @@ struct Ce {
     PackArgs<S> px = {}, pw = {};
     l.x = {a.x, a.ldx, a.n, p.dp};
     if (!p.x_direct) {
-      px = pack(a.x, a.ldx, a.n, a, p.dp, nullptr, nullptr, w.ximg);
+      px = pack(a.x, a.ldx, a.n, a, p.dp, a.target, nullptr, w.ximg);
+      px.rowexp = w.rowexp;
       l.x = {w.ximg, p.dp, a.n, p.dp};
     }
     l.dp = p.dp;
-    l.scale = w.scale;
+    l.scale = w.scale + 1;
+    l.rowexp = w.rowexp;
     l.target = a.target;
     l.n = a.n;
     l.ntiles = int(ceil_div(a.n, p.bn));
@@ -1112,14 +1167,15 @@ struct Ce {
     l.zt = w.zt;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
+      const float* bias = a.bias ? a.bias + c0 : nullptr;
       l.w = {wt + c0 * a.ldw, a.ldw, nc, p.dp};
       if (!p.w_direct) {
-        pw = pack(wt + c0 * a.ldw, a.ldw, nc, a, p.dp, nullptr, nullptr, w.wimg);
+        pw = pack(wt + c0 * a.ldw, a.ldw, nc, a, p.dp, nullptr, bias, w.wimg);
         l.w = {w.wimg, p.dp, nc, p.dp};
       }
       prepare({}, px, pw, w, s);
       px.src = nullptr;
-      l.bias = a.bias ? a.bias + c0 : nullptr;
+      l.bias = bias;
       l.class0 = c0;
       l.vtiles = int(ceil_div(nc, p.bm));
       l.part = w.part + c0 / p.bm * p.npad;
@@ -1229,6 +1285,7 @@ struct Ce {
     }
     if (dw) {
       g.b = l.x;
+      if (p.split) g.b.p = w.ximg2;
       g.scale = w.scale;
       g.k = a.n;
       g.m = nc;
@@ -1258,9 +1315,13 @@ struct Ce {
                            w.gscale};
     LogitArgs l = {};
     PackArgs<S> px = pack(a.x, a.ldx, a.n, a, p.dp, a.target, nullptr, w.ximg), pw = {};
+    px.grad = per_row ? grad : nullptr;
+    px.rowexp = w.rowexp;
+    px.dst2 = w.ximg2;
     l.x = {w.ximg, p.dp, a.n, p.dp};
     l.dp = p.dp;
-    l.scale = w.scale;
+    l.scale = w.scale + 1;
+    l.rowexp = w.rowexp;
     l.target = a.target;
     l.n = a.n;
     l.ntiles = int(p.npad / p.bn);

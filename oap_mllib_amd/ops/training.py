@@ -159,7 +159,11 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
     no class and not ``ignore_index`` gives its row the loss NaN and no gradient.
 
     ``reduction``: "mean" over the rows that are not ignored (0 if all are), "sum" or "none"
-    (n losses).  Losses are float32, the gradients of ``x`` and ``weight`` have their type.
+    (n losses; a row with the upstream gradient 0 takes no part in the gradients, whatever ``x``
+    holds there).  Losses are float32, the gradients of ``x`` and ``weight`` have their type.
+    Larger float32 problems form their products from 22 bits of every number (at least 2^-40 of its
+    row's largest in ``x``, of all classes' largest in ``weight``); there, and in float16, rows
+    whose upstream gradient is below 2^-15 of the largest lose bits of their gradient.
     """
     _float_tensor("x", x, 2)
     _float_tensor("weight", weight, 2)

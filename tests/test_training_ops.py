@@ -327,6 +327,72 @@ def test_ce_many_tiles_gpu(dtype, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("what", ["rows", "classes", "targets", "weights"])
+def test_ce_large_numbers_left_out_gpu(what):
+    """Finite numbers of any size in rows and classes that are left out change nothing else (fp32
+    problems whose operands are scaled by their largest number)."""
+    n, v, d = 300, 50_000, 128
+    x, w = rand((n, d), 1, torch.float32, "cuda"), rand((v, d), 2, torch.float32, "cuda", 0.2)
+    t = torch.randint(0, v // 2, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    b = None
+    if what == "classes":
+        b = torch.zeros(v, device="cuda")
+        b[v // 2:] = -INF
+        w[v // 2:] = 1e30
+        ce_check(x, w, t, b)
+        return
+    up = torch.ones(n, device="cuda")
+    if what == "weights":
+        up[::3] = 0  # (rows with a loss of their own)
+    else:
+        t[::3] = -100 if what == "rows" else v + 5
+    clean = [q.clone().requires_grad_() for q in (x, w)]
+    x[::3] = 1e30
+    dirty = [q.requires_grad_() for q in (x, w)]
+    loss = []
+    for leaves in (clean, dirty):
+        rows = ops.softmax_cross_entropy(*leaves, t, reduction="none")
+        loss.append((rows.detach()[up > 0], *torch.autograd.grad(rows, leaves, up)))
+    if what == "rows":
+        ce_check(clean[0].detach(), clean[1].detach(), t, None)
+    for a, c in zip(*loss):
+        assert torch.equal(a.nan_to_num(7.0), c.nan_to_num(7.0))
+
+
+@pytest.mark.gpu
+def test_ce_rows_of_any_size_gpu():
+    """A row's loss and its gradient of x do not depend on what the other rows hold."""
+    n, v, d = 300, 50_000, 128
+    x, w = rand((n, d), 1, torch.float32, "cuda"), rand((v, d), 2, torch.float32, "cuda", 0.2)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    x[1::3] *= 1e-12
+    got = []
+    for big in (1.0, 1e12):
+        leaf = torch.cat([x[:150], x[150:] * big]).requires_grad_()
+        rows = ops.softmax_cross_entropy(leaf, w, t, reduction="none")
+        got.append((rows.detach()[:150], torch.autograd.grad(rows.sum(), leaf)[0][:150]))
+    for a, c in zip(*got):
+        assert torch.equal(a, c)
+    ce_check(x, w, t, None, reduction="none")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_ce_rows_without_upstream_gradient(device):
+    x, w = rand((6, 9), 1, device=device), rand((11, 9), 2, device=device).requires_grad_()
+    t = torch.tensor([0, 3, 10, 5, 5, 1], device=device)
+    up = torch.tensor([1.0, 0.0, -2.0, 0.0, 0.5, 1.0], device=device)
+    got = []
+    for bad in (0.0, math.nan):
+        leaf = x.clone()
+        leaf[1], leaf[3] = bad, -bad
+        leaf.requires_grad_()
+        rows = ops.softmax_cross_entropy(leaf, w, t, reduction="none")
+        got.append(torch.autograd.grad(rows, [leaf, w], up))
+    for a, c in zip(*got):
+        assert torch.equal(a, c) and not a.isnan().any()
+
+
+@pytest.mark.gpu
 def test_ce_rows_in_turns_gpu():
     """More rows than one turn of the forward pass keeps statistics for: every row's loss is that
     of a call on its own part of the rows, but for the order in which 15625 tiles' sums are joined

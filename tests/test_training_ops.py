@@ -327,6 +327,24 @@ def test_ce_many_tiles_gpu(dtype, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(50, 30_001, 72), (33, 26_000, 1100), (700, 20_003, 1100),
+                                   (257, 15_000, 1032), (300, 9000, 100)])
+def test_ce_each_tile_gpu(dtype, n, v, d):
+    """Few rows of many classes, the largest tiles (long rows), and middling problems; rows with
+    a stride, left-out rows and classes."""
+    x = rand((n, d + 8), 1, dtype, "cuda", 0.3)[:, :d]
+    w = rand((v, d), 2, dtype, "cuda", 0.3)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    b = rand((v,), 4)
+    b[3::17] = -INF
+    b[t] = 0.5
+    t[::9] = -100
+    ce_check(x, w, t.cuda(), b.cuda(), reduction="sum")
+    ce_check(x, w, t.cuda(), None, want=(True, False, False))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["rows", "classes", "targets", "weights"])
 def test_ce_large_numbers_left_out_gpu(what):
     """Finite numbers of any size in rows and classes that are left out change nothing else (fp32

@@ -494,8 +494,8 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 // A few rows (one, or up to four): the class rows are read once from memory and that is what
 // bounds it, so they go straight into registers.  G lanes share a class, four 16-byte chunks
 // each; the rows of x stay in registers; every group keeps its own (max, sum) and the workgroup
-// joins them.  The chip streams classes with enough loads in flight: two classes per lane group.
-// One row, 2M x 100 fp32: 142 us, 5.6 TB/s.
+// joins them.  One row, 2M x 100 fp32: 137 us, 5.8 TB/s (two classes at a time in a lane group, or
+// twice the workgroups, 141 to 147 us: the loads of 4 workgroups a CU are enough in flight).
 struct FewArgs {
   const void *w, *x;
   int64_t ldw, ldx, classes;
@@ -506,7 +506,7 @@ struct FewArgs {
   float* zt;
 };
 
-constexpr int kFewBlocks = 2048;
+constexpr int kFewBlocks = 1024;
 constexpr int kFewRows = 4;
 constexpr int kFewIters = 4;
 
@@ -536,43 +536,34 @@ __global__ __launch_bounds__(256) void oap_ce_few(FewArgs a) {
     s[r] = 0.f;
   }
   const T* w = static_cast<const T*>(a.w);
-  const int64_t step = int64_t(gridDim.x) * GROUPS;
-  for (int64_t c0 = int64_t(blockIdx.x) * GROUPS + g; c0 < a.classes; c0 += 2 * step) {
-    Vec16<T> v[2][kFewIters];
+  for (int64_t c = int64_t(blockIdx.x) * GROUPS + g; c < a.classes;
+       c += int64_t(gridDim.x) * GROUPS) {
+    Vec16<T> v[kFewIters];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t c = c0 + u * step < a.classes ? c0 + u * step : c0;
-#pragma unroll
-      for (int i = 0; i < kFewIters; ++i) {
-        v[u][i] = {};
-        if ((q + i * G) * CH < a.dim)
-          v[u][i] = *reinterpret_cast<const Vec16<T>*>(w + c * a.ldw + (q + i * G) * CH);
-      }
+    for (int i = 0; i < kFewIters; ++i) {
+      v[i] = {};
+      if ((q + i * G) * CH < a.dim)
+        v[i] = *reinterpret_cast<const Vec16<T>*>(w + c * a.ldw + (q + i * G) * CH);
     }
+    float b = a.bias ? a.bias[c] : 0.f;
+    const bool out = b == -INFINITY;
+    if (!out) b = fmaxf(b * kLog2e, -FLT_MAX);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t c = c0 + u * step;
-      if (c >= a.classes) break;  // (uniform in the group)
-      float b = a.bias ? a.bias[c] : 0.f;
-      const bool out = b == -INFINITY;
-      if (!out) b = fmaxf(b * kLog2e, -FLT_MAX);
+    for (int r = 0; r < N; ++r) {
+      float z = 0.f;
 #pragma unroll
-      for (int r = 0; r < N; ++r) {
-        float z = 0.f;
+      for (int i = 0; i < kFewIters; ++i)
 #pragma unroll
-        for (int i = 0; i < kFewIters; ++i)
+        for (int j = 0; j < CH; ++j)
+          z = __builtin_fmaf(x[r][i][j], static_cast<float>(v[i].v[j]), z);
 #pragma unroll
-          for (int j = 0; j < CH; ++j)
-            z = __builtin_fmaf(x[r][i][j], static_cast<float>(v[u][i].v[j]), z);
-#pragma unroll
-        for (int k = G / 2; k >= 1; k >>= 1) z += __shfl_xor(z, k, 64);
-        z = out ? -INFINITY : __builtin_fmaf(z, kLog2e, b);
-        if (c == tgt[r] && q == 0) a.zt[r] = z;
-        // (NaN stays in the sum)
-        const float mm = fmaxf(m[r], z), ref = mm > -INFINITY ? mm : 0.f;
-        s[r] = s[r] * pow2(m[r] - ref) + pow2(z - ref);
-        m[r] = mm;
-      }
+      for (int k = G / 2; k >= 1; k >>= 1) z += __shfl_xor(z, k, 64);
+      z = out ? -INFINITY : __builtin_fmaf(z, kLog2e, b);
+      if (c == tgt[r] && q == 0) a.zt[r] = z;
+      // (NaN stays in the sum)
+      const float mm = fmaxf(m[r], z), ref = mm > -INFINITY ? mm : 0.f;
+      s[r] = s[r] * pow2(m[r] - ref) + pow2(z - ref);
+      m[r] = mm;
     }
   }
 #pragma unroll

@@ -491,35 +491,84 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
   }
 }
 
-// A few rows (one, or up to four): the class rows are read once from memory and that is what
-// bounds it, so they go straight into registers.  G lanes share a class, four 16-byte chunks
-// each; the rows of x stay in registers; every group keeps its own (max, sum) and the workgroup
-// joins them.  One row, 2M x 100 fp32: 137 us, 5.8 TB/s (two classes at a time in a lane group, or
-// twice the workgroups, 141 to 147 us: the loads of 4 workgroups a CU are enough in flight).
+// A few rows (up to eight): the class rows are read once from memory and that is what bounds it,
+// so they go straight into registers.  G lanes share a class, ITERS 16-byte chunks each; the rows
+// of x stay in registers.  The sums over the lanes are formed so that a lane ends with the logit of
+// one row (as many rows at once as there are), and keeps that row's (max, sum) over the group's
+// classes; the workgroup joins them.
+// 2M x 100 fp32: one row 135 us (5.9 TB/s), four 140, eight 166 (tiles: 237 and 260); 8-byte loads
+// 202, single elements (101 features) 206 us; one row in bf16, 8-byte loads, 123 us.
 struct FewArgs {
   const void *w, *x;
   int64_t ldw, ldx, classes;
   int n, dim;
+  int width;  // bytes of a load that the class rows' alignment allows: 16, 8, or 0 for an element
   const float* bias;
   const int64_t* target;
   float2* part;  // [workgroup][n]
   float* zt;
 };
 
-constexpr int kFewBlocks = 1024;
-constexpr int kFewRows = 4;
-constexpr int kFewIters = 4;
+constexpr int kFewBlocks = 1024;  // 4 per CU: their loads in flight are enough
+constexpr int kFewRows = 8;
+// chunks of a lane: the rows of x take 64 registers, or 128 (eight rows)
+constexpr int few_iters(int rows, int element) { return rows > 1 && element == 2 ? 2 : 4; }
 
-template <typename T, int N, int G>
+// One step of a sum over lanes, B the bit in which the lane's partner differs.  The partners of 8
+// and 4 differ in the lower bits too, so the steps go from the highest bit down.
+template <int B>
+__device__ inline float lane_partner(float v) {
+  constexpr int CTRL = B == 8 ? 0x140 : B == 4 ? 0x141 : B == 2 ? 0x4E : 0xB1;
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// sum of a in the lanes without bit B, of b in those with it
+template <int B>
+__device__ inline float lane_halves(float a, float b, int lane) {
+  const unsigned ua = unsigned(__float_as_int(a)), ub = unsigned(__float_as_int(b));
+  if constexpr (B == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(ua, ub, false, false);
+    return __int_as_float(int(r[0])) + __int_as_float(int(r[1]));
+  } else if constexpr (B == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(ua, ub, false, false);
+    return __int_as_float(int(r[0])) + __int_as_float(int(r[1]));
+  } else {
+    const bool second = lane & B;
+    return (second ? b : a) + lane_partner<B>(second ? a : b);
+  }
+}
+// z[0 .. N) summed over groups of 2 B lanes; the group's lanes end with N / (2 B)-ths of the rows
+template <int B, int N>
+__device__ inline float lane_sums(float (&z)[N], int lane) {
+  if constexpr (B == 0) {
+    return z[0];
+  } else if constexpr (N == 1) {
+    float w[1] = {lane_halves<B>(z[0], z[0], lane)};
+    return lane_sums<B / 2>(w, lane);
+  } else {
+    float w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = lane_halves<B>(z[i], z[i + N / 2], lane);
+    return lane_sums<B / 2>(w, lane);
+  }
+}
+
+// WIDE: the class rows are whole 16-byte chunks
+template <typename T, int N, int G, bool WIDE>
 __global__ __launch_bounds__(256) void oap_ce_few(FewArgs a) {
-  constexpr int CH = gt_chunk<T>(), GROUPS = 256 / G;
+  constexpr int CH = gt_chunk<T>(), GROUPS = 256 / G, ITERS = few_iters(N, sizeof(T));
+  constexpr int PER = G / N;  // lanes of a group that end with the same row
+  static_assert(PER >= 1, "a lane for every row");
+  struct alignas(8) Half {
+    T v[CH / 2];
+  };
   __shared__ float2 red[N][GROUPS];
-  const int q = threadIdx.x & (G - 1), g = threadIdx.x / G;
-  float x[N][kFewIters][CH];
+  const int q = threadIdx.x & (G - 1), g = threadIdx.x / G, mine = q / PER;
+  float x[N][ITERS][CH];
 #pragma unroll
   for (int r = 0; r < N; ++r)
 #pragma unroll
-    for (int i = 0; i < kFewIters; ++i)
+    for (int i = 0; i < ITERS; ++i)
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
         const int k = (q + i * G) * CH + j;
@@ -527,48 +576,55 @@ __global__ __launch_bounds__(256) void oap_ce_few(FewArgs a) {
                          ? static_cast<float>(static_cast<const T*>(a.x)[r * a.ldx + k])
                          : 0.f;
       }
-  int64_t tgt[N];
-  float m[N], s[N];
-#pragma unroll
-  for (int r = 0; r < N; ++r) {
-    tgt[r] = r < a.n ? a.target[r] : -1;
-    m[r] = -INFINITY;
-    s[r] = 0.f;
-  }
+  const int64_t tgt = mine < a.n && q % PER == 0 ? a.target[mine] : -1;
+  float m = -INFINITY, s = 0.f;
   const T* w = static_cast<const T*>(a.w);
   for (int64_t c = int64_t(blockIdx.x) * GROUPS + g; c < a.classes;
        c += int64_t(gridDim.x) * GROUPS) {
-    Vec16<T> v[kFewIters];
+    Vec16<T> v[ITERS];
 #pragma unroll
-    for (int i = 0; i < kFewIters; ++i) {
+    for (int i = 0; i < ITERS; ++i) {
       v[i] = {};
-      if ((q + i * G) * CH < a.dim)
-        v[i] = *reinterpret_cast<const Vec16<T>*>(w + c * a.ldw + (q + i * G) * CH);
+      const int k = (q + i * G) * CH;
+      const T* p = w + c * a.ldw + k;
+      if (WIDE) {
+        if (k < a.dim) v[i] = *reinterpret_cast<const Vec16<T>*>(p);
+      } else if (a.width == 8) {
+#pragma unroll
+        for (int h = 0; h < CH; h += CH / 2)
+          if (k + h < a.dim) {
+            const Half o = *reinterpret_cast<const Half*>(p + h);
+#pragma unroll
+            for (int j = 0; j < CH / 2; ++j) v[i].v[h + j] = o.v[j];
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+          if (k + j < a.dim) v[i].v[j] = p[j];
+      }
     }
     float b = a.bias ? a.bias[c] : 0.f;
     const bool out = b == -INFINITY;
     if (!out) b = fmaxf(b * kLog2e, -FLT_MAX);
+    float sums[N];
 #pragma unroll
     for (int r = 0; r < N; ++r) {
-      float z = 0.f;
+      sums[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < kFewIters; ++i)
+      for (int i = 0; i < ITERS; ++i)
 #pragma unroll
         for (int j = 0; j < CH; ++j)
-          z = __builtin_fmaf(x[r][i][j], static_cast<float>(v[i].v[j]), z);
-#pragma unroll
-      for (int k = G / 2; k >= 1; k >>= 1) z += __shfl_xor(z, k, 64);
-      z = out ? -INFINITY : __builtin_fmaf(z, kLog2e, b);
-      if (c == tgt[r] && q == 0) a.zt[r] = z;
-      // (NaN stays in the sum)
-      const float mm = fmaxf(m[r], z), ref = mm > -INFINITY ? mm : 0.f;
-      s[r] = s[r] * pow2(m[r] - ref) + pow2(z - ref);
-      m[r] = mm;
+          sums[r] = __builtin_fmaf(x[r][i][j], static_cast<float>(v[i].v[j]), sums[r]);
     }
+    float z = lane_sums<G / 2>(sums, q);
+    z = out ? -INFINITY : __builtin_fmaf(z, kLog2e, b);
+    if (c == tgt) a.zt[mine] = z;
+    // (NaN stays in the sum)
+    const float mm = fmaxf(m, z), ref = mm > -INFINITY ? mm : 0.f;
+    s = s * pow2(m - ref) + pow2(z - ref);
+    m = mm;
   }
-#pragma unroll
-  for (int r = 0; r < N; ++r)
-    if (q == 0) red[r][g] = make_float2(m[r], s[r]);
+  if (q % PER == 0) red[mine][g] = make_float2(m, s);
   __syncthreads();
   if (threadIdx.x < unsigned(a.n)) {
     const int r = threadIdx.x;
@@ -950,7 +1006,13 @@ Plan make_plan(const CeArgs& a, bool grad) {
   // operands while k is short (1024 x 2M x 100 10.6 against 11.7 ms; 2048 x 20000 x 1000 1.10
   // against 1.09 ms).  fp32 keeps two: that loop skips the empty steps of a short k.
   p.single = es == 2 || (p.split && p.dp <= 512);
-  if (p.bn == 64 && p.bm > 64) p.bm = 256;  // few rows of many classes
+  // few rows of many classes (16 x 2M x 100 fp32 in tiles of 32 rows 260 us, of 64 390 us; one
+  // buffer for those of 64, 377 against 394 us, two for those of 32, 188 against 201 us for 8 x
+  // 400000 x 1000 bf16)
+  if (p.bn == 64 && p.bm > 64) {
+    p.bm = 256;
+    if (a.n <= 32) p.bn = 32;
+  }
   // the forward pass keeps 8 bytes of each row and class tile: as many rows at a time as take
   // 1 GiB, at least 4096
   p.rows = a.n;
@@ -979,10 +1041,20 @@ Plan make_plan(const CeArgs& a, bool grad) {
   return p;
 }
 
-// Features that the lane groups of oap_ce_few cover
+int few_width(const CeArgs& a) {
+  const int64_t es = elem_size(a.elem);
+  const uintptr_t of = uintptr_t(a.dim * es) | uintptr_t(a.ldw * es) |
+                       reinterpret_cast<uintptr_t>(a.w);
+  return of % 16 == 0 ? 16 : of % 8 == 0 ? 8 : 0;
+}
+
+// Whether oap_ce_few takes the call: the rows and features that its lane groups cover.  In 16 bits
+// the conversions weigh, and tiles are faster (4 x 400000 x 1000 bf16 179 against 281 us) unless
+// they need an image of classes that are not aligned (4 x 2M x 100 bf16 369 against 124 us).
 bool few_rows(const CeArgs& a) {
-  return a.n <= kFewRows && a.dim <= 64 * kFewIters * 16 / elem_size(a.elem) &&
-         direct(a, a.w, a.ldw);
+  const int es = elem_size(a.elem);
+  if (a.n > kFewRows || a.dim > 64 * few_iters(int(a.n), es) * 16 / es) return false;
+  return es == 4 || a.n == 1 || (a.n <= 4 && few_width(a) < 16);
 }
 
 struct Carver {
@@ -1067,8 +1139,10 @@ struct Ce {
   static void logits(const Plan& p, const LogitArgs& l, hipStream_t s) {
     if (p.bm == 64)
       logits_tile<64, 64, 2, false, GRAD>(l, s);
+    else if (p.bn == 32)
+      logits_tile<256, 32, 4, false, GRAD>(l, s);
     else if (p.bn == 64)
-      logits_tile<256, 64, 4, false, GRAD>(l, s);
+      logits_tile<256, 64, 4, true, GRAD>(l, s);
     else if (p.bn == 128 && p.bm == 256) {
       if constexpr (sizeof(T) == 2) logits_tile<256, 128, 2, true, GRAD>(l, s);
     } else if (p.bn == 128 && p.single)
@@ -1204,13 +1278,16 @@ struct Ce {
   static int few_launch(const FewArgs& f, hipStream_t s) {
     const int blocks =
         int(std::max<int64_t>(1, std::min<int64_t>(kFewBlocks, ceil_div(f.classes, 256 / G))));
-    oap_ce_few<S, N, G><<<dim3(unsigned(blocks)), 256, 0, s>>>(f);
+    if (f.width == 16)
+      oap_ce_few<S, N, G, true><<<dim3(unsigned(blocks)), 256, 0, s>>>(f);
+    else
+      oap_ce_few<S, N, G, false><<<dim3(unsigned(blocks)), 256, 0, s>>>(f);
     OAP_HIP_CHECK(hipGetLastError());
     return blocks;
   }
   template <int N>
   static int few_lanes(const FewArgs& f, hipStream_t s) {
-    const int per = kFewIters * gt_chunk<S>();  // features of a lane
+    const int per = few_iters(N, sizeof(S)) * gt_chunk<S>();  // features of a lane
     if (f.dim <= 8 * per) return few_launch<N, 8>(f, s);
     if (f.dim <= 16 * per) return few_launch<N, 16>(f, s);
     if (f.dim <= 32 * per) return few_launch<N, 32>(f, s);
@@ -1225,11 +1302,15 @@ struct Ce {
     f.classes = a.classes;
     f.n = int(a.n);
     f.dim = a.dim;
+    f.width = few_width(a);
     f.bias = a.bias;
     f.target = a.target;
     f.part = w.part;
     f.zt = w.zt;
-    return a.n == 1 ? few_lanes<1>(f, s) : few_lanes<kFewRows>(f, s);
+    if (a.n == 1) return few_lanes<1>(f, s);
+    if constexpr (sizeof(S) == 4)
+      if (a.n > 4) return few_lanes<8>(f, s);
+    return few_lanes<4>(f, s);
   }
 
   template <int B>

@@ -345,6 +345,26 @@ def test_ce_each_tile_gpu(dtype, n, v, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(5, 5000, 100), (6, 3000, 1032), (7, 33, 40), (8, 999, 1024),
+                                   (8, 30_000, 64), (5, 7, 8), (2, 2000, 200), (8, 1, 4),
+                                   (9, 40_000, 8), (20, 30_001, 100), (32, 26_000, 300)])
+def test_ce_small_batches_gpu(dtype, n, v, d):
+    """Up to eight rows at once from registers, up to 32 in narrow tiles."""
+    x, w = rand((n, d), 1, dtype, "cuda", 0.5), rand((v, d), 2, dtype, "cuda", 0.5)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    b = rand((v,), 4)
+    b[1::7] = -INF
+    b[t] = 0.5
+    for bias in (None, b.cuda()):
+        ce_check(x, w, t.cuda(), bias, reduction="none")
+    t[n // 2] = -100
+    x[n // 2] = math.nan
+    w[b.cuda() == -INF] = math.nan
+    ce_check(x, w, t.cuda(), b.cuda(), want=(True, True, True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["rows", "classes", "targets", "weights"])
 def test_ce_large_numbers_left_out_gpu(what):
     """Finite numbers of any size in rows and classes that are left out change nothing else (fp32

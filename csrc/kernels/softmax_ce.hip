@@ -965,9 +965,9 @@ constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
 // fp32 problems of more than 128 rows and at least this many products take the split operands:
 // their images cost two launches and two passes over the weights (1024 x 20000 x 128: 181 against
-// 259 us with gradients, 2048 x 20000 x 1000 1.09 against 2.45 ms; 300 x 5000 x 512 147 against 130
-// us, 200 x 20000 x 300 without gradients 52 against 47 us; 192 x 1M x 100 1.78 against 2.14 ms, but
-// 128 x 1M x 100, one row tile, 1.54 against 1.38 ms, without gradients 420 against 309 us).
+// 259 us with gradients, 2048 x 20000 x 1000 1.09 against 2.45 ms; 300 x 5000 x 512 147 against
+// 130 us, 200 x 20000 x 300 without gradients 52 against 47 us; 192 x 1M x 100 1.78 against 2.14
+// ms, but 128 x 1M x 100, one row tile, 1.54 against 1.38 ms, without gradients 420 against 309 us).
 constexpr double kSplitWork = 1.5e9;
 
 // Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps

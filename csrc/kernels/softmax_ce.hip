@@ -250,8 +250,8 @@ struct LogitArgs {
 
 // Tile of a workgroup: workgroups go to the 8 XCDs in turn, so each XCD takes a run of
 // consecutive tiles and its L2 sees the same class rows again for every row tile.
-__device__ inline int xcd_tile(int total) {
-  const int b = blockIdx.x, per = total >> 3, rest = total & 7;
+__device__ inline int xcd_tile(int b, int total) {
+  const int per = total >> 3, rest = total & 7;
   const int x = b & 7, i = b >> 3;
   return x * per + (x < rest ? x : rest) + i;
 }
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
   __shared__ int left_out;
   const int tid = threadIdx.x, lane = tid & 63;
   int vt, nt;
-  tile_at(xcd_tile(a.vtiles * a.ntiles), a.vtiles, a.ntiles, vt, nt);
+  tile_at(xcd_tile(blockIdx.x, a.vtiles * a.ntiles), a.vtiles, a.ntiles, vt, nt);
   const int v0 = vt * BM, n0 = nt * BN;
   if (tid == 0) left_out = 0;
   __syncthreads();
@@ -831,10 +831,9 @@ struct ProdArgs {
 // part to the same elements, so the order of the sums is fixed.  65536 classes of 8192 x 2048
 // bf16: 2.03 ms (1.08 PF/s); dW of them 2.07 ms (1.06 PF/s).
 template <typename T, int BM, int BN, int WAVES_M>
-__global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dx(ProdArgs a) {
+__device__ void dx_tile(const ProdArgs& a, int block, char* lds) {
   typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M> Tile;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int t = xcd_tile(a.mtiles * a.ntiles * a.splits);
+  const int t = xcd_tile(block, a.mtiles * a.ntiles * a.splits);
   const int sp = t / (a.mtiles * a.ntiles), u = t - sp * a.mtiles * a.ntiles;
   int mt, nt;
   tile_at(u, a.mtiles, a.ntiles, mt, nt);
@@ -864,6 +863,48 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dx(Pr
             *o = a.add ? *o + v : v;
           }
     }
+}
+
+template <typename S, typename T, int BM, int BN, int WAVES_M>
+__device__ void dw_tile(const ProdArgs& a, int block, char* lds) {
+  typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M> Tile;
+  int mt, nt;
+  tile_at(xcd_tile(block, a.mtiles * a.ntiles), a.mtiles, a.ntiles, mt, nt);
+  gt_f32x16 acc[Tile::MI][Tile::NI];
+  Tile::clear(acc);
+  Tile::run(a.a, a.b, mt * BM, nt * BN, 0, a.k, lds, acc);
+  const float per = gt_is_split<T> ? ldexpf(a.unscale, -*a.scale) : a.unscale;
+  const float g = *a.gscale;
+  S* out = static_cast<S*>(a.out);
+  const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
+#pragma unroll
+  for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t i = i0 + Tile::row_of(mi, e);
+      if (i >= a.m) continue;
+      const bool out_of = a.bias && a.bias[i] == -INFINITY;
+#pragma unroll
+      for (int ni = 0; ni < Tile::NI; ++ni) {
+        const int64_t j = j0 + 32 * ni;
+        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : acc[mi][ni][e] * per * g);
+      }
+    }
+}
+
+// Both products of a piece in one launch, dx's workgroups (each with more of k) first: the last of
+// one fill up with the first of the other (bf16 with gradients, 3000 x 20000 x 784 618 against 628
+// us, 300 x 50001 x 1000 235 against 259 us).  The largest tiles have no registers for both and
+// take a launch each.
+enum GradPart { kBoth, kDx, kDw };
+template <typename S, typename T, int B, GradPart PART>
+__global__ __launch_bounds__(kGtThreads, gt_occupancy(B, B)) void oap_ce_grads(ProdArgs x,
+                                                                            ProdArgs w, int nx) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  if (PART == kDx || (PART == kBoth && int(blockIdx.x) < nx))
+    dx_tile<T, B, B, 2>(x, blockIdx.x, lds);
+  else
+    dw_tile<S, T, B, B, 2>(w, blockIdx.x - nx, lds);
 }
 
 // What is left of a piece: db of its classes (the first workgroups), and after the last piece the
@@ -900,34 +941,6 @@ __global__ __launch_bounds__(256) void oap_ce_finish(FinishArgs<T> a) {
     for (int s = 0; s < a.splits; ++s) v += a.slab[int64_t(s) * a.count + i];
     a.dx[i] = static_cast<T>(v * (g * a.unscale));
   }
-}
-
-template <typename S, typename T, int BM, int BN, int WAVES_M>
-__global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_dw(ProdArgs a) {
-  typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M> Tile;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  int mt, nt;
-  tile_at(xcd_tile(a.mtiles * a.ntiles), a.mtiles, a.ntiles, mt, nt);
-  gt_f32x16 acc[Tile::MI][Tile::NI];
-  Tile::clear(acc);
-  Tile::run(a.a, a.b, mt * BM, nt * BN, 0, a.k, lds, acc);
-  const float per = gt_is_split<T> ? ldexpf(a.unscale, -*a.scale) : a.unscale;
-  const float g = *a.gscale;
-  S* out = static_cast<S*>(a.out);
-  const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
-#pragma unroll
-  for (int mi = 0; mi < Tile::MI; ++mi)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t i = i0 + Tile::row_of(mi, e);
-      if (i >= a.m) continue;
-      const bool out_of = a.bias && a.bias[i] == -INFINITY;
-#pragma unroll
-      for (int ni = 0; ni < Tile::NI; ++ni) {
-        const int64_t j = j0 + 32 * ni;
-        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : acc[mi][ni][e] * per * g);
-      }
-    }
 }
 
 template <typename S>
@@ -967,7 +980,7 @@ constexpr int64_t kPieceBytes = int64_t(1) << 30;
 // their images cost two launches and two passes over the weights (1024 x 20000 x 128: 181 against
 // 259 us with gradients, 2048 x 20000 x 1000 1.09 against 2.45 ms; 300 x 5000 x 512 147 against
 // 130 us, 200 x 20000 x 300 without gradients 52 against 47 us; 192 x 1M x 100 1.78 against 2.14
-// ms, but 128 x 1M x 100, one row tile, 1.54 against 1.38 ms, without gradients 420 against 309 us).
+// ms, but 128 x 1M x 100, one row tile, 1.54 against 1.38 ms, without gradients 420 against 309).
 constexpr double kSplitWork = 1.5e9;
 
 // Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps
@@ -1315,65 +1328,66 @@ struct Ce {
     return few_lanes<4>(f, s);
   }
 
-  template <int B>
-  static void dx_tile(const ProdArgs& g, hipStream_t s) {
-    constexpr int lds = GtTile<T, B, kAlongK, B, kAcrossK, 2>::kLds;
-    auto k = oap_ce_dx<T, B, B, 2>;
+  // dx's tiles and dW's; none where out is null
+  template <int B, GradPart PART>
+  static void grads_tile(const ProdArgs& x, const ProdArgs& w, hipStream_t s) {
+    constexpr int lds = std::max(GtTile<T, B, kAlongK, B, kAcrossK, 2>::kLds,
+                                 GtTile<T, B, kAcrossK, B, kAcrossK, 2>::kLds);
+    const int nx = x.out && PART != kDw ? x.mtiles * x.ntiles * x.splits : 0;
+    const int nw = w.out && PART != kDx ? w.mtiles * w.ntiles : 0;
+    if (nx + nw == 0) return;
+    auto k = oap_ce_grads<S, T, B, PART>;
     set_lds(k, lds);
-    k<<<dim3(unsigned(g.mtiles * g.ntiles * g.splits)), kGtThreads, lds, s>>>(g);
+    k<<<dim3(unsigned(nx + nw)), kGtThreads, lds, s>>>(x, w, nx);
     OAP_HIP_CHECK(hipGetLastError());
   }
-  template <int B>
-  static void dw_tile(const ProdArgs& g, hipStream_t s) {
-    constexpr int lds = GtTile<T, B, kAcrossK, B, kAcrossK, 2>::kLds;
-    auto k = oap_ce_dw<S, T, B, B, 2>;
-    set_lds(k, lds);
-    k<<<dim3(unsigned(g.mtiles * g.ntiles)), kGtThreads, lds, s>>>(g);
-    OAP_HIP_CHECK(hipGetLastError());
+  static void grads(int tile, const ProdArgs& x, const ProdArgs& w, hipStream_t s) {
+    if (tile == 64) {
+      grads_tile<64, kBoth>(x, w, s);
+    } else if (tile == 128) {
+      grads_tile<128, kBoth>(x, w, s);
+    } else if constexpr (sizeof(T) == 2) {
+      grads_tile<256, kDx>(x, w, s);
+      grads_tile<256, kDw>(x, w, s);
+    }
   }
 
   static void products(const CeArgs& a, const Plan& p, const Work& w, const LogitArgs& l,
                        int64_t nc, int64_t c0, float unscale, void* dx, void* dw,
                        hipStream_t s) {
-    ProdArgs g = {};
-    g.n = a.dim;
-    g.gscale = w.gscale;
-    g.unscale = unscale;
-    g.a = {w.dz, p.piece, p.npad, p.piece};
+    ProdArgs gx = {}, gw = {};
+    gx.n = gw.n = a.dim;
+    gx.gscale = gw.gscale = w.gscale;
+    gx.unscale = gw.unscale = unscale;
+    gx.a = gw.a = {w.dz, p.piece, p.npad, p.piece};
     if (dx) {
-      g.b = l.w;
-      g.scale = w.scale + 1;
-      g.k = nc;
-      g.m = a.n;
-      g.mtiles = int(ceil_div(a.n, p.xtile));
-      g.ntiles = int(ceil_div(a.dim, p.xtile));
-      g.splits = p.splits;
-      g.out = w.slab;
-      g.add = c0 > 0;
-      if (p.xtile == 64)
-        dx_tile<64>(g, s);
-      else if (p.xtile == 128)
-        dx_tile<128>(g, s);
-      else if constexpr (sizeof(T) == 2)
-        dx_tile<256>(g, s);
+      gx.b = l.w;
+      gx.scale = w.scale + 1;
+      gx.k = nc;
+      gx.m = a.n;
+      gx.mtiles = int(ceil_div(a.n, p.xtile));
+      gx.ntiles = int(ceil_div(a.dim, p.xtile));
+      gx.splits = p.splits;
+      gx.out = w.slab;
+      gx.add = c0 > 0;
     }
     if (dw) {
-      g.b = l.x;
-      if (p.split) g.b.p = w.ximg2;
-      g.scale = w.scale;
-      g.k = a.n;
-      g.m = nc;
-      g.mtiles = int(ceil_div(nc, p.wtile));
-      g.ntiles = int(ceil_div(a.dim, p.wtile));
-      g.splits = 1;
-      g.out = static_cast<S*>(dw) + c0 * a.dim;
-      g.bias = a.bias ? a.bias + c0 : nullptr;
-      if (p.wtile == 64)
-        dw_tile<64>(g, s);
-      else if (p.wtile == 128)
-        dw_tile<128>(g, s);
-      else if constexpr (sizeof(T) == 2)
-        dw_tile<256>(g, s);
+      gw.b = l.x;
+      if (p.split) gw.b.p = w.ximg2;
+      gw.scale = w.scale;
+      gw.k = a.n;
+      gw.m = nc;
+      gw.mtiles = int(ceil_div(nc, p.wtile));
+      gw.ntiles = int(ceil_div(a.dim, p.wtile));
+      gw.splits = 1;
+      gw.out = static_cast<S*>(dw) + c0 * a.dim;
+      gw.bias = a.bias ? a.bias + c0 : nullptr;
+    }
+    if (p.xtile == p.wtile) {
+      grads(p.xtile, gx, gw, s);
+    } else {
+      grads(p.xtile, gx, {}, s);
+      grads(p.wtile, {}, gw, s);
     }
   }
 

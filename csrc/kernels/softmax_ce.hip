@@ -299,21 +299,27 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
     if (b == -INFINITY) left_out = 1;
   }
   __syncthreads();
+  const int i0 = Tile::row0(), j0 = Tile::col0();
+  int ex[Tile::NI] = {};  // (loaded ahead of the products, which hide the wait)
+  if constexpr (gt_is_split<T>) {
+#pragma unroll
+    for (int ni = 0; ni < Tile::NI; ++ni) {
+      const int64_t n = n0 + j0 + 32 * ni;
+      ex[ni] = a.rowexp[n < a.n ? n : a.n - 1];
+    }
+  }
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
   Tile::run(a.w, a.x, v0, n0, 0, a.dp, lds, acc);
-  const int i0 = Tile::row0(), j0 = Tile::col0();
-  const bool masked = left_out != 0, plain = !masked && !a.bias;
   // what takes a row's sums of products to logits in units of ln 2 (finite: a sum of 0 stays 0)
   float per[Tile::NI];
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
     per[ni] = kLog2e;
-    if constexpr (gt_is_split<T>) {
-      const int64_t n = n0 + j0 + 32 * ni;
-      per[ni] = fminf(ldexpf(kLog2e, -(*a.scale + a.rowexp[n < a.n ? n : a.n - 1])), FLT_MAX);
-    }
+    if constexpr (gt_is_split<T>)
+      per[ni] = fminf(ldexpf(kLog2e, -(*a.scale + ex[ni])), FLT_MAX);
   }
+  const bool masked = left_out != 0, plain = !masked && !a.bias;
   if (!plain) {
 #pragma unroll
     for (int mi = 0; mi < Tile::MI; ++mi)

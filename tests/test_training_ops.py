@@ -365,6 +365,22 @@ def test_ce_small_batches_gpu(dtype, n, v, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 3, 4, 8])
+@pytest.mark.parametrize("d,shift", [(101, 0), (100, 0), (100, 4), (102, 2), (96, 3), (520, 1)])
+def test_ce_few_rows_of_any_alignment_gpu(dtype, n, d, shift):
+    v = 2500
+    x = rand((n, d + shift), 1, dtype, "cuda", 0.5)[:, shift:]
+    w = rand((v, d + shift), 2, dtype, "cuda", 0.5)[:, shift:]
+    b = rand((v,), 4, device="cuda")
+    b[1::7] = -INF
+    t = torch.arange(n, device="cuda") * 7 + 3
+    ce_check(x, w, t, None, want=(False, False, False))
+    w[b == -INF] = math.nan
+    ce_check(x, w, t, b, "none")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["rows", "classes", "targets", "weights"])
 def test_ce_large_numbers_left_out_gpu(what):
     """Finite numbers of any size in rows and classes that are left out change nothing else (fp32

@@ -1,8 +1,8 @@
 // Softmax cross entropy of logits z = x W^T + b over V classes, for N rows of D features:
 //   m_n = max_v z_nv,  s_n = sum_v exp(z_nv - m_n),  loss_n = log s_n + (m_n - z_{n, t_n})
 //   dz_nv = g_n (exp(z_nv - m_n) / s_n - [v = t_n]),  dx = dz W,  dW = dz^T x,  db_v = sum_n dz_nv
-// N V logits are never stored.  The forward pass keeps (max, sum of exp) of each row and 256
-// classes; the backward pass goes over the classes in pieces, forms a piece's logits again,
+// N V logits are never stored.  The forward pass keeps (max, sum of exp) of each row and class
+// tile; the backward pass goes over the classes in pieces, forms a piece's logits again,
 // stores its dz in the operand type and multiplies it into dx and dW while it is in cache.
 //
 // Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers: x and a

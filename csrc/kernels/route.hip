@@ -417,8 +417,23 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
       }
     }
     wave_sync();
-    if (live) {
-      // weights: lane l of the token takes slots l, l + L, ...
+    if (live && a.k <= L) {  // weights: a lane per slot, which reads its logit once
+      const int i = lane < a.k ? mysel[lane] : -1;
+      const float zr = i >= 0 ? load_one(row + i) : -INFINITY;
+      float zref = a.sigmoid ? 0.f : zmax;
+      if (a.renormalize) {
+        zref = group_max<L>(zr);
+        if (a.sigmoid) zref = fminf(zref, 0.f);
+      }
+      const float score = i >= 0 ? rel_score(a.sigmoid, zr, zref) : 0.f;
+      const float norm = a.renormalize ? group_sum<L>(score) : a.sigmoid ? 1.f : sum;
+      if (lane < a.k) {
+        a.weights[tok * a.k + lane] = i >= 0 ? score / norm * a.scale : 0.f;
+        a.indices[tok * a.k + lane] = i;
+        if (i >= 0) atomicAdd(&hist[i], 1);
+      }
+    } else if (live) {
+      // lane l of the token takes slots l, l + L, ...
       float zref = -INFINITY, norm = 0.f;
       if (a.renormalize) {
         for (int r = lane; r < a.k; r += L)

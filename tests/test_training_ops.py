@@ -366,6 +366,18 @@ def test_ce_small_batches_gpu(dtype, n, v, d):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(40, 700, 24), (300, 9000, 100), (600, 12_000, 1100)])
+def test_ce_each_gradient_alone_gpu(dtype, n, v, d):
+    x, w = rand((n, d), 1, dtype, "cuda", 0.3), rand((v, d), 2, dtype, "cuda", 0.3)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    b = rand((v,), 4, device="cuda")
+    for want in ((True, False, False), (False, True, False), (False, False, True),
+                 (False, True, True)):
+        ce_check(x, w, t, b, want=want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [1, 3, 4, 8])
 @pytest.mark.parametrize("d,shift", [(101, 0), (100, 0), (100, 4), (102, 2), (96, 3), (520, 1)])
 def test_ce_few_rows_of_any_alignment_gpu(dtype, n, d, shift):

@@ -349,8 +349,9 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
     const int64_t n = n0 + j;
     const float unit = plain ? per[ni] : 1.f;
     const int64_t tg = n < a.n ? a.target[n] - a.class0 - v0 - i0 : -1;
-    // the target's offset where it may be one of this lane's classes, else -1
-    const int tgt = tg >= 0 && tg < Tile::WM ? int(tg) : -1;
+    // the target's offset where it may be one of this lane's classes, else -1 (i0 holds the half
+    // wave's four, so the last of a lane's offsets is also the last within the tile)
+    const int tgt = tg >= 0 && tg <= Tile::row_of(Tile::MI - 1, 15) ? int(tg) : -1;
     if constexpr (!GRAD) {
       float m = -INFINITY;
 #pragma unroll

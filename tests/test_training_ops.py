@@ -990,3 +990,20 @@ def test_second_derivatives_are_refused():
         assert torch.equal(plain, g.detach())
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v,d,copies", [(130, 8, 1), (515, 40, 1), (515, 40, 40), (300, 1100, 50),
+                                        (9000, 100, 1)])
+def test_ce_target_at_every_place_of_a_tile_gpu(dtype, v, d, copies):
+    """Every class is a target: the first and the last of each lane's, of a wave's and of a tile's
+    (also beside a class that is left out)."""
+    x = rand((v * copies, d), 1, dtype, "cuda", 0.5)
+    w = rand((v, d), 2, dtype, "cuda", 0.5)
+    t = torch.arange(v).repeat(copies).cuda()
+    ce_check(x, w, t, None, "sum")
+    b = rand((v,), 4)
+    b[3::4], b[64], b[128 % v] = -INF, -INF, -INF
+    t[b.cuda()[t] == -INF] = -100
+    ce_check(x, w, t, b.cuda())

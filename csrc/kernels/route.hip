@@ -255,7 +255,8 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
     float zmax = -INFINITY;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      z[j] = z[j] == z[j] ? z[j] : -INFINITY;  // a NaN logit is an expert that is left out
+      // a NaN logit is an expert that is left out; -0 + 0 is 0, equal in the keys too
+      z[j] = z[j] == z[j] ? z[j] + 0.f : -INFINITY;
       zmax = fmaxf(zmax, z[j]);
     }
     float sum = 0.f;

@@ -1007,3 +1007,30 @@ def test_ce_target_at_every_place_of_a_tile_gpu(dtype, v, d, copies):
     b[3::4], b[64], b[128 % v] = -INF, -INF, -INF
     t[b.cuda()[t] == -INF] = -100
     ce_check(x, w, t, b.cuda())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_route_signed_zeros(device, dtype):
+    """-0 and +0 are equal: among them the lowest index goes first, on either side of the last
+    choice."""
+    z = rand((40, 48), 1, dtype, device)
+    z[::2] = -z[::2].abs()  # (rows in which the zeros come first)
+    z[:, 1::3] = 0.0
+    z[:, 4::6] = -0.0
+    z[5] = -0.0
+    z[6, ::2], z[6, 1::2] = -0.0, 0.0
+    z[7, ::2], z[7, 1::2] = 0.0, -0.0
+    for score in ("softmax", "sigmoid"):
+        for k in (1, 2, 3, 7):
+            route_check(z, k, score)
+            route_check(z, k, score, renorm=False)
+            route_check(z, k, score, None, 8, 3)
+            route_check(z, k, score, rand((48,), 2, device=device, scale=0.1))
+    for k in (1, 2):  # one +0 (two would be a tie that is looked at again)
+        w, idx, counts = ops.route(torch.tensor([[-0.0, 0.0, -1.0], [-2.0, -0.0, 0.0]], dtype=dtype,
+                                                device=device), k)
+        assert idx.tolist() == [[0, 1][:k], [1, 2][:k]]
+    w, idx, counts = ops.route(torch.tensor([[-0.0, 0.0, -1.0, 0.0]], dtype=dtype, device=device),
+                               2)
+    assert idx.tolist() == [[0, 1]] and counts.tolist() == [1, 1, 0, 0]

@@ -36,6 +36,12 @@ void parallel(int64_t n, const std::function<void(int64_t, int64_t)>& f) {
   pool.parallel_for(n, [&](int, int64_t b, int64_t e) { f(b, e); });
 }
 
+// A logit of the gate as it counts: NaN is an expert that is left out, +inf the largest finite
+// number (its score is the limit's, not inf / inf).
+double gate_logit(float v) {
+  return v == v ? double(std::min(v, std::numeric_limits<float>::max())) : -kInf;
+}
+
 double sigmoid(double z) { return 1.0 / (1.0 + std::exp(-z)); }
 
 }  // namespace
@@ -70,8 +76,7 @@ void route_host(const kern::RouteArgs& a) {
     for (int64_t t = b; t < end; ++t) {
       double zmax = -kInf, sum = 0.0;
       for (int e = 0; e < E; ++e) {
-        const float v = logits[t * a.ld + e];
-        z[e] = v == v ? double(v) : -kInf;
+        z[e] = gate_logit(logits[t * a.ld + e]);
         zmax = std::max(zmax, z[e]);
       }
       for (int e = 0; e < E; ++e) {
@@ -155,16 +160,15 @@ void route_grad_host(const kern::RouteGradArgs& a) {
       if (all) {
         double zmax = -kInf, sum = 0.0;
         for (int e = 0; e < E; ++e) {
-          const float v = logits[t * a.ld + e];
-          if (v > zmax) zmax = v;
+          zmax = std::max(zmax, gate_logit(logits[t * a.ld + e]));
         }
         for (int e = 0; e < E; ++e) {
-          const float v = logits[t * a.ld + e];
-          if (v > -kInf) sum += std::exp(double(v) - zmax);
+          const double v = gate_logit(logits[t * a.ld + e]);
+          if (v > -kInf) sum += std::exp(v - zmax);
         }
         for (int e = 0; e < E; ++e) {
-          const float v = logits[t * a.ld + e];
-          if (v > -kInf) d[e] -= std::exp(double(v) - zmax) / sum * dot;
+          const double v = gate_logit(logits[t * a.ld + e]);
+          if (v > -kInf) d[e] -= std::exp(v - zmax) / sum * dot;
         }
       }
       for (int e = 0; e < E; ++e) out[t * E + e] = float(d[e]);

@@ -19,6 +19,7 @@
 #include "kernels/route.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "runtime/common.h"
@@ -35,6 +36,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 template <typename T>
 __device__ inline float load_one(const T* p) {
   return static_cast<float>(*p);
+}
+// A logit as it counts: NaN is an expert that is left out; +inf the largest finite number (its
+// score is the limit's, not inf / inf); -0 is 0, equal in the keys too.
+__device__ inline float as_logit(float v) {
+  v = v == v ? v : -INFINITY;
+  return fminf(v, FLT_MAX) + 0.f;
 }
 
 // v of lane ^ M in groups of L lanes, or of the lane mirrored in them: either way a reduction of
@@ -117,10 +124,7 @@ __device__ void decide_exactly(const RouteArgs& a, const T* row, int lane, doubl
   const double kout = -INFINITY;
   const int E = a.experts;
   const bool grouped = a.top_groups < a.groups, wide = a.bias || grouped;
-  auto logit = [&](int e) {
-    const float v = load_one(row + e);
-    return v == v ? v : -INFINITY;
-  };
+  auto logit = [&](int e) { return as_logit(load_one(row + e)); };
   if (wide) {
     float zmax = -INFINITY;
     double sum = 0.0;
@@ -255,8 +259,7 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
     float zmax = -INFINITY;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
-      // a NaN logit is an expert that is left out; -0 + 0 is 0, equal in the keys too
-      z[j] = z[j] == z[j] ? z[j] + 0.f : -INFINITY;
+      z[j] = as_logit(z[j]);
       zmax = fmaxf(zmax, z[j]);
     }
     float sum = 0.f;
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
     wave_sync();
     if (live && a.k <= L) {  // weights: a lane per slot, which reads its logit once
       const int i = lane < a.k ? mysel[lane] : -1;
-      const float zr = i >= 0 ? load_one(row + i) : -INFINITY;
+      const float zr = i >= 0 ? as_logit(load_one(row + i)) : -INFINITY;
       float zref = a.sigmoid ? 0.f : zmax;
       if (a.renormalize) {
         zref = group_max<L>(zr);
@@ -438,11 +441,12 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
       float zref = -INFINITY, norm = 0.f;
       if (a.renormalize) {
         for (int r = lane; r < a.k; r += L)
-          if (mysel[r] >= 0) zref = fmaxf(zref, load_one(row + mysel[r]));
+          if (mysel[r] >= 0) zref = fmaxf(zref, as_logit(load_one(row + mysel[r])));
         zref = group_max<L>(zref);
         if (a.sigmoid) zref = fminf(zref, 0.f);
         for (int r = lane; r < a.k; r += L)
-          if (mysel[r] >= 0) norm += rel_score(a.sigmoid, load_one(row + mysel[r]), zref);
+          if (mysel[r] >= 0)
+            norm += rel_score(a.sigmoid, as_logit(load_one(row + mysel[r])), zref);
         norm = group_sum<L>(norm);
       } else {
         zref = a.sigmoid ? 0.f : zmax;
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(kThreads) void oap_route(RouteArgs a, bool vec) {
         const int i = mysel[r];
         float w = 0.f;
         if (i >= 0) {
-          w = rel_score(a.sigmoid, load_one(row + i), zref) / norm * a.scale;
+          w = rel_score(a.sigmoid, as_logit(load_one(row + i)), zref) / norm * a.scale;
           atomicAdd(&hist[i], 1);
         }
         a.weights[tok * a.k + r] = w;
@@ -513,13 +517,12 @@ __global__ __launch_bounds__(kThreads) void oap_route_grad(RouteGradArgs a, int 
         const T* row = z + (t0 + t) * a.ld;
         float m = -INFINITY;
         for (int e = lane; e < E; e += 16) {
-          const float v = load_one(row + e);
-          m = v > m ? v : m;
+          m = fmaxf(m, as_logit(load_one(row + e)));
         }
         m = group_max<16>(m);
         float s = 0.f;
         for (int e = lane; e < E; e += 16) {
-          const float v = load_one(row + e);
+          const float v = as_logit(load_one(row + e));
           s += v > -INFINITY ? expf(v - m) : 0.f;
         }
         s = group_sum<16>(s);
@@ -550,7 +553,7 @@ __global__ __launch_bounds__(kThreads) void oap_route_grad(RouteGradArgs a, int 
     if (all) {
       for (int i = tid; i < nt * E; i += kThreads) {
         const int t = i / E;
-        const float v = load_one(z + (t0 + t) * a.ld + (i - t * E));
+        const float v = as_logit(load_one(z + (t0 + t) * a.ld + (i - t * E)));
         float d = tile[i];
         if (v > -INFINITY) d -= expf(v - zmax[t]) / rsum[t] * dense[t];
         out[i] = static_cast<T>(d);

@@ -314,8 +314,9 @@ def route(logits, k: int, *, score: str = "softmax", bias=None, groups: int = 1,
     scores if ``renormalize``, times ``scale``.
 
     An expert whose logit is ``-inf`` or NaN, or whose bias is ``-inf`` or NaN, is left out; where
-    fewer than ``k`` are left the last slots hold index -1 and weight 0.  At most 1024 experts,
-    32 choices, 64 groups and 2^31 - 1 tokens.  The gradient goes from ``weights`` to ``logits``.
+    fewer than ``k`` are left the last slots hold index -1 and weight 0.  A logit of ``+inf`` counts
+    as the largest finite float32 number.  At most 1024 experts, 32 choices, 64 groups and 2^31 - 1
+    tokens.  The gradient goes from ``weights`` to ``logits``.
     """
     _float_tensor("logits", logits, 2)
     native = _loader.load()

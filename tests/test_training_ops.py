@@ -1034,3 +1034,36 @@ def test_route_signed_zeros(device, dtype):
     w, idx, counts = ops.route(torch.tensor([[-0.0, 0.0, -1.0, 0.0]], dtype=dtype, device=device),
                                2)
     assert idx.tolist() == [[0, 1]] and counts.tolist() == [1, 1, 0, 0]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_route_infinite_logits(device, dtype):
+    """A logit of +inf counts as the largest finite fp32 number: it is chosen, whatever the score,
+    the bias and the groups, and its token's weights are numbers."""
+    z = rand((12, 40), 1, dtype, device)
+    z[0, 7] = INF
+    z[1, 30], z[1, 3] = INF, INF
+    z[2] = INF
+    z[3, 5], z[3, 6], z[3, 7] = INF, math.nan, -INF
+    z[4, 11], z[4, 12] = INF, torch.finfo(dtype).max
+    capped = z.float().clamp(max=torch.finfo(torch.float32).max)
+    bias = rand((40,), 2, device=device, scale=0.1)
+    g = rand((12, 4), 3, device=device)
+    for score in ("softmax", "sigmoid"):
+        for b, groups, top in ((None, 1, 1), (bias, 1, 1), (None, 8, 3), (bias, 8, 3)):
+            for renorm in (True, False):
+                got = []
+                for logits in (z, capped):
+                    leaf = logits.clone().requires_grad_()
+                    out = ops.route(leaf, 4, score=score, bias=b, groups=groups, top_groups=top,
+                                    renormalize=renorm)
+                    got.append((*out, torch.autograd.grad(out[0], leaf, g)[0]))
+                (w, i, c, d), (rw, ri, rc, rd) = got
+                assert torch.equal(i, ri) and torch.equal(c, rc) and torch.equal(w, rw)
+                assert torch.equal(d, rd.to(dtype))
+                assert w.isfinite().all() and d.isfinite().all()
+                assert (i[:, 0] >= 0).all()
+                if b is None:
+                    assert i[0, 0] == 7 and i[1, :2].tolist() == [3, 30]
+                    assert i[2].tolist() == [0, 1, 2, 3] and i[4, 0] == 11

@@ -744,7 +744,8 @@ __global__ __launch_bounds__(1024) void oap_ce_total(RowArgs a) {
 
 // Upstream gradient of every row as g_n = gscale * coef_n with |coef_n| <= 1: products of the
 // coefficient with a probability then fit 16 bits.  Rows without a loss (or with a target that
-// is no class) get the coefficient 0.
+// is no class) get the coefficient 0.  gscale is the largest magnitude that is a number, and a
+// row's gradient that is none is its coefficient: it reaches that row's dx, and no other's.
 struct CoefArgs {
   const float* grad;  // null: nothing to do
   int per_row, mean;
@@ -762,9 +763,9 @@ __device__ inline void coefficients(const CoefArgs& a) {
   for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
     const int64_t t = a.target[i];
     k += t != a.ignore;
-    if (a.per_row && t >= 0 && t < a.classes && t != a.ignore) {
-      const float g = fabsf(a.grad[i]);
-      m = g <= m ? m : g;  // (a NaN is kept)
+    if (t >= 0 && t < a.classes && t != a.ignore) {
+      const float g = a.per_row ? fabsf(a.grad[i]) : 1.f;
+      m = g > m && g < INFINITY ? g : m;
     }
   }
   red[threadIdx.x] = m;
@@ -772,20 +773,25 @@ __device__ inline void coefficients(const CoefArgs& a) {
   for (int h = 512; h >= 1; h >>= 1) {
     __syncthreads();
     if (threadIdx.x < unsigned(h)) {
-      const float o = red[threadIdx.x + h];
-      red[threadIdx.x] = o <= red[threadIdx.x] ? red[threadIdx.x] : o;
+      red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + h]);
       cnt[threadIdx.x] += cnt[threadIdx.x + h];
     }
   }
   __syncthreads();
   const float top = red[0];
-  if (threadIdx.x == 0)
-    *a.gscale =
-        a.per_row ? top : a.mean ? a.grad[0] / float(cnt[0] ? cnt[0] : 1) : a.grad[0];
+  if (threadIdx.x == 0)  // (0 if no row has a loss)
+    *a.gscale = a.per_row || top == 0.f
+                    ? top
+                    : a.mean ? a.grad[0] / float(cnt[0] ? cnt[0] : 1) : a.grad[0];
   for (int64_t i = threadIdx.x; i < a.n; i += 1024) {
     const int64_t t = a.target[i];
     const bool has = t >= 0 && t < a.classes && t != a.ignore;
-    a.coef[i] = !has ? 0.f : a.per_row ? (top == 0.f ? 0.f : a.grad[i] / top) : 1.f;
+    float c = has ? 1.f : 0.f;
+    if (has && a.per_row) {
+      const float g = a.grad[i];
+      c = !(fabsf(g) < INFINITY) ? g : top == 0.f ? 0.f : g / top;
+    }
+    a.coef[i] = c;
   }
 }
 
@@ -919,6 +925,8 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(B, B)) void oap_ce_grads(P
 template <typename T>
 struct FinishArgs {
   const float* gscale;
+  const float* coef;
+  const float* bias;    // of the piece, or null
   const float* dbpart;  // [row tile][vp], or null
   int rtiles;
   int64_t vp, classes;
@@ -926,6 +934,7 @@ struct FinishArgs {
   const float* slab;  // [split][count], or null
   int splits;
   int64_t count;
+  int dim;
   float unscale;
   T* dx;
 };
@@ -939,14 +948,19 @@ __global__ __launch_bounds__(256) void oap_ce_finish(FinishArgs<T> a) {
     if (v >= a.classes) return;
     float s = 0.f;
     for (int t = 0; t < a.rtiles; ++t) s += a.dbpart[int64_t(t) * a.vp + v];
-    a.db[v] = s * g;
+    // (a class that is left out has no gradient, whatever the rows' upstream gradients are)
+    a.db[v] = a.bias && a.bias[v] == -INFINITY ? 0.f : s * g;
     return;
   }
+  const float scale = g * a.unscale;
   for (int64_t i = int64_t(blockIdx.x - dbblocks) * 256 + threadIdx.x; i < a.count;
        i += int64_t(gridDim.x - dbblocks) * 256) {
     float v = 0.f;
     for (int s = 0; s < a.splits; ++s) v += a.slab[int64_t(s) * a.count + i];
-    a.dx[i] = static_cast<T>(v * (g * a.unscale));
+    v *= scale;
+    // an upstream gradient that is no number leaves the rows without a loss at 0
+    if (!(fabsf(scale) < INFINITY) && a.coef[i / a.dim] == 0.f) v = 0.f;
+    a.dx[i] = static_cast<T>(v);
   }
 }
 
@@ -1446,6 +1460,8 @@ struct Ce {
       products(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
       FinishArgs<S> f = {};
       f.gscale = w.gscale;
+      f.coef = w.coef;
+      f.bias = bias;
       int64_t blocks = 0;
       if (db) {
         f.dbpart = w.dbpart;
@@ -1459,6 +1475,7 @@ struct Ce {
         f.slab = w.slab;
         f.splits = p.splits;
         f.count = a.n * a.dim;
+        f.dim = a.dim;
         f.unscale = 1.f / pscale;
         f.dx = static_cast<S*>(dx);
         blocks += stride_grid(f.count);

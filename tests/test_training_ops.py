@@ -1067,3 +1067,46 @@ def test_route_infinite_logits(device, dtype):
                 if b is None:
                     assert i[0, 0] == 7 and i[1, :2].tolist() == [3, 30]
                     assert i[2].tolist() == [0, 1, 2, 3] and i[4, 0] == 11
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, INF, -INF])
+def test_ce_upstream_gradients_that_are_no_numbers(device, dtype, bad):
+    """An upstream gradient that is infinite or NaN reaches its own row's gradient of x only; rows
+    and classes that are left out keep the gradient 0."""
+    sizes = [(9, 30, 16), (70, 300, 64)]
+    if device == "cuda":
+        sizes += [(300, 9000, 100), (300, 50_000, 128), (520, 9000, 1100)]
+    for n, v, d in sizes:
+        x = rand((n, d), 1, dtype, device, 0.3).requires_grad_()
+        w = rand((v, d), 2, dtype, device, 0.3).requires_grad_()
+        b = rand((v,), 3, device=device)
+        b[4::5] = -INF
+        b.requires_grad_()
+        t = (torch.arange(n, device=device) * 5 + 1) % v // 5 * 5
+        t[2::7] = -100
+        up = torch.rand(n, generator=torch.Generator().manual_seed(4)).to(device) + 0.5
+        up[0] = 2.0  # (the largest that is a number)
+        worse = up.clone()
+        worse[3], worse[n - 1] = bad, bad
+        assert t[3] >= 0 and t[n - 1] >= 0
+        up[3], up[n - 1] = 0.0, 0.0
+        rows = ops.softmax_cross_entropy(x, w, t, b, reduction="none")
+        want, = torch.autograd.grad(rows, [x], up, retain_graph=True)
+        dx, dw, db = torch.autograd.grad(rows, [x, w, b], worse)
+        others = torch.ones(n, dtype=torch.bool, device=device)
+        others[3], others[n - 1] = False, False
+        assert torch.equal(dx[others], want[others]), (n, v, d)
+        assert not dx[~others].isfinite().any()
+        out = b == -INF
+        assert not dw[out].any() and not db[out].any()
+        assert not dw[~out].isfinite().any() and not db[~out].isfinite().any()
+        # one number for all rows
+        loss = ops.softmax_cross_entropy(x, w, t, b)
+        dx, dw, db = torch.autograd.grad(loss, [x, w, b], torch.tensor(bad, device=device))
+        assert not dx[t == -100].any() and not dx[t >= 0].isfinite().any()
+        assert not dw[out].any() and not db[out].any()
+        loss = ops.softmax_cross_entropy(x, w, torch.full_like(t, -100), b)
+        for g in torch.autograd.grad(loss, [x, w, b], torch.tensor(bad, device=device)):
+            assert not g.any()

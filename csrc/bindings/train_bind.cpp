@@ -182,6 +182,14 @@ void register_train(py::module_& m) {
               ce_args(elem, x, ldx, w, ldw, bias, 0, 0, n, classes, dim), want_dx, want_dw,
               want_db);
         });
+  // (rows of a turn, classes of a piece, fp32 operands split): how a call is divided
+  m.def("softmax_ce_plan",
+        [](const std::string& elem, uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw,
+           uintptr_t bias, int64_t n, int64_t classes, int64_t dim, bool grad) {
+          const kern::CePlan p =
+              kern::ce_plan(ce_args(elem, x, ldx, w, ldw, bias, 0, 0, n, classes, dim), grad);
+          return py::make_tuple(p.rows, p.classes, p.split);
+        });
   m.def("softmax_ce_forward",
         [](int device, uintptr_t stream, const std::string& elem, uintptr_t x, int64_t ldx,
            uintptr_t w, int64_t ldw, uintptr_t bias, uintptr_t target, int64_t ignore, int64_t n,

@@ -40,5 +40,13 @@ size_t ce_backward_bytes(const CeArgs& a, bool want_dx, bool want_dw, bool want_
 void ce_backward(const CeArgs& a, const float2* stat, const float* grad, bool per_row, bool mean,
                  void* dx, void* dw, float* db, void* work, hipStream_t s);
 
+// How a call is divided: rows of a turn of the forward pass, classes of a piece (of the pass that
+// `grad` names), and whether fp32 operands are split in two fp16 numbers
+struct CePlan {
+  int64_t rows, classes;
+  bool split;
+};
+CePlan ce_plan(const CeArgs& a, bool grad);
+
 }  // namespace kern
 }  // namespace oap

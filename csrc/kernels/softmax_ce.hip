@@ -1523,6 +1523,12 @@ void ce_dispatch(const CeArgs& a, F&& f) {
 
 }  // namespace
 
+CePlan ce_plan(const CeArgs& a, bool grad) {
+  check(a);
+  const Plan p = make_plan(a, grad);
+  return {p.rows, p.piece, p.split};
+}
+
 size_t ce_forward_bytes(const CeArgs& a) {
   check(a);
   if (a.n == 0) return 0;

@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from oap_mllib_amd import ops
+from oap_mllib_amd import _loader, ops
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -1110,3 +1110,100 @@ def test_ce_upstream_gradients_that_are_no_numbers(device, dtype, bad):
         loss = ops.softmax_cross_entropy(x, w, torch.full_like(t, -100), b)
         for g in torch.autograd.grad(loss, [x, w, b], torch.tensor(bad, device=device)):
             assert not g.any()
+
+
+def ce_plan(x, w, b, grad):
+    """(rows of a turn, classes of a piece, fp32 operands split) of a call"""
+    elem = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}[x.dtype]
+    return _loader.load().softmax_ce_plan(elem, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
+                                          0 if b is None else b.data_ptr(), *x.shape[:1],
+                                          *w.shape, grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,n,v,d,split", [(torch.bfloat16, 8190, 140_001, 64, False),
+                                               (torch.float16, 8000, 131_100, 24, False),
+                                               (torch.float32, 2000, 300_001, 16, True),
+                                               (torch.float32, 100, 1_100_003, 8, False)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_ce_several_pieces_gpu(dtype, n, v, d, split, bias):
+    """Classes in several pieces, weights, targets and left-out classes in each, and the weights'
+    magnitudes different from piece to piece."""
+    x = rand((n, d), 1, dtype, "cuda", 0.5)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    w = rand((v, d), 2, torch.float32, "cuda", 1 / math.sqrt(d)) + 0.25 / math.sqrt(d)
+    b = None
+    if bias:
+        b = rand((v,), 4, device="cuda")
+        b[5::11] = -INF
+        b[t] = 0.25
+    t[::9] = -100
+    plan = ce_plan(x, w.to(dtype), b, True)
+    pieces = range(0, v, plan[1])
+    assert len(pieces) > 1 and plan[2] == split
+    for i, c in enumerate(pieces):
+        w[c:c + plan[1]] *= (1.0, 0.0625, 4.0)[i % 3]
+        assert ((t >= c) & (t < c + plan[1])).any()
+    w = w.to(dtype)
+    leaves = [q.requires_grad_() for q in (x, w, b) if q is not None]
+    loss = ops.softmax_cross_entropy(x, w, t, b, reduction="sum")
+    grads = torch.autograd.grad(loss, leaves)
+    with torch.no_grad():
+        kept = torch.nonzero(t >= 0)[:, 0]
+        xd, wd = x.double()[kept], w.double()
+        z = xd @ wd.t()
+        if bias:
+            z += b.double()
+        hot = t[kept][:, None]
+        lse = torch.logsumexp(z, 1)
+        ref = (lse - z.gather(1, hot)[:, 0]).sum()
+        zerr = (d + 8) * E32 * (xd.norm(dim=1).max() * wd.norm(dim=1).max()).item() + \
+            4 * E32 * lse.abs().max().item()
+        assert abs(loss.double() - ref) <= n * 2 * zerr + 4 * E32 * ref.abs()
+        p = z.sub_(lse[:, None]).exp_()
+        one = torch.ones_like(hot, dtype=torch.float64)
+        mags = [p.scatter_add(1, hot, one)]
+        p.scatter_add_(1, hot, -one)
+        wants = [torch.zeros(n, d, device="cuda").double().index_copy(0, kept, p @ wd),
+                 p.t() @ xd, p.sum(0)]
+        mags = [torch.zeros(n, d, device="cuda").double().index_copy(0, kept, mags[0] @ wd.abs()),
+                mags[0].t() @ xd.abs(), mags[0].sum(0)]
+        u = half_step(dtype)
+        # dx: a run of at most 8192 classes, 16 of them (2 in fp32, with as many fewer classes) a
+        # step, and the runs' and pieces' sums: below 1024 steps of two roundings
+        for name, got, want, mag, steps in zip(("dx", "dw", "db"), grads, wants, mags,
+                                               (2048, n + 8, n + 8)):
+            uo = u if name != "db" else 0
+            rel = 2 * zerr + 16 * E32 + uo + steps * E32
+            # fp16: dz keeps 2^-39; results keep half of 2^-24
+            tiny = 2.0 ** -25 + 2.0 ** -39 * {"dx": v, "dw": n, "db": 0}[name] * 4 \
+                if dtype == torch.float16 and name != "db" else 1e-37
+            err = (got.double() - want).abs() - (mag * (rel + uo) + uo * want.abs() + tiny)
+            assert not (err > 0).any(), (name, err.max())
+
+
+@pytest.mark.gpu
+def test_ce_rows_in_several_turns_gpu():
+    """More rows than one turn of the forward pass keeps statistics for: a row's loss is that of a
+    call on its own part of the rows, but for the order in which 7813 tiles' sums are joined (up to
+    489 joins in a row by a thread, 4 to 10 levels above them, three roundings each)."""
+    n, v, d = 20_000, 2_000_000, 4
+    x, w = rand((n, d), 1, torch.bfloat16, "cuda"), rand((v, d), 2, torch.bfloat16, "cuda")
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    t[::7] = -100
+    assert ce_plan(x, w, None, False)[0] < n <= 2 * ce_plan(x, w, None, False)[0]
+    whole = ops.softmax_cross_entropy(x, w, t, reduction="none")
+    parts = torch.cat([ops.softmax_cross_entropy(x[a:a + 5000], w, t[a:a + 5000], reduction="none")
+                       for a in range(0, n, 5000)])
+    assert ((whole - parts).abs() <= 2 * 499 * 3 * E32 + 4 * E32 * parts.abs()).all()
+    mean = ops.softmax_cross_entropy(x, w, t)
+    ref = whole.double().sum() / (t != -100).sum()
+    assert abs(mean.item() - ref.item()) <= E32 * abs(ref.item())
+    # some rows against 64 bits, on both sides of the border
+    turn = ce_plan(x, w, None, False)[0]
+    some = torch.tensor([1, 2, turn - 1, turn, turn + 1, n - 1], device="cuda")
+    z = x[some].double() @ w.double().t()
+    ref = torch.logsumexp(z, 1) - z.gather(1, t[some].clamp(min=0)[:, None])[:, 0]
+    ref[t[some] == -100] = 0
+    zerr = (d + 8) * E32 * (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
+    assert ((whole[some] - ref).abs() <= 2 * zerr + 499 * 3 * E32 + 4 * E32 * (ref.abs() + 20)).all()

@@ -193,14 +193,14 @@ void register_train(py::module_& m) {
   m.def("softmax_ce_forward",
         [](int device, uintptr_t stream, const std::string& elem, uintptr_t x, int64_t ldx,
            uintptr_t w, int64_t ldw, uintptr_t bias, uintptr_t target, int64_t ignore, int64_t n,
-           int64_t classes, int64_t dim, uintptr_t loss, uintptr_t stat, uintptr_t total,
-           bool mean, uintptr_t work) {
+           int64_t classes, int64_t dim, uintptr_t loss, uintptr_t stat, uintptr_t miss,
+           uintptr_t total, bool mean, uintptr_t work) {
           const kern::CeArgs a =
               ce_args(elem, x, ldx, w, ldw, bias, target, ignore, n, classes, dim);
           on(device, stream, a.elem,
              [&](hipStream_t s) {
-               kern::ce_forward(a, at<float>(loss), at<float2>(stat), at<float>(total), mean,
-                                at<void>(work), s);
+               kern::ce_forward(a, at<float>(loss), at<float2>(stat), at<float>(miss),
+                                at<float>(total), mean, at<void>(work), s);
              },
              [&] {
                ce_forward_host(a, at<float>(loss), at<float2>(stat), at<float>(total), mean);
@@ -209,14 +209,15 @@ void register_train(py::module_& m) {
   m.def("softmax_ce_backward",
         [](int device, uintptr_t stream, const std::string& elem, uintptr_t x, int64_t ldx,
            uintptr_t w, int64_t ldw, uintptr_t bias, uintptr_t target, int64_t ignore, int64_t n,
-           int64_t classes, int64_t dim, uintptr_t stat, uintptr_t grad, bool per_row, bool mean,
-           uintptr_t dx, uintptr_t dw, uintptr_t db, uintptr_t work) {
+           int64_t classes, int64_t dim, uintptr_t stat, uintptr_t miss, uintptr_t grad,
+           bool per_row, bool mean, uintptr_t dx, uintptr_t dw, uintptr_t db, uintptr_t work) {
           const kern::CeArgs a =
               ce_args(elem, x, ldx, w, ldw, bias, target, ignore, n, classes, dim);
           on(device, stream, a.elem,
              [&](hipStream_t s) {
-               kern::ce_backward(a, at<const float2>(stat), at<const float>(grad), per_row, mean,
-                                 at<void>(dx), at<void>(dw), at<float>(db), at<void>(work), s);
+               kern::ce_backward(a, at<const float2>(stat), at<const float>(miss),
+                                 at<const float>(grad), per_row, mean, at<void>(dx), at<void>(dw),
+                                 at<float>(db), at<void>(work), s);
              },
              [&] {
                ce_backward_host(a, at<const float2>(stat), at<const float>(grad), per_row, mean,

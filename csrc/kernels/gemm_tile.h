@@ -24,6 +24,10 @@
 // largest keep an absolute error of 2^-40 of that.  Three 16-bit MFMAs take a fifth of the time
 // of the fp32 ones.  A row lies as runs of 32 numbers, their 32 h and then their 32 l, so 128
 // bytes of a row hold 32 k in either order of k.
+//
+// The A operand may lie in fp32 instead (RAW) and is split on its way to LDS, at a power of two of
+// its own for each row of the result: a row then keeps 22 bits of its numbers, or 2^-40 of its
+// largest, whatever the others hold, and the scale needs to be known only when the tile is read.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -35,6 +39,7 @@ namespace kern {
 
 typedef __bf16 gt_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 gt_f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 gt_f16x4 __attribute__((ext_vector_type(4)));
 typedef short gt_s16x4 __attribute__((ext_vector_type(4)));
 typedef short gt_s16x8 __attribute__((ext_vector_type(8)));
 typedef float gt_f32x4 __attribute__((ext_vector_type(4)));
@@ -117,12 +122,13 @@ struct GtOperand {
   const void* p;
   int64_t ld;
   int64_t rows, cols;
+  const float* scale;  // RAW: the power of two of each row (kAlongK) or column (kAcrossK)
 };
 
 enum GtOrder { kAlongK, kAcrossK };
 
 // One operand of R rows of a tile
-template <typename T, int R, GtOrder ORDER>
+template <typename T, int R, GtOrder ORDER, bool RAW = false>
 struct GtSide {
   static constexpr int BK = gt_block<T>(), CH = gt_chunk<T>();
   static constexpr int kBytes = R * 128;                // of a staged block
@@ -134,8 +140,10 @@ struct GtSide {
   static constexpr bool kTransposed = ORDER == kAcrossK && (sizeof(T) == 2 || kSplit);
   // LDS reads of a fragment
   static constexpr int kReads = (ORDER == kAlongK ? 1 : kTransposed ? 2 : 4) * (kSplit ? 2 : 1);
+  static constexpr int kWrites = (RAW ? 2 : 1) * kLoads;  // LDS writes of a thread
   typedef typename GtFrag<T>::type Frag;
   static_assert(kLoads >= 1, "a thread stages at least 16 bytes of each operand");
+  static_assert(!RAW || kSplit, "only split operands are made from fp32");
 
   // xor on the chunk index of k row r
   __device__ static int swizzle(int r) {
@@ -151,6 +159,8 @@ struct GtSide {
     int left;          // k from the block's first to the end of the operand or the range
     int sub;           // the thread's place in k within a block: its chunk's first k, or row
     uint32_t lds;      // byte in the staged block
+    // RAW: of the thread's rows (kAlongK) or its four columns
+    float mul[RAW ? (ORDER == kAlongK ? kLoads : 4) : 1];
 
     __device__ void init(const GtOperand& o, int64_t r0, int64_t k0, int64_t k1) {
       const int t = threadIdx.x;
@@ -163,10 +173,13 @@ struct GtSide {
         for (int i = 0; i < kLoads; ++i) {
           const int q = r + i * kStep;
           off[i] = uint32_t(q < last ? q : last) * ldb + chunk * 16;
+          if constexpr (RAW) mul[i] = o.scale[r0 + (q < last ? q : last)];
         }
         left = int((k1 < o.cols ? k1 : o.cols) - k0);
-        sub = kSplit ? 0 : chunk * CH;
-        lds = r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
+        sub = kSplit && !RAW ? 0 : chunk * CH;
+        // (RAW: four numbers, whose h are half a chunk, and their l four chunks on)
+        lds = RAW ? r * 128 + (((chunk >> 1) ^ ((r >> 1) & 7)) << 4) + (chunk & 1) * 8
+                  : r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4);
       } else {
         const int k = t / kChunks, chunk = t % kChunks;
         base = static_cast<const char*>(o.p) + k0 * o.ld * sizeof(T) + r0 * sizeof(T);
@@ -177,7 +190,12 @@ struct GtSide {
           off[i] = uint32_t(k + i * kStep) * ldb + uint32_t((c < last ? c : last) * sizeof(T));
         left = int((k1 < o.rows ? k1 : o.rows) - k0);
         sub = k;
-        lds = k * kRowBytes + ((chunk ^ swizzle(k)) << 4);
+        const int at = RAW ? (chunk & ~7) + ((chunk & 7) >> 1) : chunk;
+        lds = k * kRowBytes + ((at ^ swizzle(k)) << 4) + (RAW ? (chunk & 1) * 8 : 0);
+        if constexpr (RAW) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mul[j] = o.scale[r0 + (c < last ? c : last) + j];
+        }
       }
     }
     // loads the block and steps to the next.  Buffer loads: an offset beyond the resource reads
@@ -197,9 +215,23 @@ struct GtSide {
     }
     __device__ void store(char* block, const gt_u32x4 (&v)[kLoads]) const {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i)
-        *reinterpret_cast<gt_u32x4*>(block + lds +
-                                     i * kStep * (ORDER == kAlongK ? 128 : kRowBytes)) = v[i];
+      for (int i = 0; i < kLoads; ++i) {
+        constexpr int kRow = ORDER == kAlongK ? 128 : kRowBytes;
+        if constexpr (RAW) {
+          const gt_f32x4 f = __builtin_bit_cast(gt_f32x4, v[i]);
+          gt_f16x4 h, l;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = f[j] * mul[ORDER == kAlongK ? i : j];
+            h[j] = static_cast<_Float16>(x);
+            l[j] = static_cast<_Float16>(x - static_cast<float>(h[j]));
+          }
+          *reinterpret_cast<gt_f16x4*>(block + lds + i * kStep * kRow) = h;
+          *reinterpret_cast<gt_f16x4*>(block + (lds ^ 64) + i * kStep * kRow) = l;
+        } else {
+          *reinterpret_cast<gt_u32x4*>(block + lds + i * kStep * kRow) = v[i];
+        }
+      }
     }
   };
 
@@ -275,13 +307,14 @@ struct GtSide {
 //
 // SINGLE: one LDS buffer and two barriers a block.  Half the LDS lets a third workgroup share the
 // CU, which hides more than the second buffer does while k is short.
-template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M_, bool SINGLE = false>
+template <typename T, int BM_, GtOrder OA, int BN_, GtOrder OB, int WAVES_M_, bool SINGLE = false,
+          bool RAW_A = false>
 struct GtTile {
   static constexpr int BM = BM_, BN = BN_;
   static constexpr int WAVES_M = WAVES_M_, WAVES_N = 4 / WAVES_M;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;
   static constexpr int MI = WM / 32, NI = WN / 32;
-  typedef GtSide<T, BM, OA> SideA;
+  typedef GtSide<T, BM, OA, RAW_A> SideA;
   typedef GtSide<T, BN, OB> SideB;
   static constexpr int BK = SideA::BK;
   static constexpr int kBuf = SideA::kBytes + SideB::kBytes;
@@ -300,6 +333,7 @@ struct GtTile {
     constexpr int kMfmas = MI * NI * gt_mfmas<T>;
     constexpr int kReads = SideA::kReads * MI + SideB::kReads * NI;
     constexpr int kMoves = SideA::kLoads + SideB::kLoads;
+    constexpr int kWrites = SideA::kWrites + SideB::kWrites;
     constexpr int G = kMfmas < 8 ? kMfmas : 8;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -308,7 +342,7 @@ struct GtTile {
       if (!STORES || g < G / 2) __builtin_amdgcn_sched_group_barrier(0x100, kR, 0);
       if (LOADS) __builtin_amdgcn_sched_group_barrier(0x020, (kMoves + G - 1) / G, 0);
       if (STORES && g >= G / 2)
-        __builtin_amdgcn_sched_group_barrier(0x200, (2 * kMoves + G - 1) / G, 0);
+        __builtin_amdgcn_sched_group_barrier(0x200, (2 * kWrites + G - 1) / G, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, kMfmas / G, 0);
     }
     __builtin_amdgcn_sched_barrier(0);

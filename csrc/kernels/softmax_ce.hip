@@ -5,12 +5,14 @@
 // tile; the backward pass goes over the classes in pieces, forms a piece's logits again,
 // stores its dz in the operand type and multiplies it into dx and dW while it is in cache.
 //
-// Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers: x and a
-// piece's classes are then copied into split images at powers of two, and dz, at most 1 in
-// magnitude, is stored split at the scale 2^14.  A product keeps 22 bits; |dz| below 2^-24 keeps an
-// absolute 2^-39.  Every row of x has a scale of its own in the logits (a row is right whatever the
-// others hold), a piece's classes have one, and so have the rows in dW: there a number keeps an
-// absolute 2^-40 of the largest that takes part in the same sums.
+// Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers.  A product
+// then keeps 22 bits of each: x and a piece's classes are copied into split images at powers of
+// two, every row of x at its own in the logits (a row is right whatever the others hold), a
+// piece's classes at one, and so the rows in dW: a number keeps an absolute 2^-40 of the largest
+// there.  dz is stored in fp32 and split as a tile of it is read, at a power of two per row for dx
+// (its largest magnitude is known, 1 - p of the target) and per class for dW (from maxima that the
+// logits' epilogue keeps): a probability of 2^-60 has its 22 bits where all of its sum are as
+// small.  At one scale for all, probabilities below 2^-24 lost bits and those below 2^-39 all.
 //
 // Roundings: sums, statistics, losses and dx's slabs are fp32, and a result is rounded once.  With
 // 16-bit operands dz is rounded to their type (at most 2^-8 of it in bf16, 2^-11 in fp16) before
@@ -59,6 +61,21 @@ __device__ inline float half_wave_sum(float v) {
   const auto p = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false,
                                                   false);
   return __int_as_float(p[0]) + __int_as_float(p[1]);
+}
+
+template <int CTRL>
+__device__ inline float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf,
+                                                             true)));
+}
+__device__ inline float half_wave_max(float v) {
+  v = dpp_max<0xB1>(v);
+  v = dpp_max<0x4E>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false,
+                                                  false);
+  return fmaxf(__int_as_float(p[0]), __int_as_float(p[1]));
 }
 
 // ------------------------------------------------------------------------------ operand images
@@ -110,7 +127,7 @@ __device__ inline bool left_out_row(const PackArgs<T>& a, int64_t row) {
 constexpr int kMaxBlocks = 512;  // workgroups (and partial maxima) of an operand
 
 __device__ inline int scale_exponent(float top) {
-  if (!(top > 0.f)) return 0;
+  if (!(top > 0.f && top < INFINITY)) return 0;
   int e;
   frexpf(top, &e);  // top = f 2^e, f in [0.5, 1)
   return min(max(15 - e, -126), 126);
@@ -246,6 +263,7 @@ struct LogitArgs {
   void* dz;            // [npad][vp]
   int64_t vp;
   float* dbpart;       // [row tile][vp] sums of dz over the tile's rows, or null
+  float* dzmax;        // [row tile][vp] largest |dz| of the tile's rows, or null (split operands)
 };
 
 // Tile of a workgroup: workgroups go to the 8 XCDs in turn, so each XCD takes a run of
@@ -272,7 +290,7 @@ struct Store {
 };
 template <>
 struct Store<GtSplit> {
-  typedef _Float16 type;
+  typedef float type;
 };
 
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
@@ -392,8 +410,13 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          acc[mi][ni][e] = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref)) * cs;
+        for (int e = 0; e < 16; ++e) {
+          float p = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref));
+          // (at most 1, also where huge logits round otherwise than in the forward pass: the
+          // split's scale relies on it)
+          if constexpr (gt_is_split<T>) p = __builtin_amdgcn_fmed3f(p, 0.f, 1.f);
+          acc[mi][ni][e] = p * cs;
+        }
       if (__ballot(tgt >= 0)) {
         const int hit = tgt >= 0 && sbias[i0 + tgt] == -INFINITY ? -1 : tgt;
 #pragma unroll
@@ -436,6 +459,28 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
         a.dbpart[int64_t(nt) * a.vp + v0 + i] = v * a.unscale;
       }
     }
+    if constexpr (gt_is_split<T>) {
+      if (a.dzmax) {
+        float* smx = reinterpret_cast<float*>(lds);  // [wave column][BM]
+        if (a.dbpart) __syncthreads();
+#pragma unroll
+        for (int mi = 0; mi < Tile::MI; ++mi)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float v = 0.f;
+#pragma unroll
+            for (int ni = 0; ni < Tile::NI; ++ni) v = fmaxf(v, fabsf(acc[mi][ni][e]));
+            v = half_wave_max(v);
+            if ((lane & 31) == 0) smx[Tile::wave_n() * BM + i0 + Tile::row_of(mi, e)] = v;
+          }
+        __syncthreads();
+        for (int i = tid; i < BM; i += kGtThreads) {
+          float v = 0.f;
+          for (int k = 0; k < Tile::WAVES_N; ++k) v = fmaxf(v, smx[k * BM + i]);
+          a.dzmax[int64_t(nt) * a.vp + v0 + i] = v;
+        }
+      }
+    }
     // dz through LDS, [row][BM classes], the 16-byte chunk c of row j at slot c ^ (j & SW), then
     // out in whole rows; in parts of 32 rows of every wave where the tile is larger than LDS
     constexpr int CPR = BM * int(sizeof(T)) / 16, ROW = BM * int(sizeof(T));
@@ -444,7 +489,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
     constexpr int PARTS = kWhole ? 1 : Tile::NI, NP = Tile::NI / PARTS;  // blocks of a part
     constexpr int PW = Tile::WN / PARTS, PR = BN / PARTS;                // rows of it
     static_assert(PR * ROW <= Tile::kLds, "a part of the dz tile fits the staging buffer");
-    typedef typename Store<T>::type H;  // what is stored: T, or the two halves of a split number
+    typedef typename Store<T>::type H;  // what is stored: T, or fp32 for split operands
     struct alignas(4 * sizeof(H)) Four {
       H v[4];
     };
@@ -469,22 +514,9 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
             const int j = Tile::wave_n() * PW + 32 * np + (lane & 31);
             const int i = i0 + Tile::row_of(mi, 4 * g);
             Four f;
-            if constexpr (gt_is_split<T>) {
-              Four l;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float v = acc[mi][ni][4 * g + e];
-                f.v[e] = static_cast<H>(v);
-                l.v[e] = static_cast<H>(v - static_cast<float>(f.v[e]));
-              }
-              const int byte = (i >> 5) * 128 + (i & 31) * 2;
-              *at(j, byte) = f;
-              *at(j, byte + 64) = l;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e]);
-              *at(j, i * int(sizeof(T))) = f;
-            }
+            for (int e = 0; e < 4; ++e) f.v[e] = static_cast<H>(acc[mi][ni][4 * g + e]);
+            *at(j, i * int(sizeof(T))) = f;
           }
       __syncthreads();
 #pragma unroll
@@ -660,6 +692,7 @@ struct RowArgs {
   const float* zt;
   float* loss;
   float2* stat;
+  float* miss;   // 1 - probability of the target, or null
   float* total;  // null: none, or in a launch of its own
   int mean;
 };
@@ -721,6 +754,7 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(RowArgs a) {
       else
         l = a.zt[row] == -INFINITY ? INFINITY : kLn2 * (log2f(s) + (m - a.zt[row]));
       a.loss[row] = l;
+      if (a.miss) a.miss[row] = -expm1f(-l);
       if (t != a.ignore) {
         sum += double(l);
         ++count;
@@ -753,7 +787,20 @@ struct CoefArgs {
   int64_t ignore, classes, n;
   float* coef;
   float* gscale;
+  // split operands, for dx: the power of two of each row's dz, or null
+  float* rowscale;
+  const float2* stat;
+  const float* miss;
 };
+
+// |dz| of a row is at most |c| (1 - p of the target): the target's own, and the sum of all others'.
+// It goes to [2^12, 2^13), which leaves room for the roundings of the logits and of the loss (2^-24
+// of the row's largest logit m, in units of ln 2, and 2^-23), from which 1 - p comes.
+__device__ inline float row_scale(float c, float miss, float m) {
+  float top = fmaxf(miss, 0.f) + 0x1p-22f * (1.f + fabsf(m));
+  top = fabsf(c) * (top < 1.f ? top : 1.f);
+  return ldexpf(1.f, scale_exponent(top) - 2);
+}
 
 __device__ inline void coefficients(const CoefArgs& a) {
   __shared__ float red[1024];
@@ -792,6 +839,7 @@ __device__ inline void coefficients(const CoefArgs& a) {
       c = !(fabsf(g) < INFINITY) ? g : top == 0.f ? 0.f : g / top;
     }
     a.coef[i] = c;
+    if (a.rowscale) a.rowscale[i] = row_scale(c, a.miss[i], a.stat[i].x);
   }
 }
 
@@ -835,17 +883,20 @@ struct ProdArgs {
   void* out;           // dW: [m][n] elements; dx: fp32 slabs [split][m][n]
   int add;             // dx: add to the slab
   const float* gscale; // dW
-  const int* scale;    // split images: the exponent of b, or null
+  const int* scale;    // split operands: the exponent of b, or null
   float unscale;
   const float* bias;   // dW: rows of classes that are left out are zero
 };
+
+// the exponent of a power of two
+__device__ inline int exponent_of(float p) { return (__float_as_int(p) >> 23) - 127; }
 
 // dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
 // part to the same elements, so the order of the sums is fixed.  65536 classes of 8192 x 2048
 // bf16: 2.03 ms (1.08 PF/s); dW of them 2.07 ms (1.06 PF/s).
 template <typename T, int BM, int BN, int WAVES_M>
 __device__ void dx_tile(const ProdArgs& a, int block, char* lds) {
-  typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M> Tile;
+  typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M, false, gt_is_split<T>> Tile;
   const int t = xcd_tile(block, a.mtiles * a.ntiles * a.splits);
   const int sp = t / (a.mtiles * a.ntiles), u = t - sp * a.mtiles * a.ntiles;
   int mt, nt;
@@ -856,7 +907,6 @@ __device__ void dx_tile(const ProdArgs& a, int block, char* lds) {
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
   Tile::run(a.a, a.b, mt * BM, nt * BN, k0, k1, lds, acc);
-  const float per = gt_is_split<T> ? ldexpf(1.f, -*a.scale) : 1.f;
   const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
   float* out = static_cast<float*>(a.out) + (int64_t(sp) * a.m + i0) * a.n + j0;
 #pragma unroll
@@ -867,26 +917,31 @@ __device__ void dx_tile(const ProdArgs& a, int block, char* lds) {
       float* q = out + Tile::row_of(mi, 4 * g) * a.n;
       asm volatile("" : "+v"(q)::"memory");
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        const int64_t i = i0 + Tile::row_of(mi, 4 * g + e);
+        if (i >= a.m) continue;
+        int ex = 0;
+        if constexpr (gt_is_split<T>) ex = *a.scale + exponent_of(a.a.scale[i]);
 #pragma unroll
         for (int ni = 0; ni < Tile::NI; ++ni)
-          if (i0 + Tile::row_of(mi, 4 * g + e) < a.m && j0 + 32 * ni < a.n) {
+          if (j0 + 32 * ni < a.n) {
             float* o = q + e * a.n + 32 * ni;
-            const float v = gt_is_split<T> ? acc[mi][ni][4 * g + e] * per : acc[mi][ni][4 * g + e];
+            float v = acc[mi][ni][4 * g + e];
+            if constexpr (gt_is_split<T>) v = ldexpf(v, -ex);
             *o = a.add ? *o + v : v;
           }
+      }
     }
 }
 
 template <typename S, typename T, int BM, int BN, int WAVES_M>
 __device__ void dw_tile(const ProdArgs& a, int block, char* lds) {
-  typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M> Tile;
+  typedef GtTile<T, BM, kAcrossK, BN, kAcrossK, WAVES_M, false, gt_is_split<T>> Tile;
   int mt, nt;
   tile_at(xcd_tile(block, a.mtiles * a.ntiles), a.mtiles, a.ntiles, mt, nt);
   gt_f32x16 acc[Tile::MI][Tile::NI];
   Tile::clear(acc);
   Tile::run(a.a, a.b, mt * BM, nt * BN, 0, a.k, lds, acc);
-  const float per = gt_is_split<T> ? ldexpf(a.unscale, -*a.scale) : a.unscale;
   const float g = *a.gscale;
   S* out = static_cast<S*>(a.out);
   const int64_t i0 = int64_t(mt) * BM + Tile::row0(), j0 = nt * BN + Tile::col0();
@@ -897,10 +952,17 @@ __device__ void dw_tile(const ProdArgs& a, int block, char* lds) {
       const int64_t i = i0 + Tile::row_of(mi, e);
       if (i >= a.m) continue;
       const bool out_of = a.bias && a.bias[i] == -INFINITY;
+      int ex = 0;
+      if constexpr (gt_is_split<T>) ex = *a.scale + exponent_of(a.a.scale[i]);
 #pragma unroll
       for (int ni = 0; ni < Tile::NI; ++ni) {
         const int64_t j = j0 + 32 * ni;
-        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : acc[mi][ni][e] * per * g);
+        float v = acc[mi][ni][e];
+        if constexpr (gt_is_split<T>)
+          v = ldexpf(v, -ex);
+        else
+          v *= a.unscale;
+        if (j < a.n) out[i * a.n + j] = static_cast<S>(out_of ? 0.f : v * g);
       }
     }
 }
@@ -962,6 +1024,19 @@ __global__ __launch_bounds__(256) void oap_ce_finish(FinishArgs<T> a) {
     if (!(fabsf(scale) < INFINITY) && a.coef[i / a.dim] == 0.f) v = 0.f;
     a.dx[i] = static_cast<T>(v);
   }
+}
+
+// Split operands: the power of two that takes a class's largest |dz| of the piece to [2^14, 2^15)
+// (classes beyond the piece's end, which fill its last tiles: 1)
+__global__ __launch_bounds__(256) void oap_ce_class_scales(const float* __restrict__ dzmax,
+                                                           int rtiles, int64_t vp, int64_t classes,
+                                                           float* __restrict__ scale) {
+  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (v >= vp) return;
+  float m = 0.f;
+  if (v < classes)
+    for (int t = 0; t < rtiles; ++t) m = fmaxf(m, dzmax[int64_t(t) * vp + v]);
+  scale[v] = ldexpf(1.f, scale_exponent(m));
 }
 
 template <typename S>
@@ -1127,7 +1202,7 @@ struct Ce {
   struct Work {
     T *ximg, *ximg2, *wimg, *dz;
     float2* part;
-    float *zt, *coef, *gscale, *slab, *dbpart, *largest;
+    float *zt, *coef, *gscale, *slab, *dbpart, *largest, *dzmax, *classscale, *rowscale;
     int *scale, *rowexp;
   };
 
@@ -1222,17 +1297,22 @@ struct Ce {
     w.dz = c.take<T>(size_t(p.npad) * p.piece);
     w.slab = dx ? c.take<float>(size_t(p.splits) * a.n * a.dim) : nullptr;
     w.dbpart = db ? c.take<float>(size_t(p.npad / p.bn) * p.piece) : nullptr;
+    if (p.split && dw) {
+      w.dzmax = c.take<float>(size_t(p.npad / p.bn) * p.piece);
+      w.classscale = c.take<float>(p.piece);
+    }
+    w.rowscale = p.split && dx ? c.take<float>(a.n) : nullptr;
     return c.used;
   }
 
-  static void forward(const CeArgs& all, float* loss, float2* stat, float* total, bool mean,
-                      void* work, hipStream_t s) {
+  static void forward(const CeArgs& all, float* loss, float2* stat, float* miss, float* total,
+                      bool mean, void* work, hipStream_t s) {
     const Plan p = make_plan(all, false);
     Work w;
     carve_forward(all, p, work, w);
     if (few_rows(all)) {
       const int blocks = few(all, w, s);
-      rows(all, w, blocks, all.n, loss, stat, total, mean, s);
+      rows(all, w, blocks, all.n, loss, stat, nullptr, total, mean, s);
       return;
     }
     for (int64_t r0 = 0; r0 < all.n; r0 += p.rows) {
@@ -1242,7 +1322,7 @@ struct Ce {
       a.target = all.target + r0;
       forward_rows(a, p, w, s);
       rows(a, w, int(ceil_div(a.classes, p.bm)), p.npad, loss + r0, stat + r0,
-           p.rows == all.n ? total : nullptr, mean, s);
+           p.split ? miss + r0 : nullptr, p.rows == all.n ? total : nullptr, mean, s);
     }
     if (total && p.rows < all.n) sum_losses(all, loss, total, mean, s);
   }
@@ -1287,9 +1367,9 @@ struct Ce {
   // One workgroup for little work (the total needs no launch of its own then), else at least one
   // per CU.
   static void rows(const CeArgs& a, const Work& w, int tiles, int64_t npad, float* loss,
-                   float2* stat, float* total, bool mean, hipStream_t s) {
+                   float2* stat, float* miss, float* total, bool mean, hipStream_t s) {
     RowArgs r = {w.part, tiles, npad, a.n,  1,     a.target, a.ignore, a.classes,
-                 w.zt,   loss,  stat, total, mean};
+                 w.zt,   loss,  stat, miss, total, mean};
     const bool one = a.n * tiles <= 16384;
     while (r.cols < 64 && r.cols * (one ? 1 : 256) < a.n) r.cols *= 2;
     if (a.n >= 8) r.cols = std::max(r.cols, 8);
@@ -1352,8 +1432,9 @@ struct Ce {
   // dx's tiles and dW's; none where out is null
   template <int B, GradPart PART>
   static void grads_tile(const ProdArgs& x, const ProdArgs& w, hipStream_t s) {
-    constexpr int lds = std::max(GtTile<T, B, kAlongK, B, kAcrossK, 2>::kLds,
-                                 GtTile<T, B, kAcrossK, B, kAcrossK, 2>::kLds);
+    constexpr bool raw = gt_is_split<T>;
+    constexpr int lds = std::max(GtTile<T, B, kAlongK, B, kAcrossK, 2, false, raw>::kLds,
+                                 GtTile<T, B, kAcrossK, B, kAcrossK, 2, false, raw>::kLds);
     const int nx = x.out && PART != kDw ? x.mtiles * x.ntiles * x.splits : 0;
     const int nw = w.out && PART != kDx ? w.mtiles * w.ntiles : 0;
     if (nx + nw == 0) return;
@@ -1380,7 +1461,8 @@ struct Ce {
     gx.n = gw.n = a.dim;
     gx.gscale = gw.gscale = w.gscale;
     gx.unscale = gw.unscale = unscale;
-    gx.a = gw.a = {w.dz, p.piece, p.npad, p.piece};
+    gx.a = {w.dz, p.piece, a.n, p.piece, w.rowscale};
+    gw.a = {w.dz, p.piece, p.npad, p.piece, w.classscale};
     if (dx) {
       gx.b = l.w;
       gx.scale = w.scale + 1;
@@ -1412,16 +1494,16 @@ struct Ce {
     }
   }
 
-  static void backward(const CeArgs& a, const float2* stat, const float* grad, bool per_row,
-                       bool mean, void* dx, void* dw, float* db, void* work, hipStream_t s) {
+  static void backward(const CeArgs& a, const float2* stat, const float* miss, const float* grad,
+                       bool per_row, bool mean, void* dx, void* dw, float* db, void* work, hipStream_t s) {
     const Plan p = make_plan(a, true);
     Work w;
     carve_backward(a, p, work, dx, dw, db, w);
     const S* wt = static_cast<const S*>(a.w);
     // fp16 images hold dz times 2^14: |dz| <= 1 stays finite and 2^-28 is still a normal number
-    const float pscale = a.elem == Elem::F16 || p.split ? 0x1p14f : 1.f;
-    const CoefArgs coef = {grad, per_row, mean, a.target, a.ignore, a.classes, a.n, w.coef,
-                           w.gscale};
+    const float pscale = a.elem == Elem::F16 ? 0x1p14f : 1.f;
+    const CoefArgs coef = {grad,   per_row,  mean,       a.target, a.ignore, a.classes, a.n,
+                           w.coef, w.gscale, w.rowscale, stat,     miss};
     LogitArgs l = {};
     PackArgs<S> px = pack(a.x, a.ldx, a.n, a, p.dp, a.target, nullptr, w.ximg), pw = {};
     px.grad = per_row ? grad : nullptr;
@@ -1442,6 +1524,7 @@ struct Ce {
     l.dz = w.dz;
     l.vp = p.piece;
     l.dbpart = w.dbpart;
+    l.dzmax = w.dzmax;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
       const bool last = c0 + nc == a.classes;
@@ -1457,6 +1540,11 @@ struct Ce {
       l.class0 = c0;
       l.vtiles = int(ceil_div(nc, p.bm));
       logits<true>(p, l, s);
+      if (w.dzmax) {
+        oap_ce_class_scales<<<dim3(unsigned(p.piece / 256)), 256, 0, s>>>(
+            w.dzmax, l.ntiles, p.piece, nc, w.classscale);
+        OAP_HIP_CHECK(hipGetLastError());
+      }
       products(a, p, w, l, nc, c0, 1.f / pscale, dx, dw, s);
       FinishArgs<S> f = {};
       f.gscale = w.gscale;
@@ -1540,8 +1628,8 @@ size_t ce_forward_bytes(const CeArgs& a) {
   return r;
 }
 
-void ce_forward(const CeArgs& a, float* loss, float2* stat, float* total, bool mean, void* work,
-                hipStream_t s) {
+void ce_forward(const CeArgs& a, float* loss, float2* stat, float* miss, float* total, bool mean,
+                void* work, hipStream_t s) {
   check(a);
   if (a.n == 0) {  // no row: the sum and the mean are 0
     if (total) oap_ce_fill0<float><<<1, 256, 0, s>>>(total, 1);
@@ -1549,7 +1637,7 @@ void ce_forward(const CeArgs& a, float* loss, float2* stat, float* total, bool m
     return;
   }
   ce_dispatch(a, [&](auto t) {
-    decltype(t)::forward(a, loss, stat, total, mean, work, s);
+    decltype(t)::forward(a, loss, stat, miss, total, mean, work, s);
   });
 }
 
@@ -1565,14 +1653,15 @@ size_t ce_backward_bytes(const CeArgs& a, bool want_dx, bool want_dw, bool want_
   return r;
 }
 
-void ce_backward(const CeArgs& a, const float2* stat, const float* grad, bool per_row, bool mean,
-                 void* dx, void* dw, float* db, void* work, hipStream_t s) {
+void ce_backward(const CeArgs& a, const float2* stat, const float* miss, const float* grad,
+                 bool per_row, bool mean, void* dx, void* dw, float* db, void* work,
+                 hipStream_t s) {
   check(a);
   ce_dispatch(a, [&](auto t) {
     if (a.n == 0)
       decltype(t)::zeros(a, dx, dw, db, s);
     else
-      decltype(t)::backward(a, stat, grad, per_row, mean, dx, dw, db, work, s);
+      decltype(t)::backward(a, stat, miss, grad, per_row, mean, dx, dw, db, work, s);
   });
 }
 

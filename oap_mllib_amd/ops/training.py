@@ -95,9 +95,10 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         wr, ldw = _rows(weight)
         n, d = x.shape
         v = weight.shape[0]
-        # per row: max and sum for the gradients, and the loss
-        rows = torch.empty(3 * n, dtype=torch.float32, device=x.device)
-        stat, loss = rows, rows.data_ptr() + 8 * n
+        # per row: max and sum and 1 - p of the target for the gradients, and the loss
+        rows = torch.empty(4 * n, dtype=torch.float32, device=x.device)
+        stat = rows.data_ptr()
+        miss, loss = stat + 8 * n, stat + 12 * n
         out = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32,
                           device=x.device)
         total = 0
@@ -112,8 +113,8 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         if dev >= 0:
             work = _work(native.softmax_ce_forward_bytes(*head, n, v, d), x)
         native.softmax_ce_forward(dev, stream, *head, _ptr(target), ignore_index, n, v, d,
-                                  loss, _ptr(stat), total, reduction == "mean", _ptr(work))
-        ctx.save_for_backward(x, weight, bias, target, stat)
+                                  loss, stat, miss, total, reduction == "mean", _ptr(work))
+        ctx.save_for_backward(x, weight, bias, target, rows)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return out
 
@@ -121,7 +122,7 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
     @_first_order
     def backward(ctx, grad):
         native = _loader.load()
-        x, weight, bias, target, stat = ctx.saved_tensors
+        x, weight, bias, target, rows = ctx.saved_tensors
         xr, ldx = _rows(x)
         wr, ldw = _rows(weight)
         n, d = x.shape
@@ -138,9 +139,9 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         if dev >= 0:
             work = _work(native.softmax_ce_backward_bytes(*head, n, v, d, *want), x)
         native.softmax_ce_backward(dev, stream, *head, _ptr(target), ctx.ignore_index, n, v, d,
-                                   _ptr(stat), _ptr(grad), ctx.reduction == "none",
-                                   ctx.reduction == "mean", _ptr(dx), _ptr(dw), _ptr(db),
-                                   _ptr(work))
+                                   _ptr(rows), _ptr(rows) + 8 * n, _ptr(grad),
+                                   ctx.reduction == "none", ctx.reduction == "mean", _ptr(dx),
+                                   _ptr(dw), _ptr(db), _ptr(work))
         return dx, dw, db, None, None, None
 
 
@@ -162,8 +163,11 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
     (n losses; a row with the upstream gradient 0 takes no part in the gradients, whatever ``x``
     holds there).  Losses are float32, the gradients of ``x`` and ``weight`` have their type.
     Larger float32 problems form their products from 22 bits of every number (at least 2^-40 of its
-    row's largest in ``x``, of all classes' largest in ``weight``); there, and in float16, rows
-    whose upstream gradient is below 2^-15 of the largest lose bits of their gradient.
+    row's largest in ``x``, of all classes' largest in ``weight``; in the gradient of ``weight``
+    2^-40 of all rows' largest in ``x``).  In float16 the coefficients of the gradients, upstream
+    gradient times (probability - target), keep 11 bits down to 2^-28 of the largest upstream
+    gradient and nothing below 2^-39 of it, so unlikely classes of a large catalogue, and rows with
+    a small upstream gradient, lose bits of their gradient there.
     """
     _float_tensor("x", x, 2)
     _float_tensor("weight", weight, 2)

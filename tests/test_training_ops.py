@@ -1207,3 +1207,61 @@ def test_ce_rows_in_several_turns_gpu():
     ref[t[some] == -100] = 0
     zerr = (d + 8) * E32 * (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
     assert ((whole[some] - ref).abs() <= 2 * zerr + 499 * 3 * E32 + 4 * E32 * (ref.abs() + 20)).all()
+
+
+@pytest.mark.gpu
+def test_ce_fitted_rows_of_many_classes_gpu():
+    """Rows whose loss is 2e-3 to 1e-7 over a million classes: the other classes' probabilities,
+    down to 2^-43, keep their relative precision in dW, and their sum reaches dx."""
+    n, v, d, k = 130, 1_000_003, 12, 777
+    w = rand((v, d), 1, device="cuda", scale=0.3) + 1
+    w[:, 0] = 0
+    w[k] = 0
+    w[k, 0] = 1
+    x = rand((n, d), 2, device="cuda", scale=0.3)
+    x[:, 0] = torch.linspace(20, 30, n)
+    t = torch.full((n,), k, device="cuda")
+    for up in (None, 2.0 ** -torch.arange(n).remainder(9).float().cuda()):
+        leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+        rows = ops.softmax_cross_entropy(*leaves, t, reduction="none")
+        rows = rows if up is None else rows * up
+        dx, dw = torch.autograd.grad(rows.sum(), leaves)
+        x64, w64 = x.double(), w.double()
+        z = x64 @ w64.t()
+        lse = torch.logsumexp(z, 1)
+        zerr = (d + 8) * E32 * (x64.abs() @ w64.abs().t()).max().item() + 4 * E32 * lse.max().item()
+        p = (z - lse[:, None]).exp()
+        p[:, k] = 0  # the target's dz is minus the sum of the others
+        miss = p.sum(1)
+        if up is not None:
+            p *= up[:, None].double()
+        rel = 2 * zerr + 16 * E32
+        others = torch.arange(v, device="cuda") != k
+        want, mag = p.t() @ x64, p.t() @ x64.abs()
+        err = (dw.double() - want).abs()[others] / mag[others]
+        assert err.max() <= rel + (n + 8) * E32, err.max()
+        # dx beyond the first feature: the target's weights are 0 there
+        want, mag = p @ w64, p @ w64.abs()
+        err = (dx.double() - want).abs()[:, 1:] / mag[:, 1:]
+        assert err.max() <= rel + v * E32, err.max()
+        # ... and in the first, the target's alone: p - 1 in fp32
+        scale = 1.0 if up is None else up.double()
+        assert ((dx[:, 0].double() + miss * scale).abs()
+                <= scale * (miss * rel + 2 * zerr + 8 * E32)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+def test_ce_unlikely_classes_gpu(bias):
+    """Untrained rows over 300 thousand classes whose probabilities range over 2^-10 to 2^-50: each
+    class's row of dW has the relative precision of fp32 sums."""
+    n, v, d = 200, 300_007, 28
+    x, w = rand((n, d), 1, device="cuda"), rand((v, d), 2, device="cuda", scale=0.5)
+    t = torch.randint(0, 1000, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    b = None
+    if bias:
+        b = rand((v,), 4, device="cuda", scale=3.0)
+        b[t] = 1.0
+    ce_check(x, w, t, b, "sum")
+    ce_check(x, w, t, b, "none", torch.rand(n, generator=torch.Generator().manual_seed(5)).cuda()
+             + 0.5)

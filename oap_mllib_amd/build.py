@@ -65,8 +65,26 @@ def _obj(src: Path) -> Path:
     return BUILD / (str(rel).replace(os.sep, "__") + ".o")
 
 
-def _stale(src: Path, obj: Path) -> bool:
-    if not obj.exists():
+def _command(src: Path, debug: bool) -> list[str]:
+    obj = _obj(src)
+    cmd = [HIPCC] + _common_flags(debug) + _includes()
+    if src.suffix == ".hip":
+        cmd += ["-x", "hip", f"--offload-arch={ARCH}", "-munsafe-fp-atomics"] + NO_PACKED_FP32
+    else:
+        cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]
+        if "linalg" in src.parts:  # host fp64 dense kernels: x86-64-v3 (both hosts have it)
+            cmd += ["-mavx2", "-mfma", "-fopenmp-simd"]
+    return cmd + ["-MMD", "-MF", str(obj.with_suffix(".d")), "-c", str(src), "-o", str(obj)]
+
+
+def _stale(src: Path, debug: bool) -> bool:
+    """Whether the object is missing, older than what it was made from, or made by another
+    command (other flags, another architecture)."""
+    obj = _obj(src)
+    cmd = obj.with_suffix(".cmd")
+    if not obj.exists() or not cmd.exists():
+        return True
+    if cmd.read_text() != "\n".join(_command(src, debug)):
         return True
     ot = obj.stat().st_mtime
     dep = obj.with_suffix(".d")
@@ -91,17 +109,13 @@ def _common_flags(debug: bool) -> list[str]:
 
 def _compile(src: Path, debug: bool) -> tuple[Path, str]:
     obj = _obj(src)
-    cmd = [HIPCC] + _common_flags(debug) + _includes()
-    if src.suffix == ".hip":
-        cmd += ["-x", "hip", f"--offload-arch={ARCH}", "-munsafe-fp-atomics"] + NO_PACKED_FP32
-    else:
-        cmd += ["-x", "c++", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]
-        if "linalg" in src.parts:  # host fp64 dense kernels: x86-64-v3 (both hosts have it)
-            cmd += ["-mavx2", "-mfma", "-fopenmp-simd"]
-    cmd += ["-MMD", "-MF", str(obj.with_suffix(".d")), "-c", str(src), "-o", str(obj)]
+    cmd = _command(src, debug)
+    made_by = obj.with_suffix(".cmd")
+    made_by.unlink(missing_ok=True)  # (written again only when this compile has ended well)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {src}\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    made_by.write_text("\n".join(cmd))
     warn = "\n".join(w for w in r.stderr.splitlines() if "'-packed-fp32-ops'" not in w)
     return obj, warn
 
@@ -112,7 +126,7 @@ def build(jobs: int | None = None, clean: bool = False, debug: bool = False,
         shutil.rmtree(BUILD)
     BUILD.mkdir(parents=True, exist_ok=True)
     srcs = _sources()
-    todo = [s for s in srcs if _stale(s, _obj(s))]
+    todo = [s for s in srcs if _stale(s, debug)]
     jobs = jobs or min(8, os.cpu_count() or 4)
     if todo:
         if verbose:

@@ -5,14 +5,14 @@
 // tile; the backward pass goes over the classes in pieces, forms a piece's logits again,
 // stores its dz in the operand type and multiplies it into dx and dW while it is in cache.
 //
-// Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers.  A product
-// then keeps 22 bits of each: x and a piece's classes are copied into split images at powers of
-// two, every row of x at its own in the logits (a row is right whatever the others hold), a
-// piece's classes at one, and so the rows in dW: a number keeps an absolute 2^-40 of the largest
-// there.  dz is stored in fp32 and split as a tile of it is read, at a power of two per row for dx
-// (its largest magnitude is known, 1 - p of the target) and per class for dW (from maxima that the
-// logits' epilogue keeps): a probability of 2^-60 has its 22 bits where all of its sum are as
-// small.  At one scale for all, probabilities below 2^-24 lost bits and those below 2^-39 all.
+// Operands are bf16, fp16, fp32, or (larger fp32 problems) fp32 split in two fp16 numbers.  A
+// product then keeps 22 bits of each: x and a piece's classes are copied into split images at
+// powers of two, every row of x at its own in the logits (a row is right whatever the others
+// hold), a piece's classes at one, and so the rows in dW: a number keeps an absolute 2^-40 of the
+// largest there.  dz is stored in fp32 and split as a tile of it is read, at a power of two per row
+// for dx (its largest magnitude is known, 1 - p of the target) and per class for dW (from maxima
+// that the logits' epilogue keeps): a probability of 2^-60 has its 22 bits where all of its sum are
+// as small.  At one scale for all, probabilities below 2^-24 lost bits and those below 2^-39 all.
 //
 // Roundings: sums, statistics, losses and dx's slabs are fp32, and a result is rounded once.  With
 // 16-bit operands dz is rounded to their type (at most 2^-8 of it in bf16, 2^-11 in fp16) before
@@ -1495,7 +1495,8 @@ struct Ce {
   }
 
   static void backward(const CeArgs& a, const float2* stat, const float* miss, const float* grad,
-                       bool per_row, bool mean, void* dx, void* dw, float* db, void* work, hipStream_t s) {
+                       bool per_row, bool mean, void* dx, void* dw, float* db, void* work,
+                       hipStream_t s) {
     const Plan p = make_plan(a, true);
     Work w;
     carve_backward(a, p, work, dx, dw, db, w);

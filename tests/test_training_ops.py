@@ -1115,9 +1115,9 @@ def test_ce_upstream_gradients_that_are_no_numbers(device, dtype, bad):
 def ce_plan(x, w, b, grad):
     """(rows of a turn, classes of a piece, fp32 operands split) of a call"""
     elem = {torch.float32: "f32", torch.bfloat16: "bf16", torch.float16: "f16"}[x.dtype]
-    return _loader.load().softmax_ce_plan(elem, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0),
-                                          0 if b is None else b.data_ptr(), *x.shape[:1],
-                                          *w.shape, grad)
+    return _loader.load().softmax_ce_plan(elem, x.data_ptr(), x.stride(0), w.data_ptr(),
+                                          w.stride(0), 0 if b is None else b.data_ptr(),
+                                          *x.shape[:1], *w.shape, grad)
 
 
 @pytest.mark.gpu
@@ -1206,7 +1206,8 @@ def test_ce_rows_in_several_turns_gpu():
     ref = torch.logsumexp(z, 1) - z.gather(1, t[some].clamp(min=0)[:, None])[:, 0]
     ref[t[some] == -100] = 0
     zerr = (d + 8) * E32 * (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
-    assert ((whole[some] - ref).abs() <= 2 * zerr + 499 * 3 * E32 + 4 * E32 * (ref.abs() + 20)).all()
+    tol = 2 * zerr + 499 * 3 * E32 + 4 * E32 * (ref.abs() + 20)
+    assert ((whole[some] - ref).abs() <= tol).all()
 
 
 @pytest.mark.gpu

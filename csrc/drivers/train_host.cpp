@@ -22,7 +22,8 @@ namespace {
 constexpr double kInf = std::numeric_limits<double>::infinity();
 
 // One pool for the process; a pool runs one loop at a time.  The child of a fork has none of the
-// pool's threads and runs alone.
+// pool's threads and runs alone.  The pool is never taken down: a child that ends normally would
+// join threads that it does not have.
 void parallel(int64_t n, const std::function<void(int64_t, int64_t)>& f) {
   static const pid_t owner = getpid();
   if (getpid() != owner) {
@@ -30,7 +31,7 @@ void parallel(int64_t n, const std::function<void(int64_t, int64_t)>& f) {
     return;
   }
   static std::mutex mu;
-  static ThreadPool pool(
+  static ThreadPool& pool = *new ThreadPool(
       int(std::min<unsigned>(std::max(1u, std::thread::hardware_concurrency()), 16)));
   std::lock_guard<std::mutex> lock(mu);
   pool.parallel_for(n, [&](int, int64_t b, int64_t e) { f(b, e); });

@@ -1266,3 +1266,22 @@ def test_ce_unlikely_classes_gpu(bias):
     ce_check(x, w, t, b, "sum")
     ce_check(x, w, t, b, "none", torch.rand(n, generator=torch.Generator().manual_seed(5)).cuda()
              + 0.5)
+
+
+def test_host_engine_lets_a_forked_child_end():
+    """A child of a fork that ends normally (not by os._exit) takes down none of the parent's
+    threads."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = ("import os, sys, torch\n"
+            "from oap_mllib_amd import ops\n"
+            "x = torch.ones(4096)\n"
+            "ops.dropout(x, 0.5, 7)\n"
+            "pid = os.fork()\n"
+            "if pid == 0:\n"
+            "    ops.dropout(x, 0.5, 7)\n"
+            "    sys.exit(0)\n"
+            "sys.exit(os.waitpid(pid, 0)[1])\n")
+    root = Path(__file__).resolve().parent.parent
+    assert subprocess.run([sys.executable, "-c", code], timeout=60, cwd=root).returncode == 0

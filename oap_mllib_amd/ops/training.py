@@ -173,8 +173,8 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
     _float_tensor("weight", weight, 2)
     n, d = x.shape
     v = weight.shape[0]
-    if d < 1 or v < 1:
-        raise ValueError(f"softmax_cross_entropy: {d} features, {v} classes")
+    if not 1 <= d <= 1 << 20 or v < 1:
+        raise ValueError(f"softmax_cross_entropy: {d} features (1 to 2^20), {v} classes")
     _same("weight", weight, x, (v, d), x.dtype)
     _same("target", target, x, (n,))
     if target.dtype not in (torch.int64, torch.int32):
@@ -184,13 +184,16 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
         _same("bias", bias, x, (v,))
         if bias.dtype != torch.float32 or not bias.is_contiguous():
             bias = bias.float().contiguous()
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"ignore_index: expected a 64-bit integer, got {ignore_index}")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction: expected 'mean', 'sum' or 'none', got {reduction!r}")
     if target.dtype != torch.int64 or not target.is_contiguous():
         target = target.long().contiguous()
     if not x.is_cuda and x.dtype != torch.float32:
         x, weight = x.float(), weight.float()
-    return _SoftmaxCrossEntropy.apply(x, weight, bias, target, int(ignore_index), reduction)
+    return _SoftmaxCrossEntropy.apply(x, weight, bias, target, ignore_index, reduction)
 
 
 # ----------------------------------------------------------------------------------- dropout
@@ -244,7 +247,7 @@ def dropout(x, p: float, seed, *, offset: int = 0, residual=None):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"p: expected a probability, got {p}")
     offset = int(offset)
-    if offset < 0 or offset + x.numel() > 1 << 64:
+    if not 0 <= offset < 1 << 64 or offset + x.numel() > 1 << 64:
         raise ValueError(f"offset: element indices must lie in [0, 2^64), got offset {offset}")
     if isinstance(seed, torch.Tensor):
         _same("seed", seed, x, dtype=torch.int64)

@@ -1285,3 +1285,19 @@ def test_host_engine_lets_a_forked_child_end():
             "sys.exit(os.waitpid(pid, 0)[1])\n")
     root = Path(__file__).resolve().parent.parent
     assert subprocess.run([sys.executable, "-c", code], timeout=60, cwd=root).returncode == 0
+
+
+def test_numbers_beyond_64_bits_and_row_lengths_are_refused():
+    x, w, t = rand((4, 8), 1), rand((9, 8), 2), torch.zeros(4, dtype=torch.int64)
+    for bad in (1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            ops.softmax_cross_entropy(x, w, t, ignore_index=bad)
+    for fine in ((1 << 63) - 1, -(1 << 63)):
+        assert ops.softmax_cross_entropy(x, w, t, ignore_index=fine).isfinite()
+    long = torch.zeros(1, 1).expand(2, (1 << 20) + 1)
+    with pytest.raises(ValueError, match="features"):
+        ops.softmax_cross_entropy(long, long, t[:2])
+    for offset in (1 << 64, 1 << 70):  # (no element at all, but an index that is none)
+        with pytest.raises(ValueError, match="offset"):
+            ops.dropout(x[:0], 0.1, 1, offset=offset)
+    assert ops.dropout(x[:0], 0.1, 1, offset=(1 << 64) - 1).numel() == 0

@@ -255,7 +255,7 @@ struct LogitArgs {
   // statistics
   float2* part;        // [class tile][npad]: max, sum of exp(z - max)
   int64_t npad;
-  float* zt;           // [n] target's logit
+  float *zt, *ztlow;   // [n] target's logit, and what its rounding left out
   // gradient
   const float2* stat;  // [n] the row's (max, sum)
   const float* coef;   // [n] upstream gradient over its largest magnitude, 0: no loss
@@ -394,7 +394,13 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
             zt = hit ? acc[mi][ni][e] : zt;
             mine |= hit;
           }
-        if (mine) a.zt[n] = zt * unit;
+        // (the sums take the unrounded products to the rounded maximum: the loss of a row that its
+        // target decides is right only with the target's unrounded logit)
+        if (mine) {
+          const float z = zt * unit;
+          a.zt[n] = z;
+          a.ztlow[n] = __builtin_fmaf(zt, unit, -z);
+        }
       }
       const float mo = __shfl_xor(m, 32, 64), so = __shfl_xor(sum, 32, 64);
       const float mm = fmaxf(m, mo), mr = mm > -INFINITY ? mm : 0.f;
@@ -689,7 +695,7 @@ struct RowArgs {
   int cols;
   const int64_t* target;
   int64_t ignore, classes;
-  const float* zt;
+  const float *zt, *ztlow;  // (ztlow null: the sums are of rounded logits too)
   float* loss;
   float2* stat;
   float* miss;   // 1 - probability of the target, or null
@@ -751,8 +757,13 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(RowArgs a) {
         l = 0.f;
       else if (t < 0 || t >= a.classes)
         l = NAN;
-      else
-        l = a.zt[row] == -INFINITY ? INFINITY : kLn2 * (log2f(s) + (m - a.zt[row]));
+      else if (a.zt[row] == -INFINITY)
+        l = INFINITY;
+      else {
+        l = log2f(s) + (m - a.zt[row]);
+        if (a.ztlow) l -= a.ztlow[row];
+        l = l < 0.f ? 0.f : l * kLn2;  // (below 0 by roundings only)
+      }
       a.loss[row] = l;
       if (a.miss) a.miss[row] = -expm1f(-l);
       if (t != a.ignore) {
@@ -789,15 +800,14 @@ struct CoefArgs {
   float* gscale;
   // split operands, for dx: the power of two of each row's dz, or null
   float* rowscale;
-  const float2* stat;
   const float* miss;
 };
 
 // |dz| of a row is at most |c| (1 - p of the target): the target's own, and the sum of all others'.
-// It goes to [2^12, 2^13), which leaves room for the roundings of the logits and of the loss (2^-24
-// of the row's largest logit m, in units of ln 2, and 2^-23), from which 1 - p comes.
-__device__ inline float row_scale(float c, float miss, float m) {
-  float top = fmaxf(miss, 0.f) + 0x1p-22f * (1.f + fabsf(m));
+// It goes to [2^12, 2^13), which leaves room for the roundings of the logits and of the loss (2^-23
+// and what its sums lose beside a one), from which 1 - p comes.
+__device__ inline float row_scale(float c, float miss) {
+  float top = miss + 0x1p-20f;
   top = fabsf(c) * (top < 1.f ? top : 1.f);
   return ldexpf(1.f, scale_exponent(top) - 2);
 }
@@ -839,7 +849,7 @@ __device__ inline void coefficients(const CoefArgs& a) {
       c = !(fabsf(g) < INFINITY) ? g : top == 0.f ? 0.f : g / top;
     }
     a.coef[i] = c;
-    if (a.rowscale) a.rowscale[i] = row_scale(c, a.miss[i], a.stat[i].x);
+    if (a.rowscale) a.rowscale[i] = row_scale(c, a.miss[i]);
   }
 }
 
@@ -1202,7 +1212,7 @@ struct Ce {
   struct Work {
     T *ximg, *ximg2, *wimg, *dz;
     float2* part;
-    float *zt, *coef, *gscale, *slab, *dbpart, *largest, *dzmax, *classscale, *rowscale;
+    float *zt, *ztlow, *coef, *gscale, *slab, *dbpart, *largest, *dzmax, *classscale, *rowscale;
     int *scale, *rowexp;
   };
 
@@ -1276,6 +1286,7 @@ struct Ce {
     w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.part = c.take<float2>(size_t(ceil_div(a.classes, p.bm)) * p.npad);
     w.zt = c.take<float>(p.rows);
+    w.ztlow = c.take<float>(p.rows);
     w.largest = c.take<float>(2 * kMaxBlocks);
     w.scale = c.take<int>(2);
     w.rowexp = p.split ? c.take<int>(p.rows) : nullptr;
@@ -1346,6 +1357,7 @@ struct Ce {
     l.ntiles = int(ceil_div(a.n, p.bn));
     l.npad = p.npad;
     l.zt = w.zt;
+    l.ztlow = w.ztlow;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
       const float* bias = a.bias ? a.bias + c0 : nullptr;
@@ -1368,8 +1380,8 @@ struct Ce {
   // per CU.
   static void rows(const CeArgs& a, const Work& w, int tiles, int64_t npad, float* loss,
                    float2* stat, float* miss, float* total, bool mean, hipStream_t s) {
-    RowArgs r = {w.part, tiles, npad, a.n,  1,     a.target, a.ignore, a.classes,
-                 w.zt,   loss,  stat, miss, total, mean};
+    RowArgs r = {w.part, tiles,   npad, a.n,  1,    a.target, a.ignore, a.classes,
+                 w.zt,   w.ztlow, loss, stat, miss, total,    mean};
     const bool one = a.n * tiles <= 16384;
     while (r.cols < 64 && r.cols * (one ? 1 : 256) < a.n) r.cols *= 2;
     if (a.n >= 8) r.cols = std::max(r.cols, 8);
@@ -1504,7 +1516,7 @@ struct Ce {
     // fp16 images hold dz times 2^14: |dz| <= 1 stays finite and 2^-28 is still a normal number
     const float pscale = a.elem == Elem::F16 ? 0x1p14f : 1.f;
     const CoefArgs coef = {grad,   per_row,  mean,       a.target, a.ignore, a.classes, a.n,
-                           w.coef, w.gscale, w.rowscale, stat,     miss};
+                           w.coef, w.gscale, w.rowscale, miss};
     LogitArgs l = {};
     PackArgs<S> px = pack(a.x, a.ldx, a.n, a, p.dp, a.target, nullptr, w.ximg), pw = {};
     px.grad = per_row ? grad : nullptr;

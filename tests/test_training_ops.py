@@ -1301,3 +1301,29 @@ def test_numbers_beyond_64_bits_and_row_lengths_are_refused():
         with pytest.raises(ValueError, match="offset"):
             ops.dropout(x[:0], 0.1, 1, offset=offset)
     assert ops.dropout(x[:0], 0.1, 1, offset=(1 << 64) - 1).numel() == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ce_loss_of_rows_that_their_target_decides(device, dtype):
+    """Where all other logits lie at least 60 below the target's, the loss is 0 but for e^-60 per
+    class: never negative, and no larger for large logits (whose products are exact here: x and
+    weight hold small integers)."""
+    sizes = [(1, 1, 3), (4, 60, 24), (70, 300, 64)]
+    if device == "cuda":
+        sizes += [(7, 3000, 40), (20, 30_000, 24), (50, 30_000, 24), (300, 9000, 100),
+                  (160, 200_000, 48), (1100, 30_001, 40), (520, 9000, 1100)]
+    for n, v, d in sizes:
+        w = rand((v, d), 1).sign()
+        t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+        own = torch.arange(n) % 7 + 2  # the target's logit is own * d, the others' own * |sum| < it
+        x = w[t] * own[:, None]
+        z = x @ w.t()
+        gap = z.gather(1, t[:, None]) - z.scatter(1, t[:, None], -INF).amax(1, keepdim=True)
+        x = x * torch.ceil(60 / gap.clamp(min=1))
+        keep = gap[:, 0] >= 1  # (another class may have the same weights)
+        assert keep.any() and x.abs().max() < 1024
+        args = [q.to(dtype).to(device) for q in (x[keep], w)] + [t[keep].to(device)]
+        for b in (None, torch.zeros(v, device=device)):
+            loss = ops.softmax_cross_entropy(*args, b, reduction="none")
+            assert (loss >= 0).all() and (loss <= 2 * E32).all(), (n, v, d, loss.min(), loss.max())

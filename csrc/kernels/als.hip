@@ -443,10 +443,22 @@ __global__ __launch_bounds__(kAlsThreads, X3 ? 1 : 2) void oap_als_solve(SolveAr
       // sum the row's chunk partials in chunk order (deterministic)
       for (int64_t ch = a.chunk_ptr[q]; ch < a.chunk_ptr[q + 1]; ++ch) {
         const float* pp = a.partials + ch * partial_floats<NB>();
+        // (the loads of seven tiles in flight before the first sum: left to itself the compiler
+        // waits for every load in turn)
+        constexpr int kTiles = 7;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t0 = 0; t0 < NT; t0 += kTiles) {
+          f4 v[kTiles];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[t][e] += pp[t * 256 + e * 64 + lane];
+          for (int t = t0; t < NT && t < t0 + kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[t - t0][e] = pp[t * 256 + e * 64 + lane];
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int t = t0; t < NT && t < t0 + kTiles; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[t][e] += v[t - t0][e];
+        }
 #pragma unroll
         for (int f = 0; f < NB; ++f) bacc[f] += pp[NT * 256 + f * 64 + lane];
         nexp += static_cast<int>(pp[NT * 256 + NB * 64 + lane]);

@@ -170,9 +170,10 @@ void register_train(py::module_& m) {
   // workspace bytes (the addresses decide whether an operand is read in place)
   m.def("softmax_ce_forward_bytes",
         [](const std::string& elem, uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw,
-           uintptr_t bias, int64_t n, int64_t classes, int64_t dim) {
-          return kern::ce_forward_bytes(
-              ce_args(elem, x, ldx, w, ldw, bias, 0, 0, n, classes, dim));
+           uintptr_t bias, int64_t n, int64_t classes, int64_t dim, bool train) {
+          kern::CeArgs a = ce_args(elem, x, ldx, w, ldw, bias, 0, 0, n, classes, dim);
+          a.train = train;
+          return kern::ce_forward_bytes(a);
         });
   m.def("softmax_ce_backward_bytes",
         [](const std::string& elem, uintptr_t x, int64_t ldx, uintptr_t w, int64_t ldw,
@@ -193,10 +194,10 @@ void register_train(py::module_& m) {
   m.def("softmax_ce_forward",
         [](int device, uintptr_t stream, const std::string& elem, uintptr_t x, int64_t ldx,
            uintptr_t w, int64_t ldw, uintptr_t bias, uintptr_t target, int64_t ignore, int64_t n,
-           int64_t classes, int64_t dim, uintptr_t loss, uintptr_t stat, uintptr_t miss,
-           uintptr_t total, bool mean, uintptr_t work) {
-          const kern::CeArgs a =
-              ce_args(elem, x, ldx, w, ldw, bias, target, ignore, n, classes, dim);
+           int64_t classes, int64_t dim, bool train, uintptr_t loss, uintptr_t stat,
+           uintptr_t miss, uintptr_t total, bool mean, uintptr_t work) {
+          kern::CeArgs a = ce_args(elem, x, ldx, w, ldw, bias, target, ignore, n, classes, dim);
+          a.train = train;
           on(device, stream, a.elem,
              [&](hipStream_t s) {
                kern::ce_forward(a, at<float>(loss), at<float2>(stat), at<float>(miss),

@@ -23,6 +23,9 @@ struct CeArgs {
   int64_t ignore;         // rows with this target have no loss
   int64_t n, classes;
   int dim;
+  // forward: gradients will be asked for, whose pass has to see the same logits, to the last bit,
+  // as the one that forms the maxima (a row's probabilities are powers of their difference)
+  bool train;
 };
 
 // loss[i] = log sum_j exp(logit(i, j)) - logit(i, target[i]); stat[i] = the row's (max, sum of

@@ -416,13 +416,8 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float p = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref));
-          // (at most 1, also where huge logits round otherwise than in the forward pass: the
-          // split's scale relies on it)
-          if constexpr (gt_is_split<T>) p = __builtin_amdgcn_fmed3f(p, 0.f, 1.f);
-          acc[mi][ni][e] = p * cs;
-        }
+        for (int e = 0; e < 16; ++e)
+          acc[mi][ni][e] = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref)) * cs;
       if (__ballot(tgt >= 0)) {
         const int hit = tgt >= 0 && sbias[i0 + tgt] == -INFINITY ? -1 : tgt;
 #pragma unroll
@@ -804,8 +799,9 @@ struct CoefArgs {
 };
 
 // |dz| of a row is at most |c| (1 - p of the target): the target's own, and the sum of all others'.
-// It goes to [2^12, 2^13), which leaves room for the roundings of the logits and of the loss (2^-23
-// and what its sums lose beside a one), from which 1 - p comes.
+// It goes to [2^12, 2^13), which leaves room for the roundings of the loss, from which 1 - p comes
+// (2^-23 and what its sums lose beside a one), and of the logits, which differ between the passes
+// by what the scales of their pieces round (2^-40 of the largest weight).
 __device__ inline float row_scale(float c, float miss) {
   float top = miss + 0x1p-20f;
   top = fabsf(c) * (top < 1.f ? top : 1.f);
@@ -1171,10 +1167,12 @@ int few_width(const CeArgs& a) {
 
 // Whether oap_ce_few takes the call: the rows and features that its lane groups cover.  In 16 bits
 // the conversions weigh, and tiles are faster (4 x 400000 x 1000 bf16 179 against 281 us) unless
-// they need an image of classes that are not aligned (4 x 2M x 100 bf16 369 against 124 us).
+// they need an image of classes that are not aligned (4 x 2M x 100 bf16 369 against 124 us).  A
+// training call takes tiles, as its gradients do: the sums of the two run in another order, and
+// with logits of 1e7 their last bits are whole powers of e.
 bool few_rows(const CeArgs& a) {
   const int es = elem_size(a.elem);
-  if (a.n > kFewRows || a.dim > 64 * few_iters(int(a.n), es) * 16 / es) return false;
+  if (a.train || a.n > kFewRows || a.dim > 64 * few_iters(int(a.n), es) * 16 / es) return false;
   return es == 4 || a.n == 1 || (a.n <= 4 && few_width(a) < 16);
 }
 

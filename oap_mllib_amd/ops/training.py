@@ -89,7 +89,7 @@ def _work(nbytes: int, t):
 # --------------------------------------------------------------------- softmax cross entropy
 class _SoftmaxCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction, train):
         native = _loader.load()
         xr, ldx = _rows(x)
         wr, ldw = _rows(weight)
@@ -111,9 +111,10 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
         head = (elem, _ptr(xr), ldx, _ptr(wr), ldw, _ptr(bias))
         work = None
         if dev >= 0:
-            work = _work(native.softmax_ce_forward_bytes(*head, n, v, d), x)
+            work = _work(native.softmax_ce_forward_bytes(*head, n, v, d, train), x)
         native.softmax_ce_forward(dev, stream, *head, _ptr(target), ignore_index, n, v, d,
-                                  loss, stat, miss, total, reduction == "mean", _ptr(work))
+                                  train, loss, stat, miss, total, reduction == "mean",
+                                  _ptr(work))
         ctx.save_for_backward(x, weight, bias, target, rows)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return out
@@ -142,7 +143,7 @@ class _SoftmaxCrossEntropy(torch.autograd.Function):
                                    _ptr(rows), _ptr(rows) + 8 * n, _ptr(grad),
                                    ctx.reduction == "none", ctx.reduction == "mean", _ptr(dx),
                                    _ptr(dw), _ptr(db), _ptr(work))
-        return dx, dw, db, None, None, None
+        return dx, dw, db, None, None, None, None
 
 
 def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -100,
@@ -193,7 +194,9 @@ def softmax_cross_entropy(x, weight, target, bias=None, *, ignore_index: int = -
         target = target.long().contiguous()
     if not x.is_cuda and x.dtype != torch.float32:
         x, weight = x.float(), weight.float()
-    return _SoftmaxCrossEntropy.apply(x, weight, bias, target, ignore_index, reduction)
+    train = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias))
+    return _SoftmaxCrossEntropy.apply(x, weight, bias, target, ignore_index, reduction, train)
 
 
 # ----------------------------------------------------------------------------------- dropout

@@ -1327,3 +1327,47 @@ def test_ce_loss_of_rows_that_their_target_decides(device, dtype):
         for b in (None, torch.zeros(v, device=device)):
             loss = ops.softmax_cross_entropy(*args, b, reduction="none")
             assert (loss >= 0).all() and (loss <= 2 * E32).all(), (n, v, d, loss.min(), loss.max())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [10.0, 1000.0])
+def test_ce_gradients_of_large_logits(device, dtype, scale):
+    """Logits of 1e4 to 1e8, whose fp32 sums are off by much more than one: another class lies far
+    above the target, so its probability is 1 and its dz the upstream gradient, the target's is
+    minus that and all others' are 0.  The pass that forms the maxima has to see the same logits
+    as the one that forms the gradients."""
+    sizes = [(1, 50, 100), (1, 50, 1000), (4, 60, 101), (7, 90, 100), (70, 300, 64)]
+    if device == "cuda":
+        sizes += [(8, 30_000, 100), (20, 30_000, 100), (300, 15_000, 400), (520, 9000, 1100)]
+    for n, v, d in sizes:
+        x, w = rand((20 * n, d), 1, dtype, device, scale), rand((v, d), 2, dtype, device, scale)
+        z = x.double() @ w.double().t()
+        top2 = z.topk(2, dim=1)
+        # (sums of d products in any order: d 2^-23 of the sum of their magnitudes)
+        error = d * E32 * (x.double().abs() @ w.double().abs().t()).amax(1)
+        gap = top2.values[:, 0] - top2.values[:, 1]
+        rows = (gap > 2 * error + 100).nonzero()[:n, 0]
+        assert len(rows) == n
+        x, best, t = x[rows], top2.indices[rows, 0], z[rows].argmin(1)
+        for b in (None, torch.zeros(v, device=device, requires_grad=True)):
+            leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+            leaves += [b] if b is not None else []
+            loss = ops.softmax_cross_entropy(leaves[0], leaves[1], t, b, reduction="none")
+            grads = torch.autograd.grad(loss, leaves, torch.ones_like(loss))
+            xr, u = x.double(), half_step(dtype)
+            want = [w.double()[best] - w.double()[t],
+                    torch.zeros(v, d, device=device).double()
+                    .index_add_(0, best, xr).index_add_(0, t, -xr)]
+            mags = [w.double()[best].abs() + w.double()[t].abs(),
+                    torch.zeros(v, d, device=device).double()
+                    .index_add_(0, best, xr.abs()).index_add_(0, t, xr.abs())]
+            for got, ref, mag in zip(grads, want, mags):
+                err = (got.double() - ref).abs() - (n + 8) * E32 * mag \
+                    - u * ref.abs() - 1e-37  # (the others' e^-100)
+                assert (err <= 0).all(), (n, v, d, err.max())
+            if b is not None:
+                count = torch.zeros(v, device=device).double()
+                one = torch.ones(n, device=device).double()
+                count.index_add_(0, best, one).index_add_(0, t, -one)
+                assert ((grads[2].double() - count).abs() <= (n + 8) * E32 * n).all()

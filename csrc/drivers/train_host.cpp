@@ -185,7 +185,8 @@ double ce_logit(const kern::CeArgs& a, int64_t i, int64_t j) {
   const float* w = static_cast<const float*>(a.w) + j * a.ldw;
   double z = a.bias ? double(a.bias[j]) : 0.0;
   for (int k = 0; k < a.dim; ++k) z += double(x[k]) * w[k];
-  return z;
+  // (a sum refers to the maximum as it is kept, in fp32: their difference stays in range)
+  return std::fabs(z) > 0x1p28 ? double(float(z)) : z;
 }
 
 bool has_loss(const kern::CeArgs& a, int64_t i) {

@@ -255,7 +255,7 @@ struct LogitArgs {
   // statistics
   float2* part;        // [class tile][npad]: max, sum of exp(z - max)
   int64_t npad;
-  float *zt, *ztlow;   // [n] target's logit, and what its rounding left out
+  float* zt;           // [n] target's logit
   // gradient
   const float2* stat;  // [n] the row's (max, sum)
   const float* coef;   // [n] upstream gradient over its largest magnitude, 0: no loss
@@ -298,6 +298,7 @@ struct Store<GtSplit> {
 // (1.13 PF/s), 2.23 ms for each half of the classes with their dz (0.98 PF/s, 1 GiB written).
 template <typename T, int BM, int BN, int WAVES_M, bool SINGLE, bool GRAD>
 __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logits(LogitArgs a) {
+#pragma clang fp contract(off)
   typedef GtTile<T, BM, kAlongK, BN, kAlongK, WAVES_M, SINGLE> Tile;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float sbias[BM];
@@ -359,8 +360,9 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
         for (int ni = 0; ni < Tile::NI; ++ni) acc[mi][ni][e] = out ? -INFINITY : acc[mi][ni][e];
       }
   }
-  // acc: the logits in units of ln 2, or (plain) the sums; one multiply-add takes either to its
-  // distance from a row's maximum
+  // acc: the logits in units of ln 2, or (plain) the sums, which a factor takes there.  The product
+  // is rounded before a maximum is taken off: in one multiply-add, logits of 1e4 to 1e9 would lie
+  // 2^-11 to 2^6 off their own maximum, larger ones beyond the range of a power.
 #pragma unroll
   for (int ni = 0; ni < Tile::NI; ++ni) {
     const int j = j0 + 32 * ni;
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 #pragma unroll
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref));
+        for (int e = 0; e < 16; ++e) sum += pow2(acc[mi][ni][e] * unit - ref);
       if (__ballot(tgt >= 0)) {
         float zt = 0.f;
         bool mine = false;
@@ -394,13 +396,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
             zt = hit ? acc[mi][ni][e] : zt;
             mine |= hit;
           }
-        // (the sums take the unrounded products to the rounded maximum: the loss of a row that its
-        // target decides is right only with the target's unrounded logit)
-        if (mine) {
-          const float z = zt * unit;
-          a.zt[n] = z;
-          a.ztlow[n] = __builtin_fmaf(zt, unit, -z);
-        }
+        if (mine) a.zt[n] = zt * unit;
       }
       const float mo = __shfl_xor(m, 32, 64), so = __shfl_xor(sum, 32, 64);
       const float mm = fmaxf(m, mo), mr = mm > -INFINITY ? mm : 0.f;
@@ -417,7 +413,7 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
       for (int mi = 0; mi < Tile::MI; ++mi)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          acc[mi][ni][e] = pow2(__builtin_fmaf(acc[mi][ni][e], unit, -ref)) * cs;
+          acc[mi][ni][e] = pow2(acc[mi][ni][e] * unit - ref) * cs;
       if (__ballot(tgt >= 0)) {
         const int hit = tgt >= 0 && sbias[i0 + tgt] == -INFINITY ? -1 : tgt;
 #pragma unroll
@@ -690,7 +686,7 @@ struct RowArgs {
   int cols;
   const int64_t* target;
   int64_t ignore, classes;
-  const float *zt, *ztlow;  // (ztlow null: the sums are of rounded logits too)
+  const float* zt;
   float* loss;
   float2* stat;
   float* miss;   // 1 - probability of the target, or null
@@ -756,7 +752,6 @@ __global__ __launch_bounds__(1024) void oap_ce_rows(RowArgs a) {
         l = INFINITY;
       else {
         l = log2f(s) + (m - a.zt[row]);
-        if (a.ztlow) l -= a.ztlow[row];
         l = l < 0.f ? 0.f : l * kLn2;  // (below 0 by roundings only)
       }
       a.loss[row] = l;
@@ -1210,7 +1205,7 @@ struct Ce {
   struct Work {
     T *ximg, *ximg2, *wimg, *dz;
     float2* part;
-    float *zt, *ztlow, *coef, *gscale, *slab, *dbpart, *largest, *dzmax, *classscale, *rowscale;
+    float *zt, *coef, *gscale, *slab, *dbpart, *largest, *dzmax, *classscale, *rowscale;
     int *scale, *rowexp;
   };
 
@@ -1284,7 +1279,6 @@ struct Ce {
     w.wimg = p.w_direct ? nullptr : c.take<T>(size_t(std::min(p.piece, a.classes)) * p.dp);
     w.part = c.take<float2>(size_t(ceil_div(a.classes, p.bm)) * p.npad);
     w.zt = c.take<float>(p.rows);
-    w.ztlow = c.take<float>(p.rows);
     w.largest = c.take<float>(2 * kMaxBlocks);
     w.scale = c.take<int>(2);
     w.rowexp = p.split ? c.take<int>(p.rows) : nullptr;
@@ -1355,7 +1349,6 @@ struct Ce {
     l.ntiles = int(ceil_div(a.n, p.bn));
     l.npad = p.npad;
     l.zt = w.zt;
-    l.ztlow = w.ztlow;
     for (int64_t c0 = 0; c0 < a.classes; c0 += p.piece) {
       const int64_t nc = std::min(p.piece, a.classes - c0);
       const float* bias = a.bias ? a.bias + c0 : nullptr;
@@ -1378,8 +1371,8 @@ struct Ce {
   // per CU.
   static void rows(const CeArgs& a, const Work& w, int tiles, int64_t npad, float* loss,
                    float2* stat, float* miss, float* total, bool mean, hipStream_t s) {
-    RowArgs r = {w.part, tiles,   npad, a.n,  1,    a.target, a.ignore, a.classes,
-                 w.zt,   w.ztlow, loss, stat, miss, total,    mean};
+    RowArgs r = {w.part, tiles, npad, a.n,  1,     a.target, a.ignore, a.classes,
+                 w.zt,   loss,  stat, miss, total, mean};
     const bool one = a.n * tiles <= 16384;
     while (r.cols < 64 && r.cols * (one ? 1 : 256) < a.n) r.cols *= 2;
     if (a.n >= 8) r.cols = std::max(r.cols, 8);

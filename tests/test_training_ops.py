@@ -1371,3 +1371,19 @@ def test_ce_gradients_of_large_logits(device, dtype, scale):
                 one = torch.ones(n, device=device).double()
                 count.index_add_(0, best, one).index_add_(0, t, -one)
                 assert ((grads[2].double() - count).abs() <= (n + 8) * E32 * n).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [1e5, 1e9, 1e15])
+def test_ce_gradients_of_huge_logits(device, dtype, scale):
+    """The same at logits of 1e11 to 1e31, where the rounding of a maximum alone passes the range
+    of a power."""
+    test_ce_gradients_of_large_logits(device, dtype, scale)
+    x, w = rand((70, 64), 1, dtype, device, scale), rand((300, 64), 2, dtype, device, scale)
+    t = torch.arange(70, device=device)
+    loss = ops.softmax_cross_entropy(x, w, t, reduction="none")
+    z = x.double() @ w.double().t()
+    want = z.amax(1) - z[torch.arange(70, device=device), t]
+    error = 64 * E32 * (x.double().abs() @ w.double().abs().t()).amax(1)
+    assert ((loss.double() - want).abs() <= 2 * error + 4 * E32 * want + math.log(300)).all()

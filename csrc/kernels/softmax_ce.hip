@@ -19,10 +19,10 @@
 // it meets W and x, whose own rounding is as large: that is what the matrix units take, and dz in
 // two parts would double the work of dX and dW.  db sums dz in fp32 before that rounding.
 //
-// What bounds it, at 8192 x 131072 x 2048 bf16 (16.6 ms for forward and gradients, 8 N V D
-// operations): the matrix units under the chip's power limit, 1.06 to 1.13 PF/s in each product
-// (a library product of the same shapes 1.23).  At 1024 x 2M x 100 fp32 (10.4 ms): k is short, so
-// each tile's epilogue and staging weigh as much as its MFMAs (21% busy), and dz, written once and
+// What bounds it, at 8192 x 131072 x 2048 bf16 (16.7 to 17.1 ms by card for forward and gradients, 8
+// N V D operations): the matrix units under the chip's power limit, 0.98 to 1.10 PF/s in each
+// product (a library product of the same shapes 1.23).  At 1024 x 2M x 100 fp32 (11.1 ms): k is
+// short, so each tile's epilogue and staging weigh as much as its MFMAs, and dz, written once and
 // read twice, is 26 GB.
 #include "kernels/softmax_ce.h"
 
@@ -294,8 +294,8 @@ struct Store<GtSplit> {
 };
 
 // One tile of logits, classes down (in registers) and rows across (lanes): a row's reduction
-// over the tile's classes is mostly within the lane.  8192 x 131072 x 2048 bf16: 3.9 ms forward
-// (1.13 PF/s), 2.23 ms for each half of the classes with their dz (0.98 PF/s, 1 GiB written).
+// over the tile's classes is mostly within the lane.  8192 x 131072 x 2048 bf16: 4.0 ms forward
+// (1.10 PF/s), 2.26 ms for each half of the classes with their dz (0.98 PF/s, 1 GiB written).
 template <typename T, int BM, int BN, int WAVES_M, bool SINGLE, bool GRAD>
 __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logits(LogitArgs a) {
 #pragma clang fp contract(off)
@@ -532,8 +532,9 @@ __global__ __launch_bounds__(kGtThreads, gt_occupancy(BM, BN)) void oap_ce_logit
 // of x stay in registers.  The sums over the lanes are formed so that a lane ends with the logit of
 // one row (as many rows at once as there are), and keeps that row's (max, sum) over the group's
 // classes; the workgroup joins them.
-// 2M x 100 fp32: one row 135 us (5.9 TB/s), four 140, eight 166 (tiles: 237 and 260); 8-byte loads
-// 202, single elements (101 features) 206 us; one row in bf16, 8-byte loads, 123 us.
+// 2M x 100 fp32: one row 130 us (6.1 TB/s), four 140, eight 166 (tiles: 237 and 260); 8-byte loads
+// 202, single elements (101 features) 206 us.  One row in bf16, 8-byte loads: 118 us, 3.4 TB/s:
+// half the bytes in as many loads, with twice the conversions in each.
 struct FewArgs {
   const void *w, *x;
   int64_t ldw, ldx, classes;
@@ -894,7 +895,7 @@ __device__ inline int exponent_of(float p) { return (__float_as_int(p) >> 23) - 
 
 // dx: a slab per split of k (classes of the piece); the same workgroup adds the next piece's
 // part to the same elements, so the order of the sums is fixed.  65536 classes of 8192 x 2048
-// bf16: 2.03 ms (1.08 PF/s); dW of them 2.07 ms (1.06 PF/s).
+// bf16: 2.12 ms (1.04 PF/s); dW of them 2.13 ms (1.03 PF/s).
 template <typename T, int BM, int BN, int WAVES_M>
 __device__ void dx_tile(const ProdArgs& a, int block, char* lds) {
   typedef GtTile<T, BM, kAlongK, BN, kAcrossK, WAVES_M, false, gt_is_split<T>> Tile;
@@ -1069,15 +1070,15 @@ bool direct(const CeArgs& a, const void* p, int64_t ld) {
 
 // Of one dz image or one class image.  Smaller pieces stay in the last-level cache, but their
 // products fill the chip less evenly and dx's slabs are added to more often: 2^28, 2^29, 2^30, 2^31
-// took 18.2, 17.3, 16.9, 17.0 ms at 8192 x 131072 x 2048 bf16 and 11.5, 11.6, 10.7, 10.9 ms at
+// take 18.2, 17.2, 17.0, 17.1 ms at 8192 x 131072 x 2048 bf16 and 12.2, 11.8, 11.0, 11.1 ms at
 // 1024 x 2M x 100 fp32.
 constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
 // fp32 problems of more than 128 rows and at least this many products take the split operands:
-// their images cost two launches and two passes over the weights (1024 x 20000 x 128: 181 against
-// 259 us with gradients, 2048 x 20000 x 1000 1.09 against 2.45 ms; 300 x 5000 x 512 147 against
-// 130 us, 200 x 20000 x 300 without gradients 52 against 47 us; 192 x 1M x 100 1.78 against 2.14
-// ms, but 128 x 1M x 100, one row tile, 1.54 against 1.38 ms, without gradients 420 against 309).
+// their images cost two launches and two passes over the weights (1024 x 20000 x 128: 182 against
+// 250 us with gradients, 2048 x 20000 x 1000 1.18 against 2.44 ms; 300 x 5000 x 512 146 against
+// 134 us, 200 x 20000 x 300 without gradients 49 against 50 us; 192 x 1M x 100 1.89 against 2.15
+// ms, but 128 x 1M x 100, one row tile, 1.61 against 1.38 ms, without gradients 422 against 292).
 constexpr double kSplitWork = 1.5e9;
 
 // Tiles of 128 x 128, two or more of which share a CU, or of 256 x 256: one's epilogue overlaps
@@ -1115,8 +1116,8 @@ Plan make_plan(const CeArgs& a, bool grad) {
     p.bm = 256;
   // One buffer lets a third workgroup share the CU.  16 bits gain at every k that takes this tile
   // (4096 x 200000 x 128 1.82 against 1.99 ms, 4096 x 65536 x 512 1.38 against 1.42 ms), split
-  // operands while k is short (1024 x 2M x 100 10.6 against 11.7 ms; 2048 x 20000 x 1000 1.10
-  // against 1.09 ms).  fp32 keeps two: that loop skips the empty steps of a short k.
+  // operands while k is short (1024 x 2M x 100 11.0 against 11.9 ms; nothing is gained at 2048 x
+  // 20000 x 1000).  fp32 keeps two: that loop skips the empty steps of a short k.
   p.single = es == 2 || (p.split && p.dp <= 512);
   // few rows of many classes (16 x 2M x 100 fp32 in tiles of 32 rows 260 us, of 64 390 us; one
   // buffer for those of 64, 377 against 394 us, two for those of 32, 188 against 201 us for 8 x

@@ -13,12 +13,12 @@
 // lists of four; a round is the maximum of the list heads, of the lanes (DPP), and a shift of one
 // list.  16-bit logits leave room for the whole index in the unused bits, so the keys decide
 // exactly.  Otherwise two neighbours in the order may be closer than the key's last bit, or than
-// the fp32 error of c: such a token (about one in a thousand of random fp32 logits) is decided again
-// from values in 64 bits.  In 32 bits alone two experts' scores would round to the same or the other
-// order that often.  262144 x 128 fp32, eight chosen: 55 us forward (the read alone takes 26 us).
-// Equal choice values are always in doubt, one token of a wave after the other: the same gate with
-// all logits equal takes 545 us, and 8192 x 256 bf16 with groups 66 us where a bias of zeros leaves
-// the ties of 16-bit logits (32 us with a random bias).
+// the fp32 error of c: such a token (about one in a thousand of random fp32 logits) is decided
+// again from values in 64 bits.  In 32 bits alone two experts' scores would round to the same or
+// the other order that often.  262144 x 128 fp32, eight chosen: 55 us forward (the read alone takes
+// 26 us).  Equal choice values are always in doubt, one token of a wave after the other: the same
+// gate with all logits equal takes 545 us, and 8192 x 256 bf16 with groups 66 us where a bias of
+// zeros leaves the ties of 16-bit logits (32 us with a random bias).
 #include "kernels/route.h"
 
 #include <algorithm>
@@ -499,8 +499,9 @@ __global__ __launch_bounds__(16 * kCountLanes) void oap_route_counts(
 //   sigmoid                dz_c = w_c (1 - s_c) g_c
 //   softmax                dz_i = s_i (scale [i in C] g_i - sum_C g w), all experts
 // One workgroup forms the rows of a few tokens in LDS (zeros, then the chosen) and writes them
-// out in order.  262144 x 128 fp32: 45 us, 3.0 TB/s written, little more than half of a copy's rate:
-// the zeros, the chosen (a thread per token) and the write follow each other with a barrier between.
+// out in order.  262144 x 128 fp32: 45 us, 3.0 TB/s written, little more than half of a copy's
+// rate: the zeros, the chosen (a thread per token) and the write follow each other with a barrier
+// between.
 // The plain softmax reads its logits three times and writes single elements: 183 us.
 constexpr int kGradTile = 8192;  // floats of LDS
 

@@ -19,8 +19,8 @@
 // it meets W and x, whose own rounding is as large: that is what the matrix units take, and dz in
 // two parts would double the work of dX and dW.  db sums dz in fp32 before that rounding.
 //
-// What bounds it, at 8192 x 131072 x 2048 bf16 (16.7 to 17.1 ms by card for forward and gradients, 8
-// N V D operations): the matrix units under the chip's power limit, 0.98 to 1.10 PF/s in each
+// What bounds it, at 8192 x 131072 x 2048 bf16 (16.7 to 17.1 ms by card for forward and gradients,
+// 8 N V D operations): the matrix units under the chip's power limit, 0.98 to 1.10 PF/s in each
 // product (a library product of the same shapes 1.23).  At 1024 x 2M x 100 fp32 (11.1 ms): k is
 // short, so each tile's epilogue and staging weigh as much as its MFMAs, and dz, written once and
 // read twice, is 26 GB.

@@ -1387,3 +1387,78 @@ def test_ce_gradients_of_huge_logits(device, dtype, scale):
     want = z.amax(1) - z[torch.arange(70, device=device), t]
     error = 64 * E32 * (x.double().abs() @ w.double().abs().t()).amax(1)
     assert ((loss.double() - want).abs() <= 2 * error + 4 * E32 * want + math.log(300)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,v,d", [(5, 5000, 100), (6, 3000, 1032), (7, 33, 40), (8, 999, 1024),
+                                   (8, 30_000, 64), (5, 7, 8), (2, 2000, 200), (8, 1, 4),
+                                   (3, 4000, 512), (1, 3000, 2048), (4, 70, 1000)])
+def test_ce_losses_of_few_rows_gpu(dtype, n, v, d):
+    """Losses whose gradients nobody asks for: up to eight rows at once from registers."""
+    x, w = rand((n, d), 1, dtype, "cuda", 0.5), rand((v, d), 2, dtype, "cuda", 0.5)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3))
+    b = rand((v,), 4)
+    b[1::7] = -INF
+    b[t] = 0.5
+    b = b.cuda()
+    none = (False, False, False)
+    for bias in (None, b):
+        ce_check(x, w, t.cuda(), bias, reduction="none", want=none)
+    with torch.no_grad():  # (the same without a graph, whatever wants gradients)
+        leaf = w.clone().requires_grad_()
+        a = ops.softmax_cross_entropy(x, leaf, t.cuda(), b, reduction="none")
+        assert torch.equal(a, ops.softmax_cross_entropy(x, w, t.cuda(), b, reduction="none"))
+    t[n // 2] = -100
+    x[n // 2] = math.nan
+    w[b == -INF] = math.nan
+    ce_check(x, w, t.cuda(), b, want=none)
+
+
+@pytest.mark.gpu
+def test_ce_few_rows_beyond_32_bits():
+    """One row without gradients, weights of more than 2^31 elements."""
+    v, d, tail = 1_200_000, 2000, 300
+    w = torch.zeros(v, d, dtype=torch.bfloat16, device="cuda")
+    w[-tail:] = rand((tail, d), 1, torch.bfloat16, "cuda")
+    x = rand((1, d), 2, torch.bfloat16, "cuda", 0.2)
+    t = torch.tensor([v - 7], device="cuda")
+    z = cpu64(x) @ cpu64(w[-tail:]).t()
+    lse = torch.logsumexp(torch.cat([z, torch.full((1, 1), math.log(v - tail))], 1), 1)
+    zerr = 2 * (d + 10) * E32 * (cpu64(x).abs() @ cpu64(w[-tail:]).abs().t()).max().item()
+    check(ops.softmax_cross_entropy(x, w, t, reduction="none"), lse - z[:, tail - 7],
+          zerr + 4 * E32 * (lse.abs().max() + 1), "loss")
+
+
+@pytest.mark.gpu
+def test_ce_split_rows_in_several_turns_gpu():
+    """fp32 rows in two turns, classes in many pieces; losses and dx of rows on both sides of the
+    border against 64 bits, some of them with losses of 1e-3 to 1e-6."""
+    n, v, d = 9000, 2_000_000, 4
+    x, w = rand((n, d), 1, device="cuda"), rand((v, d), 2, device="cuda", scale=0.5)
+    t = torch.randint(0, v, (n,), generator=torch.Generator().manual_seed(3)).cuda()
+    w[:, 0] = 0
+    w[77] = 0
+    w[77, 0] = 1
+    rows, classes, split = ce_plan(x, w, None, False)
+    assert rows < n and split and ce_plan(x, w, None, True)[1] * 2 < v
+    some = torch.tensor([0, 1, rows - 2, rows - 1, rows, rows + 1, n - 1], device="cuda")
+    x[some, 0] = torch.tensor([3.0, 22.0, 25.0, 28.0, 28.0, 25.0, 22.0], device="cuda")
+    t[some] = 77
+    leaf = x.clone().requires_grad_()
+    loss = ops.softmax_cross_entropy(leaf, w, t, reduction="none")
+    dx, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+    w64 = w.double()
+    z = x[some].double() @ w64.t()
+    lse = torch.logsumexp(z, 1)
+    zerr = (d + 8) * E32 * (x[some].double().norm(dim=1).max() * w64.norm(dim=1).max()).item() \
+        + 4 * E32 * lse.abs().max().item()
+    # (15625 tiles of 128 classes: up to 977 joins in a row by a thread, three roundings each)
+    ref = lse - z[:, 77]
+    tol = 2 * zerr + 1000 * 3 * E32 + 4 * E32 * (ref.abs() + 20)
+    assert ((loss[some].double() - ref).abs() <= tol).all()
+    p = (z - lse[:, None]).exp()
+    p[:, 77] = 0
+    want, mag = p @ w64, p @ w64.abs()
+    err = (dx[some].double() - want).abs()[:, 1:] / mag[:, 1:]
+    assert (err <= 2 * zerr + 16 * E32 + 4000 * E32).all()
